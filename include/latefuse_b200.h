@@ -433,6 +433,33 @@ int lf_linear_lora_shrink(void* stream, int dtype, const void* x, int64_t ldx, c
                           const int32_t* tile_pairs, const int32_t* pairs, int32_t* status);
 
 /* ------------------------------------------------------------------------
+ * Projection in 8-bit integers
+ * ------------------------------------------------------------------------ */
+
+/* Each row of x (n_rows, cols) in 8-bit integers: with top = max |x| over the row,
+ *     scale[r] = top / 127          (f32)
+ *     q[r][c]  = 127 x / top, to the nearest integer, ties to even (decided exactly)
+ * so q lies in [-127, 127] and q * scale is x to within half a step.  A row of zeros
+ * gives zeros and scale 0; a row holding an infinity or NaN gives zeros and scale NaN, so
+ * everything computed from it is NaN.  x is f32, bf16 or f16 with any row stride and
+ * alignment; q has row stride ldq >= cols (bytes; a multiple of 16 with a 16-byte
+ * aligned base for lf_linear_int8); bytes of q's rows past cols are not written.  Used
+ * for activations (a row per token) and for weights (a row per output channel). */
+int lf_quantize_rows(void* stream, int dtype, const void* x, int64_t ldx, int64_t n_rows, int cols,
+                     int8_t* q, int64_t ldq, float* scale);
+
+/* y = act(float(x w^T) * x_scale[t] * w_scale[c] + bias[c]) for int8 x (m, k) with a scale
+ * per row, int8 w (n, k) with a scale per output channel (both as lf_quantize_rows
+ * writes them) and bias (n entries in dtype, or NULL); y (m, n) in dtype (f32, bf16 or
+ * f16).  The integer sum is exact; scaling, bias and activation are f32, rounded to
+ * dtype once (unlike lf_linear, which rounds before the GELU too).  Any m, n >= 1 and
+ * 1 <= k <= 131072; x and w need 16-byte aligned rows, y and bias any alignment
+ * (y rows that are 16-byte aligned are written faster).  x, w and y must not overlap. */
+int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t ldx, const float* x_scale,
+                   const int8_t* w, int64_t ldw, const float* w_scale, const void* bias,
+                   void* y, int64_t ldy, int64_t m, int n, int k, int act, int32_t* status);
+
+/* ------------------------------------------------------------------------
  * Encoder elementwise ops around the projections
  * ------------------------------------------------------------------------ */
 
@@ -450,6 +477,14 @@ int lf_linear_lora_shrink(void* stream, int dtype, const void* x, int64_t ldx, c
 int lf_add_layernorm(void* stream, int dtype, const void* a, int64_t lda, const void* b, int64_t ldb,
                      const void* vec, const void* gamma, const void* beta, float eps, int64_t n_rows,
                      int hidden, void* out, int64_t ldo);
+
+/* lf_add_layernorm (without vec) that also writes its output row, as rounded to dtype,
+ * in 8-bit integers: q and q_scale as lf_quantize_rows would give them for out, so that
+ * an 8-bit projection reads the row without a pass of its own.  q rows (row stride ldq
+ * bytes) are 8-byte aligned, n_rows scales. */
+int lf_add_layernorm_int8(void* stream, int dtype, const void* a, int64_t lda, const void* b, int64_t ldb,
+                          const void* gamma, const void* beta, float eps, int64_t n_rows, int hidden,
+                          void* out, int64_t ldo, int8_t* q, int64_t ldq, float* q_scale);
 
 /* The encoder's embeddings and their LayerNorm in one pass over gathered rows:
  *     e = round(round(word[ids[r]] + type[types[r]]) + pos[positions[r]])

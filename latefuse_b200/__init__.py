@@ -28,6 +28,14 @@ from latefuse_b200.config import LoraServingConfig
 from latefuse_b200.engine import EncoderWithLora, HFEncoderWithLora
 from latefuse_b200.head import POOLING_STRATEGIES, LRHeadOps, pool_tokens, validate_pooling
 from latefuse_b200.heads import HeadStore, LRHead
+from latefuse_b200.int8_ops import (
+    Int8Rows,
+    Int8Weight,
+    add_layernorm_int8,
+    ffn_int8,
+    linear_int8,
+    quantize_rows,
+)
 from latefuse_b200.loaders import load_peft_adapter, peft_key_fn
 from latefuse_b200.lora import LoraOps, SegmentTable, lora_apply
 from latefuse_b200.rank_buckets import RankBucketStore
@@ -81,5 +89,12 @@ __all__ = [
     "LoraOps",
     "LRHeadOps",
     "lora_apply",
+    # Projections in 8-bit integers.
+    "Int8Rows",
+    "Int8Weight",
+    "quantize_rows",
+    "linear_int8",
+    "add_layernorm_int8",
+    "ffn_int8",
     "__version__",
 ]

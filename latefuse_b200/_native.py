@@ -110,6 +110,14 @@ SIGNATURES: dict[str, tuple] = {
         c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
         c_int64, c_int64, c_void_p, c_void_p, c_void_p, ctypes.c_float, c_int64, c_int, c_void_p, c_int64,
         c_void_p]),
+    "lf_add_layernorm_int8": (c_int, [
+        c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, ctypes.c_float, c_int64, c_int,
+        c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "lf_quantize_rows": (c_int, [
+        c_void_p, c_int, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "lf_linear_int8": (c_int, [
+        c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
+        c_int64, c_int, c_int, c_int, c_void_p]),
     "lf_gelu": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64]),
     "lf_attention_varlen": (c_int, [
         c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int,
@@ -177,6 +185,25 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _SameDevice:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_same_device = _SameDevice()
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current CUDA device (launches, kernel attributes
+    and tensor maps go by the current device): nothing to do when it already is."""
+    if device.index is None or torch.cuda.current_device() == device.index:
+        return _same_device
+    return torch.cuda.device(device)
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:

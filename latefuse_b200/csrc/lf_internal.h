@@ -177,6 +177,10 @@ struct NormParams {
   int64_t ldc;
   int64_t n_a, n_b, n_c;
   int32_t* status;
+  // also the output as 8-bit integers with a scale per row (lf_quant.cuh); null: not wanted
+  int8_t* q;
+  int64_t ldq;
+  float* q_scale;
 };
 
 struct SimtParams {

@@ -1,0 +1,624 @@
+// Projection in 8-bit integers on tcgen05 (kind::i8): for int8 x (m, k) with a scale per
+// row (token) and int8 w (n, k) with a scale per row (output channel),
+//     y = act(float(sum_k x w) * x_scale * w_scale + bias)
+// The sum is exact in 32-bit integers (127^2 k < 2^31 up to k = 133,144; calls stop at
+// 131,072), so the result does not depend on tile, split or order; it becomes f32 (one
+// rounding), is scaled and biased in f32 (the scale of w and the bias in one FMA), and
+// the activation's result is rounded once to the output type.
+//
+// Two kernels, the same results bit for bit:
+//
+// linear_int8_kernel, for batches: the bf16 projection's CTA-pair GEMM (lf_linear.cu) with
+// 8-bit operands.  256 x 256 output tiles on persistent clusters of two CTAs, K blocks of
+// 128 (128 bytes: the same SW128 boxes, ring and barriers), tcgen05.mma.cta_group::2
+// M = 256, N = 256, K = 32.  A K block has the bytes of bf16's 64-wide one and twice its
+// multiplications in the same time.
+//   warp 0      TMA producer (both CTAs): an x box {128, 128} and a w box {128, 128} into
+//               a 6-stage ring, completing on the leader's barrier;
+//   warp 1      MMA issuer (leader only); TMEM holds two 256-column accumulators;
+//   warps 2-9   epilogue (both CTAs), two warps per TMEM lane quadrant, 128 columns each,
+//               32 at a time: staged per warp and written by TMA, or by the warp row by row
+//               where y's rows are not 16-byte aligned.
+//
+// linear_int8_split_kernel, for few tokens, where streaming w is the bound and 256-wide
+// tiles would leave most SMs without work: w's rows are the MMA's M (128 channels per
+// CTA), the tokens its N (16 to 128), and K is split over a cluster of up to 8 CTAs whose
+// integer partial sums meet in distributed shared memory (each CTA finishes a share of
+// the tokens).  Integer addition is exact, so the split changes no bit.
+//
+// Every wait is bounded: a timeout sets LF_STATUS_TIMEOUT and the roles unwind.
+#include <cstring>
+
+#include "lf_common.cuh"
+#include "lf_internal.h"
+#include "lf_pair.cuh"
+
+namespace lf {
+
+namespace {
+
+constexpr int kBK = 128;  // K block: 128 int8 = one SW128 row
+
+struct alignas(64) LinearInt8Params {
+  CUtensorMap x_map;  // 2D {K, M} uint8, box {128, rows}, SW128
+  CUtensorMap w_map;  // 2D {K, N} uint8, box {128, 128}, SW128
+  CUtensorMap y_map;  // 2D {N, M}, box {32, 32}: SW64 for 2-byte y, SW128 for f32 (tma_out)
+  const float* x_scale;
+  const float* w_scale;
+  const void* bias;   // N entries or null
+  void* y;
+  int64_t ldy;
+  int64_t m_rows;
+  int64_t n_tiles;
+  int32_t n, n_tiles_n, n_kb;
+  int32_t tma_out;    // y's base and row stride are 16-byte aligned
+  int32_t split;      // split kernel: CTAs of the cluster that share a tile's K
+  int32_t* status;
+};
+
+// D[tmem] (+)= A * B, 8-bit integers into s32.
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor for kind::i8: signed 8-bit A and B, both K-major, s32 D.
+__host__ __device__ constexpr uint32_t umma_idesc_i8(uint32_t m, uint32_t n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+__device__ __forceinline__ bool aborted(const int32_t* f) { return *reinterpret_cast<const volatile int32_t*>(f) != 0; }
+
+// Two accumulators of one token: scaled, biased, activated (f32).
+template <int kAct>
+__device__ __forceinline__ float2 finish2(int a0, int a1, float2 xs, float2 ws, float2 b) {
+  const float2 y = f2_fma(f2_mul(make_float2(__int2float_rn(a0), __int2float_rn(a1)), xs), ws, b);
+  if constexpr (kAct == LF_ACT_GELU) return gelu2_fast(y);
+  return y;
+}
+
+// ---------------------------------------------------------------------------
+// batches: CTA pairs, 256 x 256 tiles
+// ---------------------------------------------------------------------------
+constexpr int kBM = 128, kBN = 256;
+constexpr int kABytes = kBM * kBK;         // 16 KB: this CTA's x rows
+constexpr int kBBytes = (kBN / 2) * kBK;   // 16 KB: this CTA's half of the w rows
+constexpr int kStageBytes = kABytes + kBBytes;
+constexpr int kStages = 6;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kOutCols = 32;
+__host__ __device__ constexpr int out_buf(int es) { return 32 * kOutCols * es; }  // one warp's 32 x 32 staging tile
+constexpr int smem_bytes(int es) { return 1024 + kStages * kStageBytes + kEpiWarps * out_buf(es) + 1024; }
+static_assert(smem_bytes(4) <= 232448, "above the 227 KB of shared memory a CTA may use");
+
+template <typename T, int kAct>
+__global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_constant__ LinearInt8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_ctarank();  // 0: the leader, which issues the MMAs
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  constexpr int kOutBuf = out_buf(sizeof(T));
+
+  const uint32_t s_out0 = base + kStages * kStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(gbase + kStages * kStageBytes + kEpiWarps * kOutBuf);
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  constexpr int FULL = 0, EMPTY = kStages, ACC_FULL = 2 * kStages, ACC_EMPTY = ACC_FULL + 2, DRAIN = ACC_EMPTY + 2,
+                N_BARS = DRAIN + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(&bars[N_BARS]);
+  int32_t* s_abort = reinterpret_cast<int32_t*>(tmem_slot + 1);
+
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(bar(FULL + i), 1);   // the leader's arrive, with both CTAs' bytes
+      mbar_init(bar(EMPTY + i), 1);  // the leader's MMA commit
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(ACC_FULL + i), 1);
+      mbar_init(bar(ACC_EMPTY + i), 2 * kEpiWarps);  // both CTAs' epilogue warps
+    }
+    mbar_init(bar(DRAIN), 1);
+    *s_abort = 0;
+    fence_mbar_init();
+    prefetch_tmap(&p.x_map);
+    prefetch_tmap(&p.w_map);
+    prefetch_tmap(&p.y_map);
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc_pair(smem_u32(tmem_slot), 2 * kBN);
+  }
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers exist before either signals the other's
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  auto fail = [&]() {
+    set_status(p.status, LF_STATUS_TIMEOUT);
+    atomicExch(s_abort, 1);
+  };
+  auto wait = [&](uint32_t b, uint32_t parity) {
+    if (aborted(s_abort)) return false;
+    if (mbar_wait(b, parity)) return true;
+    if (!aborted(s_abort)) fail();
+    return false;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer (both CTAs)
+    if (lane == 0) {
+      int kk = 0;
+      bool stop = false;
+      for (int64_t t = pair; t < p.n_tiles && !stop; t += n_pairs) {
+        const int32_t m0 = int32_t(t / p.n_tiles_n) * (2 * kBM) + int32_t(rank) * kBM;
+        const int32_t n0 = int32_t(t % p.n_tiles_n) * kBN + int32_t(rank) * (kBN / 2);
+        for (int kb = 0; kb < p.n_kb; ++kb, ++kk) {
+          const int s = kk % kStages;
+          if (!wait(bar(EMPTY + s), ((kk / kStages) & 1) ^ 1)) {
+            stop = true;
+            break;
+          }
+          const uint32_t st = base + s * kStageBytes;
+          const uint32_t full = mapa_shared(bar(FULL + s), 0);
+          if (rank == 0) mbar_arrive_expect_tx(bar(FULL + s), 2 * kStageBytes);
+          tma_load_2d_pair(st, &p.x_map, full, kb * kBK, m0);
+          tma_load_2d_pair(st + kABytes, &p.w_map, full, kb * kBK, n0);
+        }
+      }
+      if (aborted(s_abort) && rank == 0) {  // loads nobody consumed land before the CTA exits (bounded)
+        for (int q = (kk > kStages ? kk - kStages : 0); q < kk; ++q)
+          mbar_wait(bar(FULL + q % kStages), (q / kStages) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (the leader's lane 0)
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = umma_idesc_i8(2 * kBM, kBN);
+      int kk = 0, n_it = 0;
+      bool stop = false;
+      for (int64_t t = pair; t < p.n_tiles && !stop; t += n_pairs, ++n_it) {
+        const int a = n_it & 1;
+        if (!wait(bar(ACC_EMPTY + a), ((n_it >> 1) & 1) ^ 1)) break;
+        tc_fence_after();
+        for (int kb = 0; kb < p.n_kb; ++kb, ++kk) {
+          const int s = kk % kStages;
+          if (!wait(bar(FULL + s), (kk / kStages) & 1)) {
+            stop = true;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t st = base + s * kStageBytes;
+#pragma unroll
+          for (int q = 0; q < kBK / 32; ++q)
+            umma_i8_pair(tmem + a * kBN, smem_desc(st + q * 32, 16, 1024, 2),
+                         smem_desc(st + kABytes + q * 32, 16, 1024, 2), idesc, (kb | q) != 0 ? 1u : 0u);
+          umma_commit_pair(bar(EMPTY + s));
+        }
+        if (!stop) umma_commit_pair(bar(ACC_FULL + a));
+      }
+      if (aborted(s_abort)) {  // every issued MMA finishes before TMEM is released (bounded)
+        umma_commit_pair_local(bar(DRAIN));
+        mbar_wait(bar(DRAIN), 0);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
+    const int quad = warp & 3;
+    const int half = (warp - 2) >> 2;  // columns [128 half, 128 half + 128) of the tile
+    const uint32_t taddr = tmem + (uint32_t(quad * 32) << 16);
+    const uint32_t my_out = s_out0 + (warp - 2) * kOutBuf;
+    uint8_t* g_out = gbase + (my_out - base);
+    const uint32_t acc_empty = mapa_shared(bar(ACC_EMPTY), 0);  // the leader's
+    const T* bias = static_cast<const T*>(p.bias);
+    T* y = static_cast<T*>(p.y);
+    const int c_begin = half * (kBN / kOutCols / 2), c_end = c_begin + kBN / kOutCols / 2;
+    int n_it = 0;
+    for (int64_t t = pair; t < p.n_tiles; t += n_pairs, ++n_it) {
+      const int a = n_it & 1;
+      const int64_t m0 = (t / p.n_tiles_n) * (2 * kBM) + int64_t(rank) * kBM + quad * 32;  // this warp's 32 rows
+      const int32_t n0 = int32_t(t % p.n_tiles_n) * kBN;
+      const float xs = m0 + lane < p.m_rows ? __ldg(p.x_scale + m0 + lane) : 0.f;
+      if (!__all_sync(0xffffffffu, wait(bar(ACC_FULL + a), (n_it >> 1) & 1))) break;
+      tc_fence_after();
+      for (int c = c_begin; c < c_end; ++c) {
+        const int col0 = n0 + c * kOutCols;
+        if (col0 >= p.n) break;
+        // the columns' scales and biases: lane i holds column i's, handed out by shuffles
+        const bool in = col0 + lane < p.n;
+        const float ws_l = in ? __ldg(p.w_scale + col0 + lane) : 0.f;
+        const float b_l = in && bias != nullptr ? DT<T>::to_f(bias[col0 + lane]) : 0.f;
+        uint32_t v[32];
+        tmem_ld32(taddr + a * kBN + c * kOutCols, v);
+        float o[32];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 ws = make_float2(__shfl_sync(0xffffffffu, ws_l, 2 * i), __shfl_sync(0xffffffffu, ws_l, 2 * i + 1));
+          const float2 b = make_float2(__shfl_sync(0xffffffffu, b_l, 2 * i), __shfl_sync(0xffffffffu, b_l, 2 * i + 1));
+          const float2 r = finish2<kAct>(int(v[2 * i]), int(v[2 * i + 1]), f2(xs), ws, b);
+          o[2 * i] = r.x;
+          o[2 * i + 1] = r.y;
+        }
+        // the store that last read this staging tile must be done with it
+        if (lane == 0) tma_store_wait_read_all();
+        __syncwarp();
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)  // SW64: 16-byte chunk q of row `lane` at q ^ ((lane >> 1) & 3)
+            *reinterpret_cast<uint4*>(g_out + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(Pack2<T>::pack(o[8 * q], o[8 * q + 1]), Pack2<T>::pack(o[8 * q + 2], o[8 * q + 3]),
+                           Pack2<T>::pack(o[8 * q + 4], o[8 * q + 5]), Pack2<T>::pack(o[8 * q + 6], o[8 * q + 7]));
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)  // SW128: chunk q of row `lane` at q ^ (lane & 7)
+            *reinterpret_cast<float4*>(g_out + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+                make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        }
+        if (p.tma_out) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&p.y_map, my_out, col0, int32_t(m0));
+            tma_store_commit();
+          }
+        } else {  // rows that are not 16-byte aligned: 32 neighbouring columns of a row at a time
+          __syncwarp();
+          for (int r = 0; r < 32 && m0 + r < p.m_rows; ++r) {
+            const T w = sizeof(T) == 2
+                            ? *reinterpret_cast<const T*>(g_out + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2)
+                            : *reinterpret_cast<const T*>(g_out + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+            if (in) y[(m0 + r) * p.ldy + col0 + lane] = w;
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc_empty + a * 8);  // this warp's TMEM reads of the tile are done
+    }
+    if (lane == 0) tma_store_wait_all();
+  }
+
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while its peer may still signal its barriers or read its operands
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc_pair(tmem, 2 * kBN);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// few tokens: 128 channels x NT tokens per CTA, K split over a cluster
+// ---------------------------------------------------------------------------
+constexpr int kSplitThreads = 64 + 128;
+__host__ __device__ constexpr int split_stages(int nt) { return nt <= 32 ? 8 : 6; }
+__host__ __device__ constexpr int split_stage_bytes(int nt) { return 128 * kBK + nt * kBK; }
+constexpr int split_smem_bytes(int nt) { return 1024 + split_stages(nt) * split_stage_bytes(nt) + 512; }
+static_assert(split_smem_bytes(128) <= 232448 && split_smem_bytes(32) <= 232448, "shared memory");
+// the partial sums (NT x 128 int32) reuse the ring
+static_assert(128 * 128 * 4 <= 6 * split_stage_bytes(128) && 16 * 128 * 4 <= 8 * split_stage_bytes(16), "ring");
+
+__device__ __forceinline__ int4 ld_dsmem_i4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+template <typename T, int NT, int kAct>
+__global__ void __launch_bounds__(kSplitThreads, 1) linear_int8_split_kernel(const __grid_constant__ LinearInt8Params p) {
+  constexpr int kSt = split_stages(NT), kSb = split_stage_bytes(NT);
+  constexpr uint32_t kTmemCols = NT < 32 ? 32 : NT;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int S = p.split;
+  const int rank = int(cluster_ctarank());
+  const int32_t n0 = int32_t(blockIdx.x / unsigned(S)) * 128;
+  const int64_t m0 = int64_t(blockIdx.y) * NT;
+  const int kb0 = int(int64_t(p.n_kb) * rank / S), kb1 = int(int64_t(p.n_kb) * (rank + 1) / S);
+
+  uint64_t* bars = reinterpret_cast<uint64_t*>(gbase + kSt * kSb);
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  constexpr int FULL = 0, EMPTY = kSt, ACC = 2 * kSt, N_BARS = ACC + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(&bars[N_BARS]);
+  int32_t* s_abort = reinterpret_cast<int32_t*>(tmem_slot + 1);
+  if (tid == 0) {
+    for (int i = 0; i < kSt; ++i) {
+      mbar_init(bar(FULL + i), 1);
+      mbar_init(bar(EMPTY + i), 1);
+    }
+    mbar_init(bar(ACC), 1);
+    *s_abort = 0;
+    fence_mbar_init();
+    prefetch_tmap(&p.x_map);
+    prefetch_tmap(&p.w_map);
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  auto wait = [&](uint32_t b, uint32_t parity) {
+    if (aborted(s_abort)) return false;
+    if (mbar_wait(b, parity)) return true;
+    set_status(p.status, LF_STATUS_TIMEOUT);
+    atomicExch(s_abort, 1);
+    return false;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int kk = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++kk) {
+        const int s = kk % kSt;
+        if (!wait(bar(EMPTY + s), ((kk / kSt) & 1) ^ 1)) break;
+        const uint32_t st = base + s * kSb;
+        mbar_arrive_expect_tx(bar(FULL + s), kSb);
+        tma_load_2d(st, &p.w_map, bar(FULL + s), kb * kBK, n0);
+        tma_load_2d(st + 128 * kBK, &p.x_map, bar(FULL + s), kb * kBK, int32_t(m0));
+      }
+      if (aborted(s_abort))  // loads nobody consumed land before the CTA exits (bounded)
+        for (int q = (kk > kSt ? kk - kSt : 0); q < kk; ++q) mbar_wait(bar(FULL + q % kSt), (q / kSt) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_i8(128, NT);
+      int kk = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++kk) {
+        const int s = kk % kSt;
+        if (!wait(bar(FULL + s), (kk / kSt) & 1)) break;
+        tc_fence_after();
+        const uint32_t st = base + s * kSb;
+#pragma unroll
+        for (int q = 0; q < kBK / 32; ++q)
+          umma_i8(tmem, smem_desc(st + q * 32, 16, 1024, 2), smem_desc(st + 128 * kBK + q * 32, 16, 1024, 2), idesc,
+                  (kk | q) != 0 ? 1u : 0u);
+        umma_commit(bar(EMPTY + s));
+      }
+      umma_commit(bar(ACC));  // also when unwinding: every issued MMA finishes before TMEM is released
+    }
+    __syncwarp();
+  } else {
+    // the CTA's partial sums, (token, channel) int32, into the ring once every MMA has read it
+    const int quad = warp & 3;
+    const bool ok = mbar_wait(bar(ACC), 0);
+    if (!ok) {
+      set_status(p.status, LF_STATUS_TIMEOUT);
+      atomicExch(s_abort, 1);
+    }
+    if (__all_sync(0xffffffffu, ok && !aborted(s_abort))) {
+      tc_fence_after();
+      int32_t* acc = reinterpret_cast<int32_t*>(gbase);
+#pragma unroll
+      for (int c = 0; c < NT / 16; ++c) {
+        float v[16];
+        tmem_ld16(tmem + (uint32_t(quad * 32) << 16) + c * 16, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[(c * 16 + i) * 128 + quad * 32 + lane] = __float_as_int(v[i]);
+      }
+      tc_fence_before();
+    }
+  }
+  __syncthreads();
+  const bool bad = aborted(s_abort);
+  cluster_sync();  // every CTA's partial sums are in place
+  if (warp >= 2 && !bad) {
+    // tokens [NT rank / S, NT (rank + 1) / S), one per warp at a time, four channels a lane
+    const T* bias = static_cast<const T*>(p.bias);
+    T* y = static_cast<T*>(p.y);
+    const int32_t ch = n0 + lane * 4;
+    float ws[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = ch + i < p.n;
+      ws[i] = in ? __ldg(p.w_scale + ch + i) : 0.f;
+      b[i] = in && bias != nullptr ? DT<T>::to_f(bias[ch + i]) : 0.f;
+    }
+    const bool whole = ch + 3 < p.n && p.tma_out;
+#pragma unroll 2
+    for (int t = NT * rank / S + (warp - 2); t < NT * (rank + 1) / S; t += 4) {
+      const int64_t row = m0 + t;
+      if (row >= p.m_rows) break;
+      int4 a = make_int4(0, 0, 0, 0);
+      for (int r = 0; r < S; ++r) {
+        const int4 v = ld_dsmem_i4(mapa_shared(base + uint32_t(t * 128 + lane * 4) * 4u, uint32_t(r)));
+        a.x += v.x;
+        a.y += v.y;
+        a.z += v.z;
+        a.w += v.w;
+      }
+      const float xs = __ldg(p.x_scale + row);
+      const float2 lo = finish2<kAct>(a.x, a.y, f2(xs), make_float2(ws[0], ws[1]), make_float2(b[0], b[1]));
+      const float2 hi = finish2<kAct>(a.z, a.w, f2(xs), make_float2(ws[2], ws[3]), make_float2(b[2], b[3]));
+      T* dst = y + row * p.ldy + ch;
+      if (whole) {
+        if constexpr (sizeof(T) == 2)
+          *reinterpret_cast<uint2*>(dst) = make_uint2(Pack2<T>::pack(lo.x, lo.y), Pack2<T>::pack(hi.x, hi.y));
+        else
+          *reinterpret_cast<float4*>(dst) = make_float4(lo.x, lo.y, hi.x, hi.y);
+      } else {
+        const float o[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (ch + i < p.n) dst[i] = DT<T>::from_f(o[i]);
+      }
+    }
+  }
+  tc_fence_before();
+  cluster_sync();  // no CTA leaves while a peer may still read its partial sums
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
+
+int encode(CUtensorMap* map, CUtensorMapDataType dt, int es, const void* base, int64_t cols, int64_t rows, int64_t ld,
+           int box_cols, int box_rows, CUtensorMapSwizzle swz, const char* what) {
+  PFN_encodeTiled enc = get_encode_tiled();
+  if (enc == nullptr) return set_error(LF_ERR_DRIVER, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+  const cuuint64_t strides[1] = {cuuint64_t(ld) * cuuint64_t(es)};
+  const cuuint32_t box[2] = {cuuint32_t(box_cols), cuuint32_t(box_rows)}, estr[2] = {1, 1};
+  const CUresult r = enc(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(LF_ERR_CUDA, "lf_linear_int8: cuTensorMapEncodeTiled(%s) failed: %d", what, int(r));
+  return LF_OK;
+}
+
+int sm_count() {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+template <typename K>
+int launch_cluster(K kern, const char* what, dim3 grid, int threads, int smem, int cluster, cudaStream_t s,
+                   const LinearInt8Params& p) {
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_error(e, what);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  e = cudaLaunchKernelEx(&cfg, kern, p);
+  if (e != cudaSuccess) return cuda_error(e, what);
+  count_launch();
+  return LF_OK;
+}
+
+template <typename T, int kAct>
+int launch_batch(LinearInt8Params& p, cudaStream_t s) {
+  p.n_tiles_n = (p.n + kBN - 1) / kBN;
+  p.n_tiles = (p.m_rows + 2 * kBM - 1) / (2 * kBM) * p.n_tiles_n;
+  const int64_t pairs = sm_count() / 2;
+  const unsigned grid = unsigned(2 * (p.n_tiles < pairs ? p.n_tiles : pairs));
+  return launch_cluster(linear_int8_kernel<T, kAct>, "launch linear_int8", dim3(grid), kThreads,
+                        smem_bytes(sizeof(T)), 2, s, p);
+}
+
+template <typename T, int kAct>
+int launch_split(LinearInt8Params& p, int nt, cudaStream_t s) {
+  p.n_tiles_n = (p.n + 127) / 128;
+  const unsigned mt = unsigned((p.m_rows + nt - 1) / nt);
+  const dim3 grid(unsigned(p.n_tiles_n) * unsigned(p.split), mt);
+  auto kern = nt == 16   ? linear_int8_split_kernel<T, 16, kAct>
+              : nt == 32 ? linear_int8_split_kernel<T, 32, kAct>
+              : nt == 64 ? linear_int8_split_kernel<T, 64, kAct>
+                         : linear_int8_split_kernel<T, 128, kAct>;
+  return launch_cluster(kern, "launch linear_int8_split", grid, kSplitThreads, split_smem_bytes(nt), p.split, s, p);
+}
+
+}  // namespace
+
+}  // namespace lf
+
+using namespace lf;
+
+extern "C" int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t ldx, const float* x_scale,
+                              const int8_t* w, int64_t ldw, const float* w_scale, const void* bias, void* y,
+                              int64_t ldy, int64_t m, int n, int k, int act, int32_t* status) {
+  const char* fn = "lf_linear_int8";
+  if (dtype != LF_DTYPE_BF16 && dtype != LF_DTYPE_F16 && dtype != LF_DTYPE_F32)
+    return set_error(LF_ERR_INVALID, "%s: unknown dtype %d", fn, dtype);
+  if (act != LF_ACT_NONE && act != LF_ACT_GELU) return set_error(LF_ERR_INVALID, "%s: unknown act %d", fn, act);
+  if (m < 0 || m > INT32_MAX - 256 || n <= 0 || n > INT32_MAX - 256 || k <= 0)
+    return set_error(LF_ERR_INVALID, "%s: m %lld, n %d, k %d", fn, (long long)m, n, k);
+  if (k > 131072) return set_error(LF_ERR_UNSUPPORTED, "%s: k %d above 131072 (the sum could leave 32 bits)", fn, k);
+  if (m == 0) return LF_OK;
+  if (x == nullptr || x_scale == nullptr || w == nullptr || w_scale == nullptr || y == nullptr)
+    return set_error(LF_ERR_INVALID, "%s: null x, w, scales or y", fn);
+  if (ldx < k || ldw < k || ldy < n) return set_error(LF_ERR_INVALID, "%s: a row stride is below its row", fn);
+  if (!aligned16(x) || !aligned16(w) || ldx % 16 != 0 || ldw % 16 != 0)
+    return set_error(LF_ERR_INVALID, "%s: x and w need 16-byte aligned rows", fn);
+  const int es = dtype == LF_DTYPE_F32 ? 4 : 2;
+  LinearInt8Params p;
+  memset(&p, 0, sizeof(p));
+  p.x_scale = x_scale;
+  p.w_scale = w_scale;
+  p.bias = bias;
+  p.y = y;
+  p.ldy = ldy;
+  p.m_rows = m;
+  p.n = n;
+  p.n_kb = (k + kBK - 1) / kBK;
+  p.tma_out = aligned16(y) && (ldy * es) % 16 == 0 ? 1 : 0;
+  p.status = status;
+
+  // 256 x 256 tiles once they fill the CTA pairs; below that 128 channels x nt tokens
+  const int sms = sm_count();
+  const int64_t big = ((m + 255) / 256) * ((n + 255) / 256);
+  const bool batch = big > sms / 4;
+  const int nt = batch ? 128 : m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+  p.split = 1;
+  if (!batch) {
+    const int64_t tiles = ((m + nt - 1) / nt) * ((n + 127) / 128);
+    while (p.split < 8 && tiles * p.split * 2 <= sms && p.split * 2 <= p.n_kb) p.split *= 2;
+  }
+  int rc;
+  if ((rc = encode(&p.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, k, m, ldx, kBK, nt, CU_TENSOR_MAP_SWIZZLE_128B, "x")))
+    return rc;
+  if ((rc = encode(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, k, n, ldw, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B, "w")))
+    return rc;
+  if (batch && p.tma_out) {
+    const CUtensorMapDataType dt = dtype == LF_DTYPE_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                   : dtype == LF_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    if ((rc = encode(&p.y_map, dt, es, y, n, m, ldy, kOutCols, 32,
+                     es == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, "y")))
+      return rc;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto tag) {
+    using T = decltype(tag);
+    if (act == LF_ACT_GELU)
+      return batch ? launch_batch<T, LF_ACT_GELU>(p, s) : launch_split<T, LF_ACT_GELU>(p, nt, s);
+    return batch ? launch_batch<T, LF_ACT_NONE>(p, s) : launch_split<T, LF_ACT_NONE>(p, nt, s);
+  };
+  if (dtype == LF_DTYPE_BF16) return go(__nv_bfloat16{});
+  if (dtype == LF_DTYPE_F16) return go(__half{});
+  return go(float{});
+}

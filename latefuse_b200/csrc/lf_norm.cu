@@ -10,6 +10,8 @@
 // mean and biased variance in f32 over the row (two passes over registers).
 // One warp per row: lane l holds elements [256 c + 8 l, 256 c + 8 l + 8) of
 // chunk c, read and written as 16-byte vectors, so a row is one pass over HBM.
+// With QUANT the rounded row, still in registers, is also written as 8-bit integers
+// with its scale (lf_quant.cuh), for an 8-bit projection that reads it next.
 //
 // GELU (ACT2FN["gelu"], src/latefuse/model/encoder.py:122,139):
 //     out = round_T(x * 0.5 * (1 + erf(x / sqrt(2))))       in f32
@@ -24,6 +26,7 @@
 
 #include "lf_common.cuh"
 #include "lf_internal.h"
+#include "lf_quant.cuh"
 
 namespace lf {
 
@@ -102,7 +105,7 @@ constexpr int kNormWarps = 8;
 // MODE 0: a alone; 1: a + b (a second matrix); 2: a + v (one row vector); 3: the
 // embeddings, round(round(a[ia] + c[ic]) + b[ib]) of gathered table rows (the
 // encoder's word + token type, then + position, each sum rounded as torch rounds it).
-template <typename T, int NC, int MODE>
+template <typename T, int NC, int MODE, bool QUANT = false>
 __global__ void __launch_bounds__(32 * kNormWarps)
 add_layernorm_kernel(const NormParams p, int full) {
   constexpr bool HAS_B = MODE != 0;
@@ -210,6 +213,31 @@ add_layernorm_kernel(const NormParams p, int full) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = (v[c][i] - mean) * rstd * gf[i] + bf[i];
       Vec8<T>::store(out + col, o);
+      if constexpr (QUANT) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c][i] = round_through<T>(o[i]);
+      }
+    }
+  }
+  if constexpr (QUANT) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (full || c * 256 + lane * 8 < H) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, mag_bits(v[c][i]));
+      }
+    const RowQuant rq(__reduce_max_sync(0xffffffffu, top));
+    if (lane == 0) p.q_scale[row] = rq.scale;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = c * 256 + lane * 8;
+      if (full || col < H) {
+        uint2 w;
+        w.x = rq.q4(v[c][0], v[c][1], v[c][2], v[c][3]);
+        w.y = rq.q4(v[c][4], v[c][5], v[c][6], v[c][7]);
+        *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) = w;
+      }
     }
   }
 }
@@ -277,7 +305,9 @@ int launch_norm(const NormParams& p, cudaStream_t s) {
   switch (nc) {
 #define LF_NORM_CASE(N)                                                                  \
   case N:                                                                                \
-    e = launch_pdl(p.ia != nullptr ? add_layernorm_kernel<T, N, 3>                       \
+    e = launch_pdl(p.q != nullptr ? (p.b != nullptr ? add_layernorm_kernel<T, N, 1, true> \
+                                                    : add_layernorm_kernel<T, N, 0, true>) \
+                   : p.ia != nullptr ? add_layernorm_kernel<T, N, 3>                     \
                    : p.b != nullptr ? add_layernorm_kernel<T, N, 1>                      \
                    : p.vec != nullptr ? add_layernorm_kernel<T, N, 2> : add_layernorm_kernel<T, N, 0>, \
                    grid, block, 0, s, p, full);                                          \
@@ -361,26 +391,35 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 using namespace lf;
 
-extern "C" int lf_add_layernorm(void* stream, int dtype, const void* a, int64_t lda, const void* b, int64_t ldb,
-                                const void* vec, const void* gamma, const void* beta, float eps, int64_t n_rows,
-                                int hidden, void* out, int64_t ldo) {
+static int add_layernorm_impl(const char* fn, void* stream, int dtype, const void* a, int64_t lda, const void* b,
+                              int64_t ldb, const void* vec, const void* gamma, const void* beta, float eps,
+                              int64_t n_rows, int hidden, void* out, int64_t ldo, bool quant, int8_t* q, int64_t ldq,
+                              float* q_scale) {
   if (dtype != LF_DTYPE_BF16 && dtype != LF_DTYPE_F16 && dtype != LF_DTYPE_F32)
-    return set_error(LF_ERR_INVALID, "lf_add_layernorm: unknown dtype %d", dtype);
+    return set_error(LF_ERR_INVALID, "%s: unknown dtype %d", fn, dtype);
   if (a == nullptr || gamma == nullptr || beta == nullptr || out == nullptr)
-    return set_error(LF_ERR_INVALID, "lf_add_layernorm: null a, gamma, beta or out");
-  if (b != nullptr && vec != nullptr) return set_error(LF_ERR_INVALID, "lf_add_layernorm: b and vec together");
+    return set_error(LF_ERR_INVALID, "%s: null a, gamma, beta or out", fn);
+  if (b != nullptr && vec != nullptr) return set_error(LF_ERR_INVALID, "%s: b and vec together", fn);
   if (n_rows < 0 || hidden <= 0 || hidden % 8 != 0)
-    return set_error(LF_ERR_INVALID, "lf_add_layernorm: hidden %d must be a positive multiple of 8", hidden);
-  if (hidden > 4096) return set_error(LF_ERR_UNSUPPORTED, "lf_add_layernorm: hidden %d above 4096", hidden);
+    return set_error(LF_ERR_INVALID, "%s: hidden %d must be a positive multiple of 8", fn, hidden);
+  if (hidden > 4096) return set_error(LF_ERR_UNSUPPORTED, "%s: hidden %d above 4096", fn, hidden);
   if (lda < hidden || ldo < hidden || (b != nullptr && ldb < hidden))
-    return set_error(LF_ERR_INVALID, "lf_add_layernorm: a row stride is below hidden %d", hidden);
+    return set_error(LF_ERR_INVALID, "%s: a row stride is below hidden %d", fn, hidden);
   const int es = dtype == LF_DTYPE_F32 ? 4 : 2;
   if (!aligned16(a) || !aligned16(out) || !aligned16(gamma) || !aligned16(beta) || (b != nullptr && !aligned16(b)) ||
       (vec != nullptr && !aligned16(vec)) ||
       (lda * es) % 16 != 0 || (ldo * es) % 16 != 0 || (b != nullptr && (ldb * es) % 16 != 0))
-    return set_error(LF_ERR_INVALID, "lf_add_layernorm: pointers and row strides must be 16-byte aligned");
+    return set_error(LF_ERR_INVALID, "%s: pointers and row strides must be 16-byte aligned", fn);
+  if (quant) {
+    if (q == nullptr || q_scale == nullptr) return set_error(LF_ERR_INVALID, "%s: null q or q_scale", fn);
+    if (ldq < hidden || ldq % 8 != 0 || (reinterpret_cast<uintptr_t>(q) & 7u) != 0)
+      return set_error(LF_ERR_INVALID, "%s: q needs 8-byte aligned rows of at least hidden %d", fn, hidden);
+  }
   if (n_rows == 0) return LF_OK;
   NormParams p = {};
+  p.q = q;
+  p.ldq = ldq;
+  p.q_scale = q_scale;
   p.a = a;
   p.b = b;
   p.lda = lda;
@@ -397,6 +436,20 @@ extern "C" int lf_add_layernorm(void* stream, int dtype, const void* a, int64_t 
   if (dtype == LF_DTYPE_BF16) return launch_norm<__nv_bfloat16>(p, s);
   if (dtype == LF_DTYPE_F16) return launch_norm<__half>(p, s);
   return launch_norm<float>(p, s);
+}
+
+extern "C" int lf_add_layernorm(void* stream, int dtype, const void* a, int64_t lda, const void* b, int64_t ldb,
+                                const void* vec, const void* gamma, const void* beta, float eps, int64_t n_rows,
+                                int hidden, void* out, int64_t ldo) {
+  return add_layernorm_impl("lf_add_layernorm", stream, dtype, a, lda, b, ldb, vec, gamma, beta, eps, n_rows, hidden,
+                            out, ldo, false, nullptr, 0, nullptr);
+}
+
+extern "C" int lf_add_layernorm_int8(void* stream, int dtype, const void* a, int64_t lda, const void* b, int64_t ldb,
+                                     const void* gamma, const void* beta, float eps, int64_t n_rows, int hidden,
+                                     void* out, int64_t ldo, int8_t* q, int64_t ldq, float* q_scale) {
+  return add_layernorm_impl("lf_add_layernorm_int8", stream, dtype, a, lda, b, ldb, nullptr, gamma, beta, eps, n_rows,
+                            hidden, out, ldo, true, q, ldq, q_scale);
 }
 
 extern "C" int lf_embed_layernorm(void* stream, int dtype, const void* word, int64_t ld_word, int64_t n_word,

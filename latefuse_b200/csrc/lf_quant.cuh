@@ -1,0 +1,60 @@
+// Symmetric 8-bit quantisation of a row: with top = max |x| over the row,
+//     scale = top / 127                 (rounded to f32)
+//     q     = round_half_even(127 x / top)          in [-127, 127]
+// The quotient is decided exactly: it is formed in f32 as v = x * (127 / top), which is
+// off by at most 127.5 * 2^-23 < 2^-15, and where v lies nearer than 2^-15 to a half the
+// remainder decides (RowQuant::settle).  So q does not depend on how a caller rounds, and
+// ties (frequent with 16-bit inputs: top = 254 * 2^e makes every second integer one) go
+// to the even step.  A row of zeros gives q = 0, scale = 0.  A row with an infinity or
+// NaN gives q = 0 and scale = NaN, so that whatever is computed from the row is NaN.
+#pragma once
+
+#include "lf_common.cuh"
+
+namespace lf {
+
+// |x| as an integer that orders like the magnitude, NaN above infinity (fmaxf would drop NaN).
+__device__ __forceinline__ uint32_t mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+struct RowQuant {
+  static constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, ties to even
+  float pre;    // a power of two that keeps top and 127 x clear of f32's ends
+  float top;    // the row's largest magnitude, times pre
+  float inv;    // 127 / top; 0 for a row of zeros or a row that is not finite
+  float scale;
+  // top_bits: the largest mag_bits of the row
+  __device__ __forceinline__ explicit RowQuant(uint32_t top_bits) {
+    const float t = __uint_as_float(top_bits);
+    const bool finite = top_bits < 0x7f800000u;
+    pre = t < 1.f ? 18446744073709551616.f : 1.f / 18446744073709551616.f;
+    top = t * pre;
+    inv = (top_bits == 0u || !finite) ? 0.f : __fdiv_rn(127.f, top);
+    scale = finite ? __fdiv_rn(t, 127.f) : __uint_as_float(0x7fc00000u);
+  }
+  // v next to r + 1/2 or r - 1/2 (r = rint(v)), or not a number: 127 x - r top is exact
+  // in two floats (the product 127 x splits exactly, and its head minus r top is a
+  // multiple of ulp(top) / 2 below 2^24 of them), so comparing it with top / 2 is exact.
+  __device__ __forceinline__ float settle(float x, float r) const {
+    if (!(fabsf(r) <= 128.f) || inv == 0.f) return 0.f;  // only rows that are not finite (or all 0) come here so
+    const float p = 127.f * x, e = fmaf(127.f, x, -p), rem = fmaf(-r, top, p);
+    const float sgn = rem < 0.f ? -1.f : 1.f;
+    const float over = (fabsf(rem) - 0.5f * top) + sgn * e;  // its sign is exact: the difference is
+    const bool odd = (__float_as_int(r + kMagic) & 1) != 0;
+    return over > 0.f || (over == 0.f && odd) ? r + sgn : r;
+  }
+  // q in the low byte (two's complement) of the result
+  __device__ __forceinline__ uint32_t q(float x) const {
+    x *= pre;
+    const float v = x * inv;
+    float m = v + kMagic;
+    const float r = m - kMagic;
+    if (!(fabsf(v - r) < 0.499969482421875f)) m = settle(x, r) + kMagic;
+    return __float_as_uint(m);
+  }
+  // q of four values, the first in the low byte
+  __device__ __forceinline__ uint32_t q4(float a, float b, float c, float d) const {
+    return __byte_perm(__byte_perm(q(a), q(b), 0x0040), __byte_perm(q(c), q(d), 0x0040), 0x5410);
+  }
+};
+
+}  // namespace lf
