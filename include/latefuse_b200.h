@@ -523,6 +523,28 @@ int lf_attention_varlen(void* stream, int dtype, const void* qkv, int64_t ld_qkv
                         const int32_t* items, int n_items, float scale, void* out, int64_t ld_out,
                         int32_t* status);
 
+/* Cross attention of packed sequences: for sequence s, query row i and head h
+ *     out[i][h] = softmax_j(scale * q_i[h] . k_j[h / group]) @ v[h / group]
+ * over the sequence's own keys j, group = n_heads / n_kv_heads (query heads that share a
+ * key head).  A sequence without keys gives rows of zeros.  q and out rows hold n_heads
+ * heads of head_dim elements side by side, k and v rows n_kv_heads; each of the four has
+ * its own row stride (elements; columns of a fused projection are fine).  head_dim is a
+ * multiple of 8 up to 128; dtype bf16 or f16; scale positive; statistics and sums in f32.
+ * `items` is a device int32 array of n_items records of 8, 16-byte aligned:
+ *     {q_start, q_len, kv_start, kv_len, q_tile, 0, 0, 0}
+ * one per sequence and 128-query tile (latefuse_b200.packing.cross_batch builds them).
+ * Key ranges may overlap or be shared; query ranges of different sequences may not.  Rows
+ * of out in no record are not written.  max_q and max_kv are the largest q_len and kv_len
+ * (they choose the kernel and how keys are split; max_q at most 128 promises that every
+ * q_tile is 0).  A record outside [0, n_q) or [0, n_kv), or past max_q, sets
+ * LF_STATUS_BAD_SEGMENT and stores nothing.  It allocates nothing and launches one
+ * kernel; a row's bits depend on max_q, max_kv and the number of records (through the
+ * choice of kernel and split), never on timing. */
+int lf_cross_attention_varlen(void* stream, int dtype, const void* q, int64_t ldq, int64_t n_q,
+                              const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t n_kv,
+                              int n_heads, int n_kv_heads, int head_dim, const int32_t* items, int n_items,
+                              int max_q, int max_kv, float scale, void* out, int64_t ld_out, int32_t* status);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,6 +25,7 @@ from latefuse_b200.batch import (
     LayerwiseBatchedWeights,
 )
 from latefuse_b200.config import LoraServingConfig
+from latefuse_b200.encoder_ops import cross_attention_varlen
 from latefuse_b200.engine import EncoderWithLora, HFEncoderWithLora
 from latefuse_b200.head import POOLING_STRATEGIES, LRHeadOps, pool_tokens, validate_pooling
 from latefuse_b200.heads import HeadStore, LRHead
@@ -38,6 +39,7 @@ from latefuse_b200.int8_ops import (
 )
 from latefuse_b200.loaders import load_peft_adapter, peft_key_fn
 from latefuse_b200.lora import LoraOps, SegmentTable, lora_apply
+from latefuse_b200.packing import CrossBatch, cross_batch
 from latefuse_b200.rank_buckets import RankBucketStore
 from latefuse_b200.store import AdapterStore, LoraWeight
 from latefuse_b200.tasks import (
@@ -89,6 +91,10 @@ __all__ = [
     "LoraOps",
     "LRHeadOps",
     "lora_apply",
+    # Attention to the encoder's states.
+    "CrossBatch",
+    "cross_batch",
+    "cross_attention_varlen",
     # Projections in 8-bit integers.
     "Int8Rows",
     "Int8Weight",

@@ -1,0 +1,990 @@
+// Cross attention of packed sequences: the queries of sequence s attend to the keys and
+// values of that sequence's encoder states, which have a length of their own:
+//     out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h / group]) v[j, h / group]
+// over the sequence's keys j (group query heads share a key head).  A sequence without
+// keys gives zeros.  head_dim is a multiple of 8 up to 128; the kernels are compiled for
+// 64 and 128 columns and read only the head's own (tensor maps and loads end at
+// head_dim, the columns past it count as zeros and cost no memory traffic).
+//
+// Softmax statistics and sums are f32, in the log2 domain; the unnormalised
+// probabilities are rounded to the 16-bit type for the second product, as the tensor
+// cores take them (each is within half a step of its value, and the sum that divides
+// them is taken before the rounding).  Keys past a sequence's end are never multiplied:
+// their scores are replaced, and their value rows are zeroed on chip, so that infinities
+// or NaN in a neighbouring sequence's states do not reach this one.
+//
+// Two kernels:
+//
+// cross_decode_kernel, for few query rows (single tokens), where reading K and V once at
+// HBM speed is the bound.  One CTA per (sequence, key head, block of query rows, share of
+// the keys): its rows are all of the group's heads and the sequence's queries (16 per
+// mma.sync tile), so K and V are read once for all of them.  Four warps take 16-key tiles
+// in turn, each with its own ring of asynchronous copies and its own running maximum and
+// sum, merged at the end through shared memory.  The keys of a sequence are split over a
+// cluster of up to 8 CTAs when there are too few sequences and heads to fill the GPU, or
+// to even out long and short ones; the cluster joins its parts through distributed
+// shared memory in rank order, so there is no workspace, no second launch and no atomic.
+//
+// cross_prompt_kernel, for many query rows, on tcgen05: the schedule of the packed
+// self-attention (lf_attention.cu) with separate query and key tables.  Work unit =
+// (128 queries of a sequence, head); a persistent CTA per SM runs two units in ping-pong:
+//   warp 0      producer: Q, K and V tiles by TMA (SW128 blocks of 64 columns);
+//   warp 1      MMA issuer: S = Q K^T into shared TMEM S buffers, O += P V into the
+//               group's TMEM accumulator;
+//   warps 2-5,  softmax groups, one thread per query row.
+//   6-9
+// With 64 columns a key tile has 128 keys; with 128 columns 64 keys, so that Q, P and
+// eight K / V stages fit in shared memory (229 KB).
+// Every wait is bounded: a timeout sets LF_STATUS_TIMEOUT and the roles unwind.
+#include <cmath>
+#include <cstring>
+
+#include "lf_common.cuh"
+#include "lf_internal.h"
+
+namespace lf {
+
+namespace {
+
+struct alignas(64) CrossParams {
+  CUtensorMap q_map, k_map, v_map;  // prompt: 3D {head_dim, heads, rows}, box {64, 1, 128 or the key tile}
+  const void *q, *k, *v;
+  int64_t ldq, ldk, ldv, n_q, n_kv;
+  int32_t n_heads, n_kv_heads, group, d;
+  const int4* items;   // two per record: {q_start, q_len, kv_start, kv_len}, {q_tile, 0, 0, 0}
+  int32_t n_items;
+  int32_t max_q;       // decode: no record's q_len is above it
+  int32_t split;       // decode: CTAs of the cluster that share a sequence's keys
+  float scale_log2;    // scale * log2(e)
+  void* out;
+  int64_t ldo;
+  int32_t* status;
+};
+
+// A record, checked against the tensors: one that names rows outside them, or a tile past
+// its queries, is reported and stores nothing.
+struct Rec {
+  int q0, nq, k0, nk, tile;
+  bool ok;
+};
+__device__ __forceinline__ Rec read_rec(const CrossParams& p, int i) {
+  const int4 a = __ldg(p.items + 2 * i), b = __ldg(p.items + 2 * i + 1);
+  Rec r{a.x, a.y, a.z, a.w, b.x, true};
+  r.ok = r.q0 >= 0 && r.nq >= 0 && int64_t(r.q0) + r.nq <= p.n_q && r.k0 >= 0 && r.nk >= 0 &&
+         int64_t(r.k0) + r.nk <= p.n_kv && r.tile >= 0 && (r.nq == 0 ? r.tile == 0 : int64_t(r.tile) * 128 < r.nq);
+  return r;
+}
+
+// ---------------------------------------------------------------------------
+// few query rows
+// ---------------------------------------------------------------------------
+constexpr int kDecodeWarps = 4;
+constexpr int kKeyTile = 16;  // keys a warp takes at a time
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// 16 bytes to shared memory, or 16 zeros when `bytes` is 0 (nothing is read then).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ float ld_dsmem_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__host__ __device__ constexpr int decode_stages(int kd) { return kd == 64 ? 4 : 3; }
+__host__ __device__ constexpr int decode_pitch(int kd) { return kd + 8; }  // f32 columns of a partial output row
+// [Q tile][ring, reused for the warps' partial outputs][warps' m and l][the CTA's m and l]
+__host__ __device__ constexpr int decode_q_bytes(int kd, int mt) { return 16 * mt * kd * 2; }
+__host__ __device__ constexpr int decode_ring_bytes(int kd) {
+  return kDecodeWarps * decode_stages(kd) * 2 * kKeyTile * kd * 2;
+}
+__host__ __device__ constexpr int decode_smem(int kd, int mt) {
+  return decode_q_bytes(kd, mt) + decode_ring_bytes(kd) + (kDecodeWarps + 1) * 16 * mt * 2 * 4;
+}
+static_assert(kDecodeWarps * 32 * decode_pitch(64) * 4 <= decode_ring_bytes(64), "partial outputs reuse the ring");
+static_assert(kDecodeWarps * 32 * decode_pitch(128) * 4 <= decode_ring_bytes(128), "partial outputs reuse the ring");
+
+template <typename T, int kD, int MT>
+__global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const __grid_constant__ CrossParams p) {
+  constexpr int kSt = decode_stages(kD), kTile = kKeyTile * kD * 2, kCh = kD / 8, kPitch = decode_pitch(kD);
+  constexpr int kRowsMax = 16 * MT;
+  constexpr bool kQRegs = MT * kD <= 128;  // Q fragments stay in registers (else re-read from shared memory)
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int S = p.split;
+  const int rank = S > 1 ? int(cluster_ctarank()) : 0;
+  const int unit = int(blockIdx.x) / S;
+  const int kvh = unit % p.n_kv_heads;
+  const uint32_t sQ = smem_u32(smem);
+  const uint32_t ring = sQ + decode_q_bytes(kD, MT) + warp * (kSt * 2 * kTile);
+  float* s_part = reinterpret_cast<float*>(smem + decode_q_bytes(kD, MT));
+  float* s_ml = s_part + decode_ring_bytes(kD) / 4;  // [warp][row]{m, l}, then the CTA's
+
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const Rec rec = read_rec(p, unit / p.n_kv_heads);
+  // the cluster's CTAs share the record, so they leave together
+  if (!rec.ok || rec.tile != 0 || rec.nq > p.max_q) {
+    if (tid == 0) set_status(p.status, LF_STATUS_BAD_SEGMENT);
+    return;
+  }
+  const int row0 = int(blockIdx.y) * kRowsMax;
+  const int rows = min(kRowsMax, rec.nq * p.group - row0);  // row r: query (row0 + r) / group, head (row0 + r) % group
+  if (rows <= 0) return;
+  const int nch = p.d / 8;              // 16-byte chunks of a head's row
+  const int nks = (p.d + 15) / 16;      // 16-column steps
+
+  // chunk c of a row sits at c ^ (row & 7) within its 128-byte line, so that ldmatrix's
+  // eight rows fall into different banks
+  auto at = [](uint32_t base, int row, int c) { return base + uint32_t(row * (kD * 2) + ((c ^ (row & 7)) << 4)); };
+
+  const T* qg = static_cast<const T*>(p.q);
+  for (int i = tid; i < kRowsMax * kCh; i += 32 * kDecodeWarps) {
+    const int r = i / kCh, c = i % kCh;
+    const bool in = r < rows && c < nch;
+    const int rr = row0 + (in ? r : 0);
+    const T* src = qg + int64_t(rec.q0 + rr / p.group) * p.ldq + int64_t(kvh * p.group + rr % p.group) * p.d + (in ? c : 0) * 8;
+    cp_async16(at(sQ, r, c), src, in ? 16u : 0u);
+  }
+  cp_async_commit();
+
+  // this CTA's 16-key tiles, every fourth one this warp's
+  const int n_tiles = (rec.nk + kKeyTile - 1) / kKeyTile;
+  const int t0 = int(int64_t(n_tiles) * rank / S), t1 = int(int64_t(n_tiles) * (rank + 1) / S);
+  const int n_my = t1 - t0 > warp ? (t1 - t0 - warp + kDecodeWarps - 1) / kDecodeWarps : 0;
+  const T* kg = static_cast<const T*>(p.k) + int64_t(kvh) * p.d;
+  const T* vg = static_cast<const T*>(p.v) + int64_t(kvh) * p.d;
+  auto issue = [&](int i) {
+    if (i < n_my) {
+      const int key0 = (t0 + warp + kDecodeWarps * i) * kKeyTile;
+      const uint32_t st = ring + (i % kSt) * (2 * kTile);
+#pragma unroll
+      for (int j = 0; j < kKeyTile * kCh / 32; ++j) {
+        const int r = (j * 32 + lane) / kCh, c = (j * 32 + lane) % kCh;
+        const bool in = key0 + r < rec.nk && c < nch;  // rows past the end and columns past the head are zeros
+        const int64_t row = rec.k0 + (in ? key0 + r : 0);
+        const int col = (in ? c : 0) * 8;
+        cp_async16(at(st, r, c), kg + row * p.ldk + col, in ? 16u : 0u);
+        cp_async16(at(st + kTile, r, c), vg + row * p.ldv + col, in ? 16u : 0u);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kSt - 1; ++i) issue(i);
+  cp_async_wait<kSt - 1>();  // Q has landed
+  __syncthreads();
+
+  uint32_t qf[kQRegs ? MT : 1][kQRegs ? kD / 16 : 1][4];
+  const int q_row = (lane & 7) + ((lane >> 3) & 1) * 8, q_chunk = lane >> 4;  // this lane's ldmatrix row of a Q tile
+  if constexpr (kQRegs) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int ks = 0; ks < kD / 16; ++ks) ldsm4(qf[m][ks], at(sQ, m * 16 + q_row, ks * 2 + q_chunk));
+  }
+  float o[MT][kD / 8][4] = {};
+  float mrow[MT][2], lrow[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) mrow[m][0] = mrow[m][1] = -INFINITY, lrow[m][0] = lrow[m][1] = 0.f;
+
+  const int k_row = (lane & 7) + (lane >> 4) * 8, k_chunk = (lane >> 3) & 1;  // K: {keys 0-7, 8-15} x {8 columns, next 8}
+  const int v_row = (lane & 7) + ((lane >> 3) & 1) * 8, v_chunk = lane >> 4;
+  for (int i = 0; i < n_my; ++i) {
+    cp_async_wait<kSt - 2>();
+    __syncwarp();
+    const uint32_t sK = ring + (i % kSt) * (2 * kTile), sV = sK + kTile;
+    float s[MT][2][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < kD / 16; ++ks) {
+      if (ks >= nks) break;
+      uint32_t kf[4];
+      ldsm4(kf, at(sK, k_row, ks * 2 + k_chunk));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        uint32_t a[4];
+        if constexpr (kQRegs) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) a[x] = qf[m][ks][x];
+        } else {
+          ldsm4(a, at(sQ, m * 16 + q_row, ks * 2 + q_chunk));
+        }
+        mma16816<T>(s[m][0], a, kf[0], kf[1]);
+        mma16816<T>(s[m][1], a, kf[2], kf[3]);
+      }
+    }
+    const int left = rec.nk - (t0 + warp + kDecodeWarps * i) * kKeyTile;  // keys of the sequence from this tile on
+    if (left < kKeyTile) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (n * 8 + (lane & 3) * 2 + (x & 1) >= left) s[m][n][x] = -INFINITY;
+    }
+    uint32_t pf[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // rows lane / 4 and lane / 4 + 8
+        float mx = fmaxf(fmaxf(s[m][0][2 * h], s[m][0][2 * h + 1]), fmaxf(s[m][1][2 * h], s[m][1][2 * h + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(mrow[m][h], mx * p.scale_log2);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;  // every score so far is -inf: p = 0
+        const float alpha = sfu_ex2(mrow[m][h] - m_use);
+        mrow[m][h] = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float e = sfu_ex2(fmaf(s[m][n][2 * h + x], p.scale_log2, -m_use));
+            s[m][n][2 * h + x] = e;
+            sum += e;
+          }
+        lrow[m][h] = lrow[m][h] * alpha + sum;
+        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+          for (int n = 0; n < kD / 8; ++n) {
+            o[m][n][2 * h] *= alpha;
+            o[m][n][2 * h + 1] *= alpha;
+          }
+        }
+      }
+      pf[m][0] = Pack2<T>::pack(s[m][0][0], s[m][0][1]);
+      pf[m][1] = Pack2<T>::pack(s[m][0][2], s[m][0][3]);
+      pf[m][2] = Pack2<T>::pack(s[m][1][0], s[m][1][1]);
+      pf[m][3] = Pack2<T>::pack(s[m][1][2], s[m][1][3]);
+    }
+#pragma unroll
+    for (int ks = 0; ks < kD / 16; ++ks) {
+      if (ks >= nks) break;
+      uint32_t vf[4];
+      ldsm4_t(vf, at(sV, v_row, ks * 2 + v_chunk));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        mma16816<T>(o[m][2 * ks], pf[m], vf[0], vf[1]);
+        mma16816<T>(o[m][2 * ks + 1], pf[m], vf[2], vf[3]);
+      }
+    }
+    issue(i + kSt - 1);  // into the slot of tile i - 1, which every lane has left
+  }
+  cp_async_wait<0>();
+  __syncthreads();  // every warp is done with the ring
+
+  // the warps' parts: output rows, maximum and sum
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = m * 16 + h * 8 + (lane >> 2);
+      float l = lrow[m][h];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      float* dst = s_part + (warp * kRowsMax + r) * kPitch + (lane & 3) * 2;
+#pragma unroll
+      for (int n = 0; n < kD / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[m][n][2 * h], o[m][n][2 * h + 1]);
+      if ((lane & 3) == 0) {
+        s_ml[(warp * kRowsMax + r) * 2] = mrow[m][h];
+        s_ml[(warp * kRowsMax + r) * 2 + 1] = l;
+      }
+    }
+  __syncthreads();
+  T* out = static_cast<T*>(p.out);
+  auto store = [&](int r, int c4, float4 v, float l) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int rr = row0 + r;
+    T* dst = out + int64_t(rec.q0 + rr / p.group) * p.ldo + int64_t(kvh * p.group + rr % p.group) * p.d + c4 * 4;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(Pack2<T>::pack(v.x * inv, v.y * inv), Pack2<T>::pack(v.z * inv, v.w * inv));
+  };
+  // n parts of one row: their joint maximum, and part i's weight 2^(m_i - max) (0 without keys)
+  float* s_cta = s_ml + kDecodeWarps * kRowsMax * 2;
+  const int c4s = p.d / 4;
+  for (int i = tid; i < rows * c4s; i += 32 * kDecodeWarps) {
+    const int r = i / c4s, c4 = i % c4s;
+    float mw[kDecodeWarps], mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kDecodeWarps; ++w) {
+      mw[w] = s_ml[(w * kRowsMax + r) * 2];
+      mx = fmaxf(mx, mw[w]);
+    }
+    const float m_use = mx == -INFINITY ? 0.f : mx;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDecodeWarps; ++w) {
+      const float f = sfu_ex2(mw[w] - m_use);
+      const float4 v = *reinterpret_cast<const float4*>(s_part + (w * kRowsMax + r) * kPitch + c4 * 4);
+      acc.x += v.x * f;
+      acc.y += v.y * f;
+      acc.z += v.z * f;
+      acc.w += v.w * f;
+      l += s_ml[(w * kRowsMax + r) * 2 + 1] * f;
+    }
+    if (S == 1) {
+      store(r, c4, acc, l);
+    } else {  // the CTA's part replaces warp 0's (only this thread reads it)
+      *reinterpret_cast<float4*>(s_part + r * kPitch + c4 * 4) = acc;
+      if (c4 == 0) {
+        s_cta[2 * r] = mx;
+        s_cta[2 * r + 1] = l;
+      }
+    }
+  }
+  if (S == 1) return;
+  cluster_sync();
+  const uint32_t a_part = smem_u32(s_part), a_cta = smem_u32(s_cta);
+  for (int i = rank * 32 * kDecodeWarps + tid; i < rows * c4s; i += S * 32 * kDecodeWarps) {
+    const int r = i / c4s, c4 = i % c4s;
+    float mx = -INFINITY;
+    for (int t = 0; t < S; ++t) mx = fmaxf(mx, ld_dsmem_f32(mapa_shared(a_cta + 8 * r, t)));
+    const float m_use = mx == -INFINITY ? 0.f : mx;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    for (int t = 0; t < S; ++t) {
+      const float f = sfu_ex2(ld_dsmem_f32(mapa_shared(a_cta + 8 * r, t)) - m_use);
+      const float4 v = ld_dsmem_f4(mapa_shared(a_part + uint32_t(r * kPitch + c4 * 4) * 4u, t));
+      acc.x += v.x * f;
+      acc.y += v.y * f;
+      acc.z += v.z * f;
+      acc.w += v.w * f;
+      l += ld_dsmem_f32(mapa_shared(a_cta + 8 * r + 4, t)) * f;
+    }
+    store(r, c4, acc, l);
+  }
+  cluster_sync();  // no CTA leaves while a peer may still read its part
+}
+
+// ---------------------------------------------------------------------------
+// many query rows
+// ---------------------------------------------------------------------------
+constexpr int kRows = 128;     // query tile rows
+constexpr int kGroups = 2;
+constexpr int kThreads = 64 + 32 * 4 * kGroups;
+constexpr float kMaxSlack = 8.f;  // log2 units the running max may lag a tile's max
+
+template <int kD>
+struct Shape {
+  static constexpr int kKeys = kD == 64 ? 128 : 64;   // key tile rows
+  static constexpr int kBlocks = kD / 64;             // 64-column SW128 blocks of a head's row
+  static constexpr int kQBytes = kRows * kD * 2;
+  static constexpr int kKvBytes = kKeys * kD * 2;     // 16 KB
+  static constexpr int kPBytes = kRows * kKeys * 2;
+  static constexpr int kKStages = kD == 64 ? 3 : 4;
+  static constexpr int kVStages = 4;
+  static constexpr int kSBufs = kD == 64 ? 3 : 4;     // TMEM S buffers shared by the groups
+  static constexpr int kOCol = kSBufs * kKeys;        // group g's O at TMEM column kOCol + kD g
+  static constexpr int kSmem = 1024 + kGroups * (kQBytes + kPBytes) + (kKStages + kVStages) * kKvBytes + 1024;
+  static_assert(kOCol + kGroups * kD <= 512, "TMEM columns");
+  static_assert(kSmem <= 232448, "above the 227 KB of shared memory a CTA may use");
+};
+
+__device__ __forceinline__ bool aborted(const int32_t* f) { return *reinterpret_cast<const volatile int32_t*>(f) != 0; }
+
+// max(a, b, c) in one instruction.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// A unit's record as every role reads it: keys to walk (at least one, so that all roles
+// take the same steps), and what is stored: 0 the result, 1 nothing, 2 zeros (no keys).
+struct Unit {
+  int q0, nq, k0, nk, tile, what;
+};
+
+template <int kKeys>
+struct Cursor {
+  int64_t unit;  // global unit index, or >= n_units when done
+  Unit it;
+  int j, n_kv;   // key tile within the unit
+  int u;         // units this group has started (for buffer parities)
+  int t;         // tiles this group has started
+};
+
+template <typename T, int kD>
+__global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_constant__ CrossParams p) {
+  using Sh = Shape<kD>;
+  constexpr int kKeys = Sh::kKeys, kKvBytes = Sh::kKvBytes;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  const uint32_t sQ = base;
+  const uint32_t sP = sQ + kGroups * Sh::kQBytes;
+  const uint32_t sK = sP + kGroups * Sh::kPBytes;
+  const uint32_t sV = sK + Sh::kKStages * kKvBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(gbase + (sV + Sh::kVStages * kKvBytes - base));
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  // per-group barriers at index (kind * kGroups + group)
+  constexpr int Q_FULL = 0, Q_EMPTY = 1, P_FULL = 2, P_EMPTY = 3, O_FULL = 4, O_EMPTY = 5;
+  auto gbar = [&](int kind, int grp) { return bar(kind * kGroups + grp); };
+  constexpr int S_FULL = 6 * kGroups, S_EMPTY = S_FULL + Sh::kSBufs, K_FULL = S_EMPTY + Sh::kSBufs,
+                K_EMPTY = K_FULL + Sh::kKStages, V_FULL = K_EMPTY + Sh::kKStages, V_EMPTY = V_FULL + Sh::kVStages,
+                DRAIN = V_EMPTY + Sh::kVStages, N_BARS = DRAIN + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(&bars[N_BARS]);
+  int32_t* s_abort = reinterpret_cast<int32_t*>(tmem_slot + 1);
+  const int64_t n_units = int64_t(p.n_items) * p.n_heads;
+
+  if (tid == 0) {
+    for (int grp = 0; grp < kGroups; ++grp) {
+      mbar_init(gbar(Q_FULL, grp), 1);
+      mbar_init(gbar(Q_EMPTY, grp), 1);
+      mbar_init(gbar(P_FULL, grp), 4);
+      mbar_init(gbar(P_EMPTY, grp), 1);
+      mbar_init(gbar(O_FULL, grp), 1);
+      mbar_init(gbar(O_EMPTY, grp), 4);
+    }
+    for (int i = 0; i < Sh::kSBufs; ++i) {
+      mbar_init(bar(S_FULL + i), 1);
+      mbar_init(bar(S_EMPTY + i), 4);
+    }
+    for (int i = 0; i < Sh::kKStages; ++i) {
+      mbar_init(bar(K_FULL + i), 1);
+      mbar_init(bar(K_EMPTY + i), 1);
+    }
+    for (int i = 0; i < Sh::kVStages; ++i) {
+      mbar_init(bar(V_FULL + i), 1);
+      mbar_init(bar(V_EMPTY + i), 1);
+    }
+    mbar_init(bar(DRAIN), 1);
+    *s_abort = 0;
+    fence_mbar_init();
+    prefetch_tmap(&p.q_map);
+    prefetch_tmap(&p.k_map);
+    prefetch_tmap(&p.v_map);
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc(smem_u32(tmem_slot), 512);
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  auto fail = [&]() {
+    set_status(p.status, LF_STATUS_TIMEOUT);
+    atomicExch(s_abort, 1);
+  };
+  auto wait = [&](uint32_t b, uint32_t parity) {
+    if (aborted(s_abort)) return false;
+    if (mbar_wait(b, parity)) return true;
+    if (!aborted(s_abort)) fail();
+    return false;
+  };
+  auto unit_of = [&](int64_t unit) {
+    const Rec r = read_rec(p, int(unit / p.n_heads));
+    if (!r.ok) {
+      set_status(p.status, LF_STATUS_BAD_SEGMENT);
+      return Unit{0, 0, 0, 1, 0, 1};
+    }
+    if (r.nq == 0) return Unit{0, 0, 0, 1, 0, 1};
+    if (r.nk == 0) return Unit{r.q0, r.nq, 0, 1, r.tile, 2};
+    return Unit{r.q0, r.nq, r.k0, r.nk, r.tile, 0};
+  };
+  // group grp takes the CTA's units 2k + grp
+  using Cur = Cursor<kKeys>;
+  auto start = [&](Cur& c, int grp) {
+    c.unit = blockIdx.x + int64_t(grp) * gridDim.x;
+    c.u = c.t = c.j = 0;
+    if (c.unit < n_units) {
+      c.it = unit_of(c.unit);
+      c.n_kv = (c.it.nk + kKeys - 1) / kKeys;
+    }
+  };
+  auto advance = [&](Cur& c) {
+    ++c.t;
+    if (++c.j < c.n_kv) return;
+    c.unit += int64_t(kGroups) * gridDim.x;
+    ++c.u;
+    c.j = 0;
+    if (c.unit < n_units) {
+      c.it = unit_of(c.unit);
+      c.n_kv = (c.it.nk + kKeys - 1) / kKeys;
+    }
+  };
+  auto live = [&](const Cur& c) { return c.unit < n_units; };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      Cur c[kGroups];
+      for (int grp = 0; grp < kGroups; ++grp) start(c[grp], grp);
+      int kc = 0, nq[kGroups] = {0, 0};
+      bool stop = false;
+      while (!stop && (live(c[0]) || live(c[1]))) {
+        for (int grp = 0; grp < kGroups && !stop; ++grp) {
+          Cur& cg = c[grp];
+          if (!live(cg)) continue;
+          const int h = int(cg.unit % p.n_heads), hk = h / p.group;
+          if (cg.j == 0) {  // the unit's Q tile, once the group's previous unit has no S left to issue
+            if (!wait(gbar(Q_EMPTY, grp), (cg.u & 1) ^ 1)) {
+              stop = true;
+              break;
+            }
+            mbar_arrive_expect_tx(gbar(Q_FULL, grp), Sh::kQBytes);
+            for (int b = 0; b < Sh::kBlocks; ++b)
+              tma_load_3d(sQ + grp * Sh::kQBytes + b * (kRows * 128), &p.q_map, gbar(Q_FULL, grp), b * 64, h,
+                          cg.it.q0 + cg.it.tile * kRows);
+            ++nq[grp];
+          }
+          const int sk = kc % Sh::kKStages, sv = kc % Sh::kVStages;
+          const int32_t krow = cg.it.k0 + cg.j * kKeys;
+          if (!wait(bar(K_EMPTY + sk), ((kc / Sh::kKStages) & 1) ^ 1)) {
+            stop = true;
+            break;
+          }
+          mbar_arrive_expect_tx(bar(K_FULL + sk), kKvBytes);
+          for (int b = 0; b < Sh::kBlocks; ++b)
+            tma_load_3d(sK + sk * kKvBytes + b * (kKeys * 128), &p.k_map, bar(K_FULL + sk), b * 64, hk, krow);
+          if (!wait(bar(V_EMPTY + sv), ((kc / Sh::kVStages) & 1) ^ 1)) {
+            stop = true;
+            // this tile's K has been issued and its V has not: drained below as one more K
+            mbar_wait(bar(K_FULL + sk), (kc / Sh::kKStages) & 1);
+            break;
+          }
+          mbar_arrive_expect_tx(bar(V_FULL + sv), kKvBytes);
+          for (int b = 0; b < Sh::kBlocks; ++b)
+            tma_load_3d(sV + sv * kKvBytes + b * (kKeys * 128), &p.v_map, bar(V_FULL + sv), b * 64, hk, krow);
+          ++kc;
+          advance(cg);
+        }
+      }
+      if (aborted(s_abort)) {  // loads nobody consumed must land before the CTA exits (bounded)
+        for (int q = (kc > Sh::kKStages ? kc - Sh::kKStages : 0); q < kc; ++q)
+          mbar_wait(bar(K_FULL + q % Sh::kKStages), (q / Sh::kKStages) & 1);
+        for (int q = (kc > Sh::kVStages ? kc - Sh::kVStages : 0); q < kc; ++q)
+          mbar_wait(bar(V_FULL + q % Sh::kVStages), (q / Sh::kVStages) & 1);
+        for (int grp = 0; grp < kGroups; ++grp)  // only a group's latest Q can be unconsumed
+          if (nq[grp] > 0) mbar_wait(gbar(Q_FULL, grp), (nq[grp] - 1) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const int nks = (p.d + 15) / 16;  // 16-column steps of a head's row
+      const uint32_t idesc_o = umma_idesc_f16(DT<T>::umma_fmt, kRows, uint32_t(nks) * 16, /*a_mn=*/0, /*b_mn=*/1);
+      struct Prev { bool valid, first, last; int t, u, kv, nk; };  // nk: 16-key steps of O += P V
+      Cur c[kGroups];
+      Prev prev[kGroups];
+      for (int grp = 0; grp < kGroups; ++grp) {
+        start(c[grp], grp);
+        prev[grp].valid = false;
+      }
+      int kc = 0;
+      bool stop = false;
+      // O_grp += P V for the group's previous tile
+      auto pv = [&](int grp, const Prev& e) -> bool {
+        const int sv = e.kv % Sh::kVStages;
+        if (!wait(gbar(P_FULL, grp), e.t & 1)) return false;
+        if (!wait(bar(V_FULL + sv), (e.kv / Sh::kVStages) & 1)) return false;
+        if (e.first && !wait(gbar(O_EMPTY, grp), (e.u & 1) ^ 1)) return false;
+        tc_fence_after();
+        const uint32_t pb = sP + grp * Sh::kPBytes;
+        const uint32_t vb = sV + sv * kKvBytes;
+#pragma unroll
+        for (int t = 0; t < kKeys / 16; ++t) {
+          if (t >= e.nk) break;
+          umma_f16(tmem + Sh::kOCol + kD * grp, smem_desc(pb + (t >> 2) * (kRows * 128) + (t & 3) * 32, 16, 1024, 2),
+                   smem_desc(vb + t * 2048, kKeys * 128, 1024, 2), idesc_o, (e.first && t == 0) ? 0u : 1u);
+        }
+        umma_commit(gbar(P_EMPTY, grp));
+        umma_commit(bar(V_EMPTY + sv));
+        if (e.last) umma_commit(gbar(O_FULL, grp));
+        return true;
+      };
+      while (!stop && (live(c[0]) || live(c[1]) || prev[0].valid || prev[1].valid)) {
+        for (int grp = 0; grp < kGroups && !stop; ++grp) {
+          Cur& cg = c[grp];
+          Prev cur{false, false, false, 0, 0, 0, 0};
+          if (live(cg)) {
+            const int sk = kc % Sh::kKStages, sb = kc % Sh::kSBufs;
+            if ((cg.j == 0 && !wait(gbar(Q_FULL, grp), cg.u & 1)) ||
+                !wait(bar(K_FULL + sk), (kc / Sh::kKStages) & 1) ||
+                !wait(bar(S_EMPTY + sb), ((kc / Sh::kSBufs) & 1) ^ 1)) {
+              stop = true;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t qa = sQ + grp * Sh::kQBytes, kb = sK + sk * kKvBytes;
+            // S over the tile's keys, to the next multiple of 16
+            const int n16 = (min(kKeys, cg.it.nk - cg.j * kKeys) + 15) / 16;
+            const uint32_t idesc = umma_idesc_f16(DT<T>::umma_fmt, kRows, uint32_t(n16) * 16, 0, 0);
+#pragma unroll
+            for (int t = 0; t < kD / 16; ++t) {
+              if (t >= nks) break;
+              umma_f16(tmem + kKeys * sb, smem_desc(qa + (t >> 2) * (kRows * 128) + (t & 3) * 32, 16, 1024, 2),
+                       smem_desc(kb + (t >> 2) * (kKeys * 128) + (t & 3) * 32, 16, 1024, 2), idesc, t > 0 ? 1u : 0u);
+            }
+            umma_commit(bar(S_FULL + sb));
+            umma_commit(bar(K_EMPTY + sk));
+            if (cg.j == cg.n_kv - 1) umma_commit(gbar(Q_EMPTY, grp));
+            cur = Prev{true, cg.j == 0, cg.j == cg.n_kv - 1, cg.t, cg.u, kc, n16};
+            ++kc;
+            advance(cg);
+          }
+          if (prev[grp].valid && !pv(grp, prev[grp])) {
+            stop = true;
+            break;
+          }
+          prev[grp] = cur;
+        }
+      }
+      if (aborted(s_abort)) {  // every issued MMA must finish before TMEM is released (bounded)
+        umma_commit(bar(DRAIN));
+        mbar_wait(bar(DRAIN), 0);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax groups (warps 2..9)
+    const int grp = (warp - 2) >> 2;
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const uint32_t lane_addr = tmem + (uint32_t(quad * 32) << 16);
+    const uint32_t o_addr = lane_addr + Sh::kOCol + kD * grp;   // this row of the group's O
+    const uint32_t prow = (row >> 3) * 1024 + (row & 7) * 128;  // this row in a SW128 block
+    const uint32_t pb = sP + grp * Sh::kPBytes - base;
+    const float2 sl2 = f2(p.scale_log2);
+    // The MMA warp issues the groups' S tiles round-robin (group 0 first), so this
+    // group's n-th tile is global tile n + min(n + grp, tiles of the other group).
+    int other_tiles = 0;
+    {
+      Cur o;
+      start(o, grp ^ 1);
+      while (live(o)) {
+        other_tiles += o.n_kv;
+        o.j = o.n_kv - 1;
+        advance(o);
+      }
+    }
+    Cur c;
+    start(c, grp);
+    float m = -INFINITY, l = 0.f;
+    while (live(c)) {
+      const int t = c.t, j = c.j;
+      const int kc = t + min(t + grp, other_tiles);
+      const int sb = kc % Sh::kSBufs;
+      const uint32_t s_addr = lane_addr + kKeys * sb;
+      const Unit it = c.it;
+      const int64_t unit = c.unit;
+      const int uu = c.u;
+      const bool last = j == c.n_kv - 1;
+      const int nvalid = min(kKeys, it.nk - j * kKeys);
+      // a warp whose 32 query rows all lie past the queries' end does no softmax (its P rows
+      // only feed O rows that are never stored)
+      const bool rows_live = quad * 32 < it.nq - it.tile * kRows;
+      const int n_half = (nvalid + 63) / 64;
+      const bool work = __all_sync(0xffffffffu, wait(bar(S_FULL + sb), (kc / Sh::kSBufs) & 1));
+      tc_fence_after();
+      // pass 1: the row max over the valid keys, 64 columns at a time
+      float mx = -INFINITY;
+      if (work && rows_live) {
+#pragma unroll 1
+        for (int hh = 0; hh < n_half; ++hh) {
+          uint32_t sv[64];
+          tmem_ld64(s_addr + hh * 64, sv);
+          if (nvalid < hh * 64 + 64) {  // warp-uniform: keys past the end do not count
+#pragma unroll
+            for (int q = 0; q < 64; ++q)
+              if (hh * 64 + q >= nvalid) sv[q] = __float_as_uint(-INFINITY);
+          }
+          float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int q = 0; q < 64; q += 2)
+            mxs[(q >> 1) & 3] = max3(mxs[(q >> 1) & 3], __uint_as_float(sv[q]), __uint_as_float(sv[q + 1]));
+          mx = max3(mx, fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
+        }
+        mx *= sl2.x;  // the scale is positive: max commutes with it
+      }
+      const float m_new = (j == 0 || mx > m + kMaxSlack) ? mx : m;
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;  // every score so far is -inf: p = 0
+      const float alpha = (j == 0) ? 1.f : sfu_ex2(m - m_use);
+      // the previous tile's O += P V has finished: P may be overwritten, O rescaled
+      const bool go = __all_sync(0xffffffffu, work && wait(gbar(P_EMPTY, grp), (t & 1) ^ 1));
+      if (go && rows_live && j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        tc_fence_after();
+#pragma unroll 1
+        for (int b = 0; b < Sh::kBlocks; ++b) {
+          uint32_t ov[64];
+          tmem_ld64(o_addr + b * 64, ov);
+#pragma unroll
+          for (int q = 0; q < 64; ++q) ov[q] = __float_as_uint(__uint_as_float(ov[q]) * alpha);
+          tmem_st64(o_addr + b * 64, ov);
+        }
+      }
+      // pass 2: p = 2^(s - max), rounded to T into the group's SW128 K-major P tile
+      float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      if (go && rows_live) {
+        const float2 neg_m = f2(-m_use);
+#pragma unroll 1
+        for (int hh = 0; hh < n_half; ++hh) {
+          uint32_t sv[64];
+          tmem_ld64(s_addr + hh * 64, sv);
+          if (nvalid < hh * 64 + 64) {  // warp-uniform: keys past the end score -inf, so p = 0
+#pragma unroll
+            for (int q = 0; q < 64; ++q)
+              if (hh * 64 + q >= nvalid) sv[q] = __float_as_uint(-INFINITY);
+          }
+#pragma unroll
+          for (int c8 = 0; c8 < 8; ++c8) {  // 16-byte chunks = 8 keys
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int col = c8 * 8 + 2 * i;
+              const float2 x = f2_fma(make_float2(__uint_as_float(sv[col]), __uint_as_float(sv[col + 1])), sl2, neg_m);
+              const float2 pr = make_float2(sfu_ex2(x.x), sfu_ex2(x.y));
+              sums[i & 1] = f2_add(sums[i & 1], pr);
+              w[i] = Pack2<T>::pack(pr.x, pr.y);
+            }
+            *reinterpret_cast<uint4*>(gbase + pb + hh * (kRows * 128) + prow + ((c8 ^ (row & 7)) << 4)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(S_EMPTY + sb));  // S has been read: the buffer may take the next S
+      const float sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+      l = (j == 0) ? sum : l * alpha + sum;
+      m = m_new;
+      // the last 16-key step of a tile that ends inside it multiplies value rows past the
+      // sequence's end by p = 0: those rows become zeros first (they may hold NaN)
+      if ((nvalid & 15) != 0) {
+        const int sv = kc % Sh::kVStages;
+        if (__all_sync(0xffffffffu, go && wait(bar(V_FULL + sv), (kc / Sh::kVStages) & 1))) {
+          const int n_zero = 16 - (nvalid & 15);
+          uint8_t* vrow = gbase + (sV + sv * kKvBytes - base) + nvalid * 128;
+          for (int i = row; i < n_zero * 8 * Sh::kBlocks; i += kRows) {
+            const int b = i / (n_zero * 8), x = i % (n_zero * 8);
+            *reinterpret_cast<uint4*>(vrow + b * (kKeys * 128) + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(gbar(P_FULL, grp));
+      advance(c);
+      if (last) {
+        // the unit's output: O / l, once its last O += P V has finished
+        if (__all_sync(0xffffffffu, wait(gbar(O_FULL, grp), uu & 1)) && rows_live) {
+          tc_fence_after();
+          const int qr = it.tile * kRows + row;
+          const float inv = it.what == 2 || l == 0.f ? 0.f : 1.f / l;
+          T* dst = reinterpret_cast<T*>(p.out) + int64_t(it.q0 + qr) * p.ldo + int64_t(unit % p.n_heads) * p.d;
+#pragma unroll 1
+          for (int b = 0; b < Sh::kBlocks; ++b) {
+            uint32_t ov[64];
+            tmem_ld64(o_addr + b * 64, ov);
+            if (qr < it.nq && it.what != 1) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                if (b * 64 + q * 8 >= p.d) break;
+                uint4 w;
+                if (it.what == 2) {  // no keys: zeros, whatever the key row read in their place holds
+                  w = make_uint4(0u, 0u, 0u, 0u);
+                } else {
+                  w.x = Pack2<T>::pack(__uint_as_float(ov[8 * q + 0]) * inv, __uint_as_float(ov[8 * q + 1]) * inv);
+                  w.y = Pack2<T>::pack(__uint_as_float(ov[8 * q + 2]) * inv, __uint_as_float(ov[8 * q + 3]) * inv);
+                  w.z = Pack2<T>::pack(__uint_as_float(ov[8 * q + 4]) * inv, __uint_as_float(ov[8 * q + 5]) * inv);
+                  w.w = Pack2<T>::pack(__uint_as_float(ov[8 * q + 6]) * inv, __uint_as_float(ov[8 * q + 7]) * inv);
+                }
+                reinterpret_cast<uint4*>(dst + b * 64)[q] = w;
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(gbar(O_EMPTY, grp));
+      }
+    }
+  }
+
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
+
+int encode_rows(CUtensorMap* map, int dtype, const void* base, int64_t ld, int64_t rows, int heads, int d, int box_rows,
+                const char* what) {
+  PFN_encodeTiled enc = get_encode_tiled();
+  if (enc == nullptr) return set_error(LF_ERR_DRIVER, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[3] = {cuuint64_t(d), cuuint64_t(heads), cuuint64_t(rows)};
+  const cuuint64_t strides[2] = {cuuint64_t(d) * 2, cuuint64_t(ld) * 2};
+  const cuuint32_t box[3] = {64, 1, cuuint32_t(box_rows)}, estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, dtype == LF_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(LF_ERR_CUDA, "lf_cross_attention_varlen: cuTensorMapEncodeTiled(%s) failed: %d", what, int(r));
+  return LF_OK;
+}
+
+template <typename T, int kD, int MT>
+int launch_decode(const CrossParams& p, unsigned row_blocks, cudaStream_t s) {
+  auto kern = cross_decode_kernel<T, kD, MT>;
+  constexpr int smem = decode_smem(kD, MT);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute(cross_decode)");
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(p.split);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(p.n_items) * unsigned(p.n_kv_heads) * unsigned(p.split), row_blocks);
+  cfg.blockDim = dim3(32 * kDecodeWarps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.split > 1 ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, p);
+  if (e != cudaSuccess) return cuda_error(e, "launch cross_decode");
+  count_launch();
+  return LF_OK;
+}
+
+template <typename T, int kD>
+int launch_prompt(const CrossParams& p, int sms, cudaStream_t s) {
+  auto kern = cross_prompt_kernel<T, kD>;
+  constexpr int smem = Shape<kD>::kSmem;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute(cross_prompt)");
+  const int64_t units = int64_t(p.n_items) * p.n_heads;
+  e = launch_pdl(kern, dim3(unsigned(units < sms ? units : sms)), dim3(kThreads), smem, s, p);
+  if (e != cudaSuccess) return cuda_error(e, "launch cross_prompt");
+  count_launch();
+  return LF_OK;
+}
+
+}  // namespace
+
+}  // namespace lf
+
+using namespace lf;
+
+extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q, int64_t ldq, int64_t n_q,
+                                         const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t n_kv,
+                                         int n_heads, int n_kv_heads, int head_dim, const int32_t* items, int n_items,
+                                         int max_q, int max_kv, float scale, void* out, int64_t ld_out,
+                                         int32_t* status) {
+  const char* fn = "lf_cross_attention_varlen";
+  if (dtype != LF_DTYPE_BF16 && dtype != LF_DTYPE_F16)
+    return set_error(LF_ERR_UNSUPPORTED, "%s: dtype %d (bf16 or f16 only)", fn, dtype);
+  if (head_dim <= 0 || head_dim > 128 || head_dim % 8 != 0)
+    return set_error(LF_ERR_UNSUPPORTED, "%s: head_dim %d (a multiple of 8 up to 128)", fn, head_dim);
+  if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0)
+    return set_error(LF_ERR_INVALID, "%s: %d heads over %d key heads", fn, n_heads, n_kv_heads);
+  if (n_q < 0 || n_kv < 0 || n_q > INT32_MAX - 128 || n_kv > INT32_MAX - 128 || n_items < 0 || max_q < 0 || max_kv < 0)
+    return set_error(LF_ERR_INVALID, "%s: bad sizes", fn);
+  if (!(scale > 0.f) || !std::isfinite(scale)) return set_error(LF_ERR_INVALID, "%s: scale must be positive and finite", fn);
+  if (n_items == 0 || n_q == 0 || max_q == 0) return LF_OK;
+  if (q == nullptr || out == nullptr || items == nullptr || (n_kv > 0 && (k == nullptr || v == nullptr)))
+    return set_error(LF_ERR_INVALID, "%s: null q, k, v, items or out", fn);
+  const int64_t wq = int64_t(n_heads) * head_dim, wk = int64_t(n_kv_heads) * head_dim;
+  if (ldq < wq || ld_out < wq || (n_kv > 0 && (ldk < wk || ldv < wk)))
+    return set_error(LF_ERR_INVALID, "%s: a row stride is below its row", fn);
+  if (!aligned16(q) || !aligned16(out) || !aligned16(items) || ldq % 8 || ld_out % 8 ||
+      (n_kv > 0 && (!aligned16(k) || !aligned16(v) || ldk % 8 || ldv % 8)))
+    return set_error(LF_ERR_INVALID, "%s: pointers and row strides must be 16-byte aligned", fn);
+  CrossParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.ldq = ldq;
+  p.ldk = ldk;
+  p.ldv = ldv;
+  p.n_q = n_q;
+  p.n_kv = n_kv;
+  p.n_heads = n_heads;
+  p.n_kv_heads = n_kv_heads;
+  p.group = n_heads / n_kv_heads;
+  p.d = head_dim;
+  p.items = reinterpret_cast<const int4*>(items);
+  p.n_items = n_items;
+  p.max_q = max_q;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.out = out;
+  p.ldo = ld_out;
+  p.status = status;
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf = dtype == LF_DTYPE_BF16;
+  const int64_t rows = int64_t(max_q) * p.group;
+  const bool decode = max_q <= kRows && rows <= 32;
+  if (decode) {
+    const int mt = rows <= 16 ? 1 : 2;
+    const int64_t blocks = (rows + 16 * mt - 1) / (16 * mt);
+    const int64_t units = int64_t(n_items) * n_kv_heads;
+    if (units * 8 > INT32_MAX || blocks > 65535) return set_error(LF_ERR_UNSUPPORTED, "%s: too many records", fn);
+    p.split = 1;
+    while (p.split < 8 && max_kv / (2 * p.split) >= 64 && (units * blocks * p.split < 2 * sms || max_kv / p.split > 1024))
+      p.split *= 2;
+    const unsigned rb = unsigned(blocks);
+    if (head_dim <= 64) {
+      if (mt == 1) return bf ? launch_decode<__nv_bfloat16, 64, 1>(p, rb, s) : launch_decode<__half, 64, 1>(p, rb, s);
+      return bf ? launch_decode<__nv_bfloat16, 64, 2>(p, rb, s) : launch_decode<__half, 64, 2>(p, rb, s);
+    }
+    if (mt == 1) return bf ? launch_decode<__nv_bfloat16, 128, 1>(p, rb, s) : launch_decode<__half, 128, 1>(p, rb, s);
+    return bf ? launch_decode<__nv_bfloat16, 128, 2>(p, rb, s) : launch_decode<__half, 128, 2>(p, rb, s);
+  }
+  const int key_tile = head_dim <= 64 ? Shape<64>::kKeys : Shape<128>::kKeys;
+  int rc;
+  if ((rc = encode_rows(&p.q_map, dtype, q, ldq, n_q, n_heads, head_dim, kRows, "q"))) return rc;
+  // no keys at all: the row read in the place of one (its result is not used) is a query row
+  const void *kb = n_kv > 0 ? k : q, *vb = n_kv > 0 ? v : q;
+  const int64_t kv_rows = n_kv > 0 ? n_kv : n_q;
+  if ((rc = encode_rows(&p.k_map, dtype, kb, n_kv > 0 ? ldk : ldq, kv_rows, n_kv_heads, head_dim, key_tile, "k"))) return rc;
+  if ((rc = encode_rows(&p.v_map, dtype, vb, n_kv > 0 ? ldv : ldq, kv_rows, n_kv_heads, head_dim, key_tile, "v"))) return rc;
+  if (head_dim <= 64) return bf ? launch_prompt<__nv_bfloat16, 64>(p, sms, s) : launch_prompt<__half, 64>(p, sms, s);
+  return bf ? launch_prompt<__nv_bfloat16, 128>(p, sms, s) : launch_prompt<__half, 128>(p, sms, s);
+}

@@ -5,8 +5,9 @@ library's tcgen05 GEMM; ``add_layernorm`` is ``nn.LayerNorm(sublayer_out + resid
 HBM (``src/latefuse/model/encoder.py:137,141``; with no residual, the embeddings'
 LayerNorm at ``:275``), ``gelu`` is the exact erf GELU of the FFN (``:122,139``),
 both with torch's rounding points, and ``attention_varlen`` is the encoder's
-masked self-attention (``:82-98``) on a padding-free batch (see the
-``lf_*`` declarations in ``include/latefuse_b200.h``).
+masked self-attention (``:82-98``) on a padding-free batch, and
+``cross_attention_varlen`` is the attention of other queries to the packed states such
+a batch gives (see the ``lf_*`` declarations in ``include/latefuse_b200.h``).
 """
 
 from __future__ import annotations
@@ -15,6 +16,7 @@ import torch
 from torch import Tensor
 
 from latefuse_b200 import _native as nat
+from latefuse_b200.packing import CrossBatch
 
 
 def _rows(t: Tensor) -> tuple[Tensor, int]:
@@ -103,6 +105,48 @@ def attention_varlen(qkv: Tensor, n_heads: int, items: Tensor, scale: float, out
                                        float(scale), out.data_ptr(), out.stride(0), nat.ptr(status))
     nat.check(rc, "lf_attention_varlen")
     return out
+
+
+def cross_attention_varlen(q: Tensor, k: Tensor, v: Tensor, batch: CrossBatch, n_heads: int,
+                           n_kv_heads: int | None = None, scale: float | None = None, out: Tensor | None = None,
+                           status: Tensor | None = None) -> Tensor:
+    """Attention of packed queries to packed encoder states of other lengths: each sequence
+    of ``batch`` (:func:`~latefuse_b200.packing.cross_batch`) attends to its own keys.
+    ``q (Tq, n_heads * d)``, ``k`` and ``v (Tk, n_kv_heads * d)`` bf16 or f16 with contiguous
+    rows of any stride that is a multiple of 8 (column slices of a fused projection are
+    fine); d a multiple of 8 up to 128; consecutive ``n_heads / n_kv_heads`` query heads
+    share a key head (``n_kv_heads`` None: as many as ``n_heads``); ``scale`` positive, None:
+    ``d ** -0.5``.  A sequence without keys gives zeros; rows of ``out`` in no sequence are
+    left as they were (undefined when ``out`` is None).  Returns ``out (Tq, n_heads * d)``."""
+    dev = nat.require_cuda(q, k, v, batch.items, out, status)
+    n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
+    tq, width = q.shape
+    if n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads or width % n_heads:
+        raise ValueError(f"{width} columns of {n_heads} heads over {n_kv_heads} key heads")
+    d = width // n_heads
+    if k.shape != v.shape or k.shape[1] != n_kv_heads * d or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"k and v must be (Tk, {n_kv_heads * d}) {q.dtype}, got {k.dtype} {tuple(k.shape)} and "
+                         f"{v.dtype} {tuple(v.shape)}")
+    if batch.n_q > tq or batch.n_kv > k.shape[0]:
+        raise ValueError(f"the batch names {batch.n_q} query and {batch.n_kv} key rows, q has {tq} and k {k.shape[0]}")
+    if q.stride(1) != 1 or k.stride(1) != 1 or v.stride(1) != 1:
+        raise ValueError("rows of q, k and v must be contiguous")
+    if out is None:
+        out = torch.empty(tq, width, dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != (tq, width) or out.stride(1) != 1:
+        raise ValueError(f"out must be a ({tq}, {width}) {q.dtype} tensor with contiguous rows")
+    with nat.on_device(dev):
+        rc = nat.lib().lf_cross_attention_varlen(
+            nat.stream_ptr(dev), nat.dtype_code(q.dtype), q.data_ptr(), _ld(q), tq, k.data_ptr(), _ld(k), v.data_ptr(),
+            _ld(v), k.shape[0], n_heads, n_kv_heads, d, batch.items.data_ptr(), batch.items.shape[0], batch.max_q,
+            batch.max_kv, d ** -0.5 if scale is None else float(scale), out.data_ptr(), _ld(out), nat.ptr(status))
+    nat.check(rc, "lf_cross_attention_varlen")
+    return out
+
+
+def _ld(t: Tensor) -> int:
+    """Row stride in elements (a single row's is its width: torch leaves it arbitrary)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 ACT_NONE, ACT_GELU = 0, 1

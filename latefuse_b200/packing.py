@@ -72,6 +72,59 @@ def attention_items(starts, lengths) -> np.ndarray:
     return items
 
 
+@dataclass
+class CrossBatch:
+    """Which rows of the queries and of the encoder's states belong together in
+    :func:`~latefuse_b200.encoder_ops.cross_attention_varlen`, on the device.  It depends
+    on the lengths alone: one is built per batch of texts and serves every layer and,
+    for single tokens, every step."""
+
+    n_seqs: int
+    n_q: int          # query rows: at least the end of the last query range
+    n_kv: int         # state rows: at least the end of the last key range
+    max_q: int
+    max_kv: int
+    items: Tensor     # (n, 8) int32 {q_start, q_len, kv_start, kv_len, q_tile, 0, 0, 0}, most work first
+
+
+def cross_batch(q_lengths, kv_lengths, device, q_starts=None, kv_starts=None) -> CrossBatch:
+    """The work list of a cross attention: sequence s has ``q_lengths[s]`` query rows and
+    ``kv_lengths[s]`` rows of encoder states (either may be 0).  Rows lie packed one
+    sequence after the other unless ``q_starts`` / ``kv_starts`` name the first row of
+    each: several sequences may share a range of states (beams of one text), query
+    ranges may not overlap."""
+    ql, kl = np.asarray(q_lengths, dtype=np.int64), np.asarray(kv_lengths, dtype=np.int64)
+    if ql.ndim != 1 or ql.shape != kl.shape:
+        raise ValueError(f"one query and one key length per sequence are needed, got {ql.shape} and {kl.shape}")
+    qs = np.cumsum(ql) - ql if q_starts is None else np.asarray(q_starts, dtype=np.int64)
+    ks = np.cumsum(kl) - kl if kv_starts is None else np.asarray(kv_starts, dtype=np.int64)
+    if qs.shape != ql.shape or ks.shape != kl.shape:
+        raise ValueError(f"{ql.shape[0]} sequences but {qs.shape[0]} query and {ks.shape[0]} key starts")
+    if ql.size and min(ql.min(), kl.min(), qs.min(), ks.min()) < 0:
+        raise ValueError("lengths and starts must not be negative")
+    n_q, n_kv = (int((st + ln).max()) if ln.size else 0 for st, ln in ((qs, ql), (ks, kl)))
+    if max(n_q, n_kv) > 2**31 - 129:
+        raise ValueError("row numbers must fit 32 bits")
+    held = ql > 0
+    by_start = np.argsort(qs[held], kind="stable")
+    if (qs[held][by_start][1:] < (qs + ql)[held][by_start][:-1]).any():
+        raise ValueError("query ranges overlap")
+    order = np.flatnonzero(held)
+    order = order[np.argsort(-kl[order], kind="stable")]
+    reps = (ql[order] + 127) // 128
+    total = int(reps.sum())
+    items = np.zeros((total, 8), dtype=np.int32)
+    for col, values in enumerate((qs, ql, ks, kl)):
+        items[:, col] = np.repeat(values[order], reps)
+    items[:, 4] = np.arange(total) - np.repeat(np.cumsum(reps) - reps, reps)
+    device = torch.device(device)
+    host = torch.from_numpy(items)
+    if device.type == "cuda":
+        host = host.pin_memory()
+    return CrossBatch(n_seqs=int(ql.size), n_q=n_q, n_kv=n_kv, max_q=int(ql.max()) if ql.size else 0,
+                      max_kv=int(kl.max()) if kl.size else 0, items=host.to(device, non_blocking=True))
+
+
 def pack_rows(input_ids: Tensor, lengths: list[int], slots: list[int], position_pad: int | None,
               token_type_ids: Tensor | None, device: torch.device) -> PackedBatch:
     """Pack the real tokens of right-padded host rows (``1 <= lengths[b] <= S``).
