@@ -459,6 +459,31 @@ int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t ldx, const 
                    const int8_t* w, int64_t ldw, const float* w_scale, const void* bias,
                    void* y, int64_t ldy, int64_t m, int n, int k, int act, int32_t* status);
 
+/* lf_quantize_rows of x (m, k) into the workspace, then lf_linear_int8: the 8-bit projection
+ * of float rows in one call of two launches.  The workspace (256-byte aligned, at least
+ * lf_linear_rows_int8_workspace_bytes) is free again when the launches have run, so calls
+ * that may overlap on the GPU need one each. */
+size_t lf_linear_rows_int8_workspace_bytes(int64_t m, int k);
+int lf_linear_rows_int8(void* stream, int dtype, const void* x, int64_t ldx, const int8_t* w, int64_t ldw,
+                        const float* w_scale, const void* bias, void* y, int64_t ldy, int64_t m, int n, int k,
+                        int act, void* workspace, size_t workspace_bytes, int32_t* status);
+
+/* The encoder layer's feed-forward half with both projections in 8-bit integers:
+ *     h = LayerNorm(round(a + r)) * gamma + beta          (as lf_add_layernorm; r may be NULL)
+ *     o = down(round(act(up(h))))
+ * up (inner, hidden) and down (hidden, inner) int8 with a scale per row, h and the middle
+ * activations quantised per token as lf_quantize_rows does; biases may be NULL.  One call
+ * of four launches over one workspace (rules as for lf_linear_rows_int8).  Alignment of a, r,
+ * gamma, beta and h as lf_add_layernorm, of up and down as lf_linear_int8; hidden a
+ * multiple of 8 up to 4096, inner up to 131072. */
+size_t lf_ffn_int8_workspace_bytes(int dtype, int64_t m, int hidden, int inner);
+int lf_ffn_int8(void* stream, int dtype, const void* a, int64_t lda, const void* r, int64_t ldr,
+                const void* gamma, const void* beta, float eps, const int8_t* up, int64_t ld_up,
+                const float* up_scale, const void* up_bias, const int8_t* down, int64_t ld_down,
+                const float* down_scale, const void* down_bias, int64_t m, int hidden, int inner, int act,
+                void* h, int64_t ldh, void* o, int64_t ldo, void* workspace, size_t workspace_bytes,
+                int32_t* status);
+
 /* ------------------------------------------------------------------------
  * Encoder elementwise ops around the projections
  * ------------------------------------------------------------------------ */

@@ -118,6 +118,15 @@ SIGNATURES: dict[str, tuple] = {
     "lf_linear_int8": (c_int, [
         c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
         c_int64, c_int, c_int, c_int, c_void_p]),
+    "lf_linear_rows_int8_workspace_bytes": (c_size_t, [c_int64, c_int]),
+    "lf_linear_rows_int8": (c_int, [
+        c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int,
+        c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "lf_ffn_int8_workspace_bytes": (c_size_t, [c_int, c_int64, c_int, c_int]),
+    "lf_ffn_int8": (c_int, [
+        c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, ctypes.c_float, c_void_p, c_int64,
+        c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_int64,
+        c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
     "lf_gelu": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64]),
     "lf_attention_varlen": (c_int, [
         c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int,
@@ -187,26 +196,23 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of ``device`` as a pointer (without building a Stream object, which
+    takes as long as a small launch)."""
+    index = torch.cuda.current_device() if device.index is None else device.index
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
-class _SameDevice:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_same_device = _SameDevice()
-
-
-def on_device(device: torch.device):
-    """A context in which ``device`` is the current CUDA device (launches, kernel attributes
-    and tensor maps go by the current device): nothing to do when it already is."""
-    if device.index is None or torch.cuda.current_device() == device.index:
-        return _same_device
-    return torch.cuda.device(device)
+def call(fn, what: str, device: torch.device, *args) -> None:
+    """``fn(stream, *args)`` on the current stream of ``device``, with ``device`` current for
+    the call (launches and kernel attributes go by the current device), checked."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        rc = fn(stream_ptr(device), *args)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(stream_ptr(device), *args)
+    if rc != LF_OK:
+        check(rc, what)
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
@@ -215,15 +221,16 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     for t in tensors:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise NativeLibraryError(
                 f"latefuse_b200 kernels need CUDA tensors; got a tensor on {t.device}. "
                 "There is no CPU implementation of the serving path."
             )
+        d = t.device
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise NativeLibraryError(f"tensors on {dev} and {t.device}")
+            dev = d
+        elif d != dev:
+            raise NativeLibraryError(f"tensors on {dev} and {d}")
     return dev
 
 

@@ -37,6 +37,22 @@ void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 int option_force_simt() { return g_force_simt.load(); }
 int option_shrink_cluster() { return g_shrink_cluster.load(); }
 
+int current_device() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return dev;
+}
+
+int device_sms(int dev) {
+  static std::atomic<int> known[64];
+  int sms = dev >= 0 && dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
+    if (dev >= 0 && dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+  }
+  return sms;
+}
+
 void* get_driver_fn(const char* name) {
   void* fn = nullptr;
   cudaDriverEntryPointQueryResult q;

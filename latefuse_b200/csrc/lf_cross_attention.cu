@@ -865,10 +865,10 @@ int encode_rows(CUtensorMap* map, int dtype, const void* base, int64_t ld, int64
 }
 
 template <typename T, int kD, int MT>
-int launch_decode(const CrossParams& p, unsigned row_blocks, cudaStream_t s) {
-  auto kern = cross_decode_kernel<T, kD, MT>;
+int launch_decode(const CrossParams& p, unsigned row_blocks, int dev, cudaStream_t s) {
+  constexpr auto kern = cross_decode_kernel<T, kD, MT>;
   constexpr int smem = decode_smem(kD, MT);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem<kern>(dev, smem);
   if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute(cross_decode)");
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -891,12 +891,12 @@ int launch_decode(const CrossParams& p, unsigned row_blocks, cudaStream_t s) {
 }
 
 template <typename T, int kD>
-int launch_prompt(const CrossParams& p, int sms, cudaStream_t s) {
-  auto kern = cross_prompt_kernel<T, kD>;
+int launch_prompt(const CrossParams& p, int dev, cudaStream_t s) {
+  constexpr auto kern = cross_prompt_kernel<T, kD>;
   constexpr int smem = Shape<kD>::kSmem;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem<kern>(dev, smem);
   if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute(cross_prompt)");
-  const int64_t units = int64_t(p.n_items) * p.n_heads;
+  const int64_t units = int64_t(p.n_items) * p.n_heads, sms = device_sms(dev);
   e = launch_pdl(kern, dim3(unsigned(units < sms ? units : sms)), dim3(kThreads), smem, s, p);
   if (e != cudaSuccess) return cuda_error(e, "launch cross_prompt");
   count_launch();
@@ -954,9 +954,7 @@ extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q,
   p.out = out;
   p.ldo = ld_out;
   p.status = status;
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int dev = current_device(), sms = device_sms(dev);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == LF_DTYPE_BF16;
   const int64_t rows = int64_t(max_q) * p.group;
@@ -971,11 +969,11 @@ extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q,
       p.split *= 2;
     const unsigned rb = unsigned(blocks);
     if (head_dim <= 64) {
-      if (mt == 1) return bf ? launch_decode<__nv_bfloat16, 64, 1>(p, rb, s) : launch_decode<__half, 64, 1>(p, rb, s);
-      return bf ? launch_decode<__nv_bfloat16, 64, 2>(p, rb, s) : launch_decode<__half, 64, 2>(p, rb, s);
+      if (mt == 1) return bf ? launch_decode<__nv_bfloat16, 64, 1>(p, rb, dev, s) : launch_decode<__half, 64, 1>(p, rb, dev, s);
+      return bf ? launch_decode<__nv_bfloat16, 64, 2>(p, rb, dev, s) : launch_decode<__half, 64, 2>(p, rb, dev, s);
     }
-    if (mt == 1) return bf ? launch_decode<__nv_bfloat16, 128, 1>(p, rb, s) : launch_decode<__half, 128, 1>(p, rb, s);
-    return bf ? launch_decode<__nv_bfloat16, 128, 2>(p, rb, s) : launch_decode<__half, 128, 2>(p, rb, s);
+    if (mt == 1) return bf ? launch_decode<__nv_bfloat16, 128, 1>(p, rb, dev, s) : launch_decode<__half, 128, 1>(p, rb, dev, s);
+    return bf ? launch_decode<__nv_bfloat16, 128, 2>(p, rb, dev, s) : launch_decode<__half, 128, 2>(p, rb, dev, s);
   }
   const int key_tile = head_dim <= 64 ? Shape<64>::kKeys : Shape<128>::kKeys;
   int rc;
@@ -985,6 +983,6 @@ extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q,
   const int64_t kv_rows = n_kv > 0 ? n_kv : n_q;
   if ((rc = encode_rows(&p.k_map, dtype, kb, n_kv > 0 ? ldk : ldq, kv_rows, n_kv_heads, head_dim, key_tile, "k"))) return rc;
   if ((rc = encode_rows(&p.v_map, dtype, vb, n_kv > 0 ? ldv : ldq, kv_rows, n_kv_heads, head_dim, key_tile, "v"))) return rc;
-  if (head_dim <= 64) return bf ? launch_prompt<__nv_bfloat16, 64>(p, sms, s) : launch_prompt<__half, 64>(p, sms, s);
-  return bf ? launch_prompt<__nv_bfloat16, 128>(p, sms, s) : launch_prompt<__half, 128>(p, sms, s);
+  if (head_dim <= 64) return bf ? launch_prompt<__nv_bfloat16, 64>(p, dev, s) : launch_prompt<__half, 64>(p, dev, s);
+  return bf ? launch_prompt<__nv_bfloat16, 128>(p, dev, s) : launch_prompt<__half, 128>(p, dev, s);
 }

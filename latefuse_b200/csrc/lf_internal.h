@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/latefuse_b200.h"
 
 namespace lf {
@@ -248,6 +250,22 @@ typedef CUresult (*PFN_encodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_
                                     CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 PFN_encodeTiled get_encode_tiled();
 void* get_driver_fn(const char* name);
+
+// The current device and its SM count (asked of the runtime once per device).
+int current_device();
+int device_sms(int dev);
+
+// Lets kernel Kern use `bytes` of dynamic shared memory on device `dev`: the attribute
+// is per device and stays, so it is set on a kernel's first launch there.
+template <auto Kern>
+cudaError_t allow_smem(int dev, int bytes) {
+  static std::atomic<uint64_t> done{0};
+  const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t(1) << dev : 0;
+  if (bit != 0 && (done.load(std::memory_order_relaxed) & bit) != 0) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 // options
 int option_force_simt();

@@ -498,17 +498,10 @@ int encode(CUtensorMap* map, CUtensorMapDataType dt, int es, const void* base, i
   return LF_OK;
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
-template <typename K>
-int launch_cluster(K kern, const char* what, dim3 grid, int threads, int smem, int cluster, cudaStream_t s,
+template <auto Kern>
+int launch_cluster(const char* what, dim3 grid, int threads, int smem, int cluster, int dev, cudaStream_t s,
                    const LinearInt8Params& p) {
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem<Kern>(dev, smem);
   if (e != cudaSuccess) return cuda_error(e, what);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -524,32 +517,37 @@ int launch_cluster(K kern, const char* what, dim3 grid, int threads, int smem, i
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, kern, p);
+  e = cudaLaunchKernelEx(&cfg, Kern, p);
   if (e != cudaSuccess) return cuda_error(e, what);
   count_launch();
   return LF_OK;
 }
 
 template <typename T, int kAct>
-int launch_batch(LinearInt8Params& p, cudaStream_t s) {
+int launch_batch(LinearInt8Params& p, int dev, cudaStream_t s) {
   p.n_tiles_n = (p.n + kBN - 1) / kBN;
   p.n_tiles = (p.m_rows + 2 * kBM - 1) / (2 * kBM) * p.n_tiles_n;
-  const int64_t pairs = sm_count() / 2;
+  const int64_t pairs = device_sms(dev) / 2;
   const unsigned grid = unsigned(2 * (p.n_tiles < pairs ? p.n_tiles : pairs));
-  return launch_cluster(linear_int8_kernel<T, kAct>, "launch linear_int8", dim3(grid), kThreads,
-                        smem_bytes(sizeof(T)), 2, s, p);
+  return launch_cluster<linear_int8_kernel<T, kAct>>("launch linear_int8", dim3(grid), kThreads, smem_bytes(sizeof(T)),
+                                                     2, dev, s, p);
+}
+
+template <typename T, int NT, int kAct>
+int launch_split(LinearInt8Params& p, int dev, cudaStream_t s) {
+  p.n_tiles_n = (p.n + 127) / 128;
+  const dim3 grid(unsigned(p.n_tiles_n) * unsigned(p.split), unsigned((p.m_rows + NT - 1) / NT));
+  return launch_cluster<linear_int8_split_kernel<T, NT, kAct>>("launch linear_int8_split", grid, kSplitThreads,
+                                                               split_smem_bytes(NT), p.split, dev, s, p);
 }
 
 template <typename T, int kAct>
-int launch_split(LinearInt8Params& p, int nt, cudaStream_t s) {
-  p.n_tiles_n = (p.n + 127) / 128;
-  const unsigned mt = unsigned((p.m_rows + nt - 1) / nt);
-  const dim3 grid(unsigned(p.n_tiles_n) * unsigned(p.split), mt);
-  auto kern = nt == 16   ? linear_int8_split_kernel<T, 16, kAct>
-              : nt == 32 ? linear_int8_split_kernel<T, 32, kAct>
-              : nt == 64 ? linear_int8_split_kernel<T, 64, kAct>
-                         : linear_int8_split_kernel<T, 128, kAct>;
-  return launch_cluster(kern, "launch linear_int8_split", grid, kSplitThreads, split_smem_bytes(nt), p.split, s, p);
+int launch(LinearInt8Params& p, bool batch, int nt, int dev, cudaStream_t s) {
+  if (batch) return launch_batch<T, kAct>(p, dev, s);
+  if (nt == 16) return launch_split<T, 16, kAct>(p, dev, s);
+  if (nt == 32) return launch_split<T, 32, kAct>(p, dev, s);
+  if (nt == 64) return launch_split<T, 64, kAct>(p, dev, s);
+  return launch_split<T, 128, kAct>(p, dev, s);
 }
 
 }  // namespace
@@ -589,7 +587,7 @@ extern "C" int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t 
   p.status = status;
 
   // 256 x 256 tiles once they fill the CTA pairs; below that 128 channels x nt tokens
-  const int sms = sm_count();
+  const int dev = current_device(), sms = device_sms(dev);
   const int64_t big = ((m + 255) / 256) * ((n + 255) / 256);
   const bool batch = big > sms / 4;
   const int nt = batch ? 128 : m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
@@ -614,9 +612,7 @@ extern "C" int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto go = [&](auto tag) {
     using T = decltype(tag);
-    if (act == LF_ACT_GELU)
-      return batch ? launch_batch<T, LF_ACT_GELU>(p, s) : launch_split<T, LF_ACT_GELU>(p, nt, s);
-    return batch ? launch_batch<T, LF_ACT_NONE>(p, s) : launch_split<T, LF_ACT_NONE>(p, nt, s);
+    return act == LF_ACT_GELU ? launch<T, LF_ACT_GELU>(p, batch, nt, dev, s) : launch<T, LF_ACT_NONE>(p, batch, nt, dev, s);
   };
   if (dtype == LF_DTYPE_BF16) return go(__nv_bfloat16{});
   if (dtype == LF_DTYPE_F16) return go(__half{});

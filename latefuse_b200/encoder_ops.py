@@ -118,35 +118,37 @@ def cross_attention_varlen(q: Tensor, k: Tensor, v: Tensor, batch: CrossBatch, n
     share a key head (``n_kv_heads`` None: as many as ``n_heads``); ``scale`` positive, None:
     ``d ** -0.5``.  A sequence without keys gives zeros; rows of ``out`` in no sequence are
     left as they were (undefined when ``out`` is None).  Returns ``out (Tq, n_heads * d)``."""
-    dev = nat.require_cuda(q, k, v, batch.items, out, status)
+    items, dtype = batch.items, q.dtype
+    dev = nat.require_cuda(q, k, v, items, out, status)
     n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
     tq, width = q.shape
     if n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads or width % n_heads:
         raise ValueError(f"{width} columns of {n_heads} heads over {n_kv_heads} key heads")
     d = width // n_heads
-    if k.shape != v.shape or k.shape[1] != n_kv_heads * d or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError(f"k and v must be (Tk, {n_kv_heads * d}) {q.dtype}, got {k.dtype} {tuple(k.shape)} and "
+    tk, wk = k.shape
+    if v.shape != k.shape or wk != n_kv_heads * d or k.dtype != dtype or v.dtype != dtype:
+        raise ValueError(f"k and v must be (Tk, {n_kv_heads * d}) {dtype}, got {k.dtype} {tuple(k.shape)} and "
                          f"{v.dtype} {tuple(v.shape)}")
-    if batch.n_q > tq or batch.n_kv > k.shape[0]:
-        raise ValueError(f"the batch names {batch.n_q} query and {batch.n_kv} key rows, q has {tq} and k {k.shape[0]}")
-    if q.stride(1) != 1 or k.stride(1) != 1 or v.stride(1) != 1:
-        raise ValueError("rows of q, k and v must be contiguous")
+    if batch.n_q > tq or batch.n_kv > tk:
+        raise ValueError(f"the batch names {batch.n_q} query and {batch.n_kv} key rows, q has {tq} and k {tk}")
     if out is None:
-        out = torch.empty(tq, width, dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype or out.shape != (tq, width) or out.stride(1) != 1:
-        raise ValueError(f"out must be a ({tq}, {width}) {q.dtype} tensor with contiguous rows")
-    with nat.on_device(dev):
-        rc = nat.lib().lf_cross_attention_varlen(
-            nat.stream_ptr(dev), nat.dtype_code(q.dtype), q.data_ptr(), _ld(q), tq, k.data_ptr(), _ld(k), v.data_ptr(),
-            _ld(v), k.shape[0], n_heads, n_kv_heads, d, batch.items.data_ptr(), batch.items.shape[0], batch.max_q,
-            batch.max_kv, d ** -0.5 if scale is None else float(scale), out.data_ptr(), _ld(out), nat.ptr(status))
-    nat.check(rc, "lf_cross_attention_varlen")
+        out = torch.empty(tq, width, dtype=dtype, device=dev)
+    elif out.dtype != dtype or out.shape != q.shape:
+        raise ValueError(f"out must be a ({tq}, {width}) {dtype} tensor with contiguous rows")
+    nat.call(nat.lib().lf_cross_attention_varlen, "lf_cross_attention_varlen", dev, nat.dtype_code(dtype), q.data_ptr(),
+             _ld(q, tq, width), tq, k.data_ptr(), _ld(k, tk, wk), v.data_ptr(), _ld(v, tk, wk), tk, n_heads, n_kv_heads, d,
+             items.data_ptr(), items.shape[0], batch.max_q, batch.max_kv, d ** -0.5 if scale is None else float(scale),
+             out.data_ptr(), _ld(out, tq, width), nat.ptr(status))
     return out
 
 
-def _ld(t: Tensor) -> int:
-    """Row stride in elements (a single row's is its width: torch leaves it arbitrary)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _ld(t: Tensor, rows: int, width: int) -> int:
+    """Row stride in elements of ``rows`` contiguous rows (a single row's is its width:
+    torch leaves it arbitrary)."""
+    s0, s1 = t.stride()
+    if s1 != 1 and width > 1:
+        raise ValueError("rows of q, k, v and out must be contiguous")
+    return s0 if rows > 1 else width
 
 
 ACT_NONE, ACT_GELU = 0, 1

@@ -30,12 +30,16 @@ def _padded(n: int) -> int:
 
 
 def _rows(t: Tensor) -> tuple[Tensor, int]:
-    """``t`` as rows of its last dimension, each contiguous and at least a row apart."""
-    k = t.shape[-1]
-    t2 = t.reshape(-1, k)
-    if (k > 1 and t2.stride(1) != 1) or (t2.shape[0] > 1 and t2.stride(0) < k):
-        t2 = t2.contiguous()
-    return t2, max(t2.stride(0), k)
+    """``t`` as rows of its last dimension, each contiguous and at least a row apart, and
+    their stride."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    m, k = t.shape
+    s0, s1 = t.stride()
+    if (k > 1 and s1 != 1) or (m > 1 and s0 < k):
+        t = t.contiguous()
+        s0 = k
+    return t, (s0 if m > 1 else k)
 
 
 class Int8Rows:
@@ -43,10 +47,10 @@ class Int8Rows:
     ``scale`` the ``(M,)`` f32 scales, ``shape`` and ``dtype`` those of the tensor it came
     from (``shape[:-1]`` has M elements)."""
 
-    __slots__ = ("q", "scale", "shape", "dtype")
+    __slots__ = ("q", "scale", "shape", "dtype", "ld")
 
     def __init__(self, q: Tensor, scale: Tensor, shape: tuple, dtype: torch.dtype):
-        self.q, self.scale, self.shape, self.dtype = q, scale, tuple(shape), dtype
+        self.q, self.scale, self.shape, self.dtype, self.ld = q, scale, tuple(shape), dtype, q.stride(0)
 
     def dequantize(self) -> Tensor:
         """The values the integers stand for, in ``shape`` and ``dtype``."""
@@ -56,11 +60,11 @@ class Int8Rows:
 class Int8Weight:
     """An ``nn.Linear`` weight ``(N, K)`` in 8-bit integers with a scale per output channel.
 
-    ``Int8Weight(q, scale)`` takes int8 ``(N, K)`` in [-127, 127] and f32 ``(N,)`` (rows are
-    laid out 16-byte aligned once, here); ``Int8Weight.from_float(weight)`` quantises a
-    float weight on its GPU."""
+    ``Int8Weight(q, scale)`` takes int8 ``(N, K)`` in [-127, 127] and f32 ``(N,)`` (rows that
+    are not 16-byte aligned are laid out so once, here); ``Int8Weight.from_float(weight)``
+    quantises a float weight on its GPU."""
 
-    __slots__ = ("q", "scale")
+    __slots__ = ("q", "scale", "shape", "ld")
 
     def __init__(self, q: Tensor, scale: Tensor):
         if q.dim() != 2 or q.dtype != torch.int8:
@@ -70,10 +74,9 @@ class Int8Weight:
         n, k = q.shape
         if not 1 <= k <= _MAX_K or n < 1:
             raise ValueError(f"weight of {n} x {k}: K must be in 1..{_MAX_K}")
-        if q.stride(1) != 1 or q.stride(0) % 16 or q.stride(0) < k or q.data_ptr() % 16:
-            laid = torch.empty(n, _padded(k), dtype=torch.int8, device=q.device)[:, :k]
-            q = laid.copy_(q)
-        self.q, self.scale = q, scale.contiguous()
+        if (k > 1 and q.stride(1) != 1) or q.data_ptr() % 16 or q.stride(0) % 16 or q.stride(0) < k:
+            q = torch.empty(n, _padded(k), dtype=torch.int8, device=q.device)[:, :k].copy_(q)
+        self.q, self.scale, self.shape, self.ld = q, scale.contiguous(), (n, k), q.stride(0)
 
     @classmethod
     def from_float(cls, weight: Tensor) -> Int8Weight:
@@ -82,20 +85,6 @@ class Int8Weight:
         rows = quantize_rows(weight)
         return cls(rows.q, rows.scale)
 
-    @property
-    def shape(self) -> torch.Size:
-        return self.q.shape
-
-
-def _quantize(x2: Tensor, ldx: int, dev: torch.device) -> tuple[Tensor, Tensor]:
-    m, k = x2.shape
-    q = torch.empty(m, _padded(k), dtype=torch.int8, device=dev)
-    scale = torch.empty(m, dtype=torch.float32, device=dev)
-    rc = nat.lib().lf_quantize_rows(nat.stream_ptr(dev), nat.dtype_code(x2.dtype), x2.data_ptr(), ldx, m, k,
-                                    q.data_ptr(), q.stride(0), scale.data_ptr())
-    nat.check(rc, "lf_quantize_rows")
-    return (q if q.shape[1] == k else q[:, :k]), scale
-
 
 def quantize_rows(x: Tensor) -> Int8Rows:
     """The rows (last dimension) of an f32, bf16 or f16 tensor in 8-bit integers with a scale
@@ -103,10 +92,24 @@ def quantize_rows(x: Tensor) -> Int8Rows:
     dev = nat.require_cuda(x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"rows of at least one element are needed, got {tuple(x.shape)}")
-    with nat.on_device(dev):
-        x2, ldx = _rows(x)
-        q, scale = _quantize(x2, ldx, dev)
-    return Int8Rows(q, scale, x.shape, x.dtype)
+    x2, ldx = _rows(x)
+    m, k = x2.shape
+    kp = _padded(k)
+    q = torch.empty(m, kp, dtype=torch.int8, device=dev)
+    scale = torch.empty(m, dtype=torch.float32, device=dev)
+    nat.call(nat.lib().lf_quantize_rows, "lf_quantize_rows", dev, nat.dtype_code(x.dtype), x2.data_ptr(), ldx, m, k,
+             q.data_ptr(), kp, scale.data_ptr())
+    return Int8Rows(q if kp == k else q[:, :k], scale, x.shape, x.dtype)
+
+
+def _bias(bias: Tensor | None, n: int, dtype: torch.dtype) -> Tensor | None:
+    if bias is None:
+        return None
+    if bias.shape != (n,):
+        raise ValueError(f"bias must have {n} entries, got {tuple(bias.shape)}")
+    if bias.dtype != dtype:
+        bias = bias.to(dtype)
+    return bias if bias.is_contiguous() else bias.contiguous()
 
 
 def linear_int8(x: Tensor | Int8Rows, weight: Int8Weight, bias: Tensor | None = None, act: int = ACT_NONE,
@@ -115,62 +118,65 @@ def linear_int8(x: Tensor | Int8Rows, weight: Int8Weight, bias: Tensor | None = 
     per row first, or :class:`Int8Rows`; ``act`` is ``ACT_NONE`` or ``ACT_GELU`` (the exact erf
     GELU).  The result has x's dtype and is rounded to it once.  Any M, N and K up to 131,072;
     ``out`` must be viewable as rows without a copy and must not overlap ``x``."""
-    rows = isinstance(x, Int8Rows)
+    rows = type(x) is Int8Rows
     dev = nat.require_cuda(x.q if rows else x, weight.q, bias, out)
-    n, k = weight.q.shape
-    if x.shape[-1] != k:
-        raise ValueError(f"x has {x.shape[-1]} columns, weight expects {k}")
-    dtype = x.dtype
-    with nat.on_device(dev):
-        if rows:
-            q, scale = x.q, x.scale
-        else:
-            x2, ldx = _rows(x)
-            q, scale = _quantize(x2, ldx, dev)
-        m = q.shape[0]
-        if out is None:
-            out = torch.empty(*x.shape[:-1], n, dtype=dtype, device=dev)
-            o2 = out if out.dim() == 2 else out.view(m, n)
-        else:
-            o2 = out.reshape(-1, n)
-            if out.dtype != dtype or o2.shape[0] != m or o2.data_ptr() != out.data_ptr() or \
-                    (n > 1 and o2.stride(-1) != 1) or (out.dim() > 2 and not out.is_contiguous()):
-                raise ValueError(f"out must be ({m}, {n}) {dtype} rows viewable without a copy")
-        b = None
-        if bias is not None:
-            if bias.shape != (n,):
-                raise ValueError(f"bias must have {n} entries, got {tuple(bias.shape)}")
-            b = (bias if bias.dtype == dtype else bias.to(dtype)).contiguous()
-        rc = nat.lib().lf_linear_int8(nat.stream_ptr(dev), nat.dtype_code(dtype), q.data_ptr(), q.stride(0),
-                                      scale.data_ptr(), weight.q.data_ptr(), weight.q.stride(0),
-                                      weight.scale.data_ptr(), nat.ptr(b), o2.data_ptr(), max(o2.stride(0), n), m, n, k,
-                                      int(act), None)
-        nat.check(rc, "lf_linear_int8")
-    return out
+    n, k = weight.shape
+    shape, dtype = x.shape, x.dtype
+    if shape[-1] != k:
+        raise ValueError(f"x has {shape[-1]} columns, weight expects {k}")
+    bias = _bias(bias, n, dtype)
+    if rows:
+        m = x.q.shape[0]
+    else:
+        x2, ldx = _rows(x)
+        m = x2.shape[0]
+    if out is None:
+        out = torch.empty(m, n, dtype=dtype, device=dev)
+        ldo, ret = n, out if len(shape) == 2 else out.view(*shape[:-1], n)
+    else:
+        o2 = out.reshape(-1, n)
+        ldo = o2.stride(0) if m > 1 else n
+        if out.dtype != dtype or o2.shape[0] != m or o2.data_ptr() != out.data_ptr() or ldo < n or \
+                (n > 1 and o2.stride(1) != 1) or (out.dim() > 2 and not out.is_contiguous()):
+            raise ValueError(f"out must be ({m}, {n}) {dtype} rows viewable without a copy")
+        ret = out
+    code, b = nat.dtype_code(dtype), nat.ptr(bias)
+    if rows:
+        nat.call(nat.lib().lf_linear_int8, "lf_linear_int8", dev, code, x.q.data_ptr(), x.ld, x.scale.data_ptr(),
+                 weight.q.data_ptr(), weight.ld, weight.scale.data_ptr(), b, out.data_ptr(), ldo, m, n, k, int(act), None)
+    else:
+        size = _rows_bytes(m, k)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        nat.call(nat.lib().lf_linear_rows_int8, "lf_linear_rows_int8", dev, code, x2.data_ptr(), ldx, weight.q.data_ptr(),
+                 weight.ld, weight.scale.data_ptr(), b, out.data_ptr(), ldo, m, n, k, int(act), ws.data_ptr(), size, None)
+    return ret
+
+
+def _rows_bytes(m: int, k: int) -> int:
+    return nat.lib().lf_linear_rows_int8_workspace_bytes(m, k)
 
 
 def add_layernorm_int8(a: Tensor, b: Tensor | None, weight: Tensor, bias: Tensor, eps: float) -> tuple[Tensor, Int8Rows]:
     """``add_layernorm(a, b, weight, bias, eps)`` and its rows in 8-bit integers, in one pass."""
     dev = nat.require_cuda(a, b, weight, bias)
-    H = a.shape[-1]
+    H, dtype = a.shape[-1], a.dtype
+    _same_rows(a, b)
+    a2, lda = _rows(a)
+    b2, ldb = _rows(b) if b is not None else (None, 0)
+    m, hp = a2.shape[0], _padded(H)
+    w, bb = _bias(weight, H, dtype), _bias(bias, H, dtype)
+    out = torch.empty(a.shape, dtype=dtype, device=dev)
+    q = torch.empty(m, hp, dtype=torch.int8, device=dev)
+    scale = torch.empty(m, dtype=torch.float32, device=dev)
+    nat.call(nat.lib().lf_add_layernorm_int8, "lf_add_layernorm_int8", dev, nat.dtype_code(dtype), a2.data_ptr(), lda,
+             nat.ptr(b2), ldb, w.data_ptr(), bb.data_ptr(), float(eps), m, H, out.data_ptr(), H, q.data_ptr(), hp,
+             scale.data_ptr())
+    return out, Int8Rows(q if hp == H else q[:, :H], scale, a.shape, dtype)
+
+
+def _same_rows(a: Tensor, b: Tensor | None) -> None:
     if b is not None and (b.shape != a.shape or b.dtype != a.dtype):
-        raise ValueError(f"a is {a.dtype} {tuple(a.shape)}, b {b.dtype} {tuple(b.shape)}")
-    if weight.shape != (H,) or bias.shape != (H,):
-        raise ValueError(f"weight and bias must have {H} entries")
-    with nat.on_device(dev):
-        a2, lda = _rows(a)
-        b2, ldb = _rows(b) if b is not None else (None, 0)
-        out = torch.empty(a.shape, dtype=a.dtype, device=dev)
-        m = a2.shape[0]
-        q = torch.empty(m, _padded(H), dtype=torch.int8, device=dev)
-        scale = torch.empty(m, dtype=torch.float32, device=dev)
-        w = (weight if weight.dtype == a.dtype else weight.to(a.dtype)).contiguous()
-        bb = (bias if bias.dtype == a.dtype else bias.to(a.dtype)).contiguous()
-        rc = nat.lib().lf_add_layernorm_int8(nat.stream_ptr(dev), nat.dtype_code(a.dtype), a2.data_ptr(), lda,
-                                             nat.ptr(b2), ldb, w.data_ptr(), bb.data_ptr(), float(eps), m, H,
-                                             out.data_ptr(), H, q.data_ptr(), q.stride(0), scale.data_ptr())
-        nat.check(rc, "lf_add_layernorm_int8")
-    return out, Int8Rows(q[:, :H], scale, a.shape, a.dtype)
+        raise ValueError(f"a is {a.dtype} {tuple(a.shape)}, the residual {b.dtype} {tuple(b.shape)}")
 
 
 def ffn_int8(a: Tensor, residual: Tensor | None, ln_weight: Tensor, ln_bias: Tensor, eps: float, up: Int8Weight,
@@ -180,8 +186,25 @@ def ffn_int8(a: Tensor, residual: Tensor | None, ln_weight: Tensor, ln_bias: Ten
     ``h = layer_norm(a + residual)`` and ``o = down(act(up(h)))``, the middle activations
     rounded to a's dtype and then quantised per token.  Returns ``(h, o)``: the layer's
     output is ``add_layernorm(o, h, ...)``."""
-    if down.shape[1] != up.shape[0]:
-        raise ValueError(f"up gives {up.shape[0]} columns, down expects {down.shape[1]}")
-    h, rows = add_layernorm_int8(a, residual, ln_weight, ln_bias, eps)
-    mid = linear_int8(rows, up, up_bias, act=act)
-    return h, linear_int8(mid, down, down_bias)
+    dev = nat.require_cuda(a, residual, ln_weight, ln_bias, up.q, up_bias, down.q, down_bias)
+    inner, hidden = up.shape
+    dtype = a.dtype
+    if a.shape[-1] != hidden or down.shape != (hidden, inner):
+        raise ValueError(f"a has {a.shape[-1]} columns, up is {up.shape}, down {down.shape}: "
+                         "up must be (inner, hidden), down (hidden, inner)")
+    _same_rows(a, residual)
+    a2, lda = _rows(a)
+    r2, ldr = _rows(residual) if residual is not None else (None, 0)
+    m = a2.shape[0]
+    w, bb = _bias(ln_weight, hidden, dtype), _bias(ln_bias, hidden, dtype)
+    ub, db = _bias(up_bias, inner, dtype), _bias(down_bias, hidden, dtype)
+    both = torch.empty(2, m, hidden, dtype=dtype, device=dev)
+    h, o = both.unbind(0)
+    lib, code = nat.lib(), nat.dtype_code(dtype)
+    size = lib.lf_ffn_int8_workspace_bytes(code, m, hidden, inner)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    nat.call(lib.lf_ffn_int8, "lf_ffn_int8", dev, code, a2.data_ptr(), lda, nat.ptr(r2), ldr, w.data_ptr(), bb.data_ptr(),
+             float(eps), up.q.data_ptr(), up.ld, up.scale.data_ptr(), nat.ptr(ub), down.q.data_ptr(), down.ld,
+             down.scale.data_ptr(), nat.ptr(db), m, hidden, inner, int(act), h.data_ptr(), hidden, o.data_ptr(), hidden,
+             ws.data_ptr(), size, None)
+    return (h, o) if a.dim() == 2 else (h.view(a.shape), o.view(a.shape))

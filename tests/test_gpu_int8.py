@@ -276,7 +276,7 @@ def test_refusals(cuda):
         quantize_rows(x.double())
     with pytest.raises(nat.NativeLibraryError, match="CUDA tensors"):
         linear_int8(x.cpu(), wt)
-    with pytest.raises(ValueError, match="down expects"):
+    with pytest.raises(ValueError, match="up must be"):
         ffn_int8(x, x, x[0], x[0], 1e-5, wt, None, Int8Weight(*weight(cuda, 64, 33, 1)), None)
     rows = quantize_rows(x)
     assert isinstance(rows, Int8Rows)
