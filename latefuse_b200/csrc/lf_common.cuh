@@ -226,6 +226,31 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
   }
 }
 
+// One lane of a converged warp, always the same.  Roles that issue MMAs or copies run
+// their loops with the whole warp and issue under this predicate: with the control flow
+// warp-uniform, descriptors and coordinates stay in uniform registers, where the same
+// loop inside `if (lane == 0)` spent about 130 clocks an MMA moving them there.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is)::"memory");
+  return is != 0;
+}
+
+// mbar_wait by a whole converged warp, whose lanes all get the same answer.  `abort` (a
+// shared word another role sets when it gives up) is looked at before a wait that would
+// block; on a timeout it is set here, with LF_STATUS_TIMEOUT in *status.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int32_t* abort, int32_t* status) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  bool ok = *reinterpret_cast<const volatile int32_t*>(abort) == 0;
+  if (__all_sync(0xffffffffu, ok) && __all_sync(0xffffffffu, mbar_wait(bar, parity))) return true;
+  if (ok && (threadIdx.x & 31) == 0) {
+    set_status(status, LF_STATUS_TIMEOUT);
+    atomicExch(abort, 1);
+  }
+  __syncwarp();
+  return false;
+}
+
 // ---------------------------------------------------------------------------
 // TMA (tiled cp.async.bulk.tensor; no load in this library uses cluster multicast)
 // ---------------------------------------------------------------------------

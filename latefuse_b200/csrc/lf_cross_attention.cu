@@ -31,10 +31,12 @@
 //   warp 0      producer: Q, K and V tiles by TMA (SW128 blocks of 64 columns);
 //   warp 1      MMA issuer: S = Q K^T into shared TMEM S buffers, O += P V into the
 //               group's TMEM accumulator;
-//   warps 2-5,  softmax groups, one thread per query row.
-//   6-9
-// With 64 columns a key tile has 128 keys; with 128 columns 64 keys, so that Q, P and
-// eight K / V stages fit in shared memory (229 KB).
+//   warps 4-7,  softmax groups, one thread per query row.  The row's scores are read from
+//   8-11        TMEM once and stay in registers (the first warpgroup hands its registers
+//               over); the probabilities go back over the scores' columns, from where the
+//               second product takes them as its TMEM operand.
+// With 64 columns a key tile has 128 keys, with 128 columns 64, so that O of both groups
+// and three (four) score buffers fit TMEM's 512 columns.
 // Every wait is bounded: a timeout sets LF_STATUS_TIMEOUT and the roles unwind.
 #include <cmath>
 #include <cstring>
@@ -393,7 +395,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const _
 // ---------------------------------------------------------------------------
 constexpr int kRows = 128;     // query tile rows
 constexpr int kGroups = 2;
-constexpr int kThreads = 64 + 32 * 4 * kGroups;
+constexpr int kThreads = 128 * (1 + kGroups);
+// Registers: the producer / MMA warpgroup gives up what the softmax warpgroups take, so
+// that a row's 128 scores stay in registers (128 x 88 + 256 x 208 = 384 x 168, the launch's).
+constexpr int kRegsIssue = 88, kRegsSoftmax = 208;
 constexpr float kMaxSlack = 8.f;  // log2 units the running max may lag a tile's max
 
 template <int kD>
@@ -402,12 +407,11 @@ struct Shape {
   static constexpr int kBlocks = kD / 64;             // 64-column SW128 blocks of a head's row
   static constexpr int kQBytes = kRows * kD * 2;
   static constexpr int kKvBytes = kKeys * kD * 2;     // 16 KB
-  static constexpr int kPBytes = kRows * kKeys * 2;
-  static constexpr int kKStages = kD == 64 ? 3 : 4;
-  static constexpr int kVStages = 4;
-  static constexpr int kSBufs = kD == 64 ? 3 : 4;     // TMEM S buffers shared by the groups
-  static constexpr int kOCol = kSBufs * kKeys;        // group g's O at TMEM column kOCol + kD g
-  static constexpr int kSmem = 1024 + kGroups * (kQBytes + kPBytes) + (kKStages + kVStages) * kKvBytes + 1024;
+  static constexpr int kKStages = kD == 64 ? 6 : 5;
+  static constexpr int kVStages = 5;
+  static constexpr int kBufs = kD == 64 ? 3 : 4;      // TMEM score buffers shared by the groups
+  static constexpr int kOCol = kBufs * kKeys;         // group g's O at TMEM column kOCol + kD g
+  static constexpr int kSmem = 1024 + kGroups * kQBytes + (kKStages + kVStages) * kKvBytes + 1024;
   static_assert(kOCol + kGroups * kD <= 512, "TMEM columns");
   static_assert(kSmem <= 232448, "above the 227 KB of shared memory a CTA may use");
 };
@@ -421,13 +425,65 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// D[tmem] (+)= A[tmem] * B[smem desc]: A's row is the TMEM lane, two 16-bit elements a column.
+__device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 128 consecutive TMEM columns of this warp's 32 lanes, both halves in flight at once.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+      "}, [%128];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+      "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+      "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+      "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127"
+      "}, [%129];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
+        "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+        "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(taddr), "r"(taddr + 64)
+      : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void set_max_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void set_max_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // A unit's record as every role reads it: keys to walk (at least one, so that all roles
 // take the same steps), and what is stored: 0 the result, 1 nothing, 2 zeros (no keys).
 struct Unit {
   int q0, nq, k0, nk, tile, what;
 };
 
-template <int kKeys>
+// A group's walk over its units and their key tiles.
 struct Cursor {
   int64_t unit;  // global unit index, or >= n_units when done
   Unit it;
@@ -447,15 +503,14 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   const uint32_t sQ = base;
-  const uint32_t sP = sQ + kGroups * Sh::kQBytes;
-  const uint32_t sK = sP + kGroups * Sh::kPBytes;
+  const uint32_t sK = sQ + kGroups * Sh::kQBytes;
   const uint32_t sV = sK + Sh::kKStages * kKvBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(gbase + (sV + Sh::kVStages * kKvBytes - base));
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   // per-group barriers at index (kind * kGroups + group)
-  constexpr int Q_FULL = 0, Q_EMPTY = 1, P_FULL = 2, P_EMPTY = 3, O_FULL = 4, O_EMPTY = 5;
+  constexpr int Q_FULL = 0, Q_EMPTY = 1, P_FULL = 2, O_FULL = 3, O_EMPTY = 4, PV_DONE = 5;
   auto gbar = [&](int kind, int grp) { return bar(kind * kGroups + grp); };
-  constexpr int S_FULL = 6 * kGroups, S_EMPTY = S_FULL + Sh::kSBufs, K_FULL = S_EMPTY + Sh::kSBufs,
+  constexpr int S_FULL = 6 * kGroups, BUF_EMPTY = S_FULL + Sh::kBufs, K_FULL = BUF_EMPTY + Sh::kBufs,
                 K_EMPTY = K_FULL + Sh::kKStages, V_FULL = K_EMPTY + Sh::kKStages, V_EMPTY = V_FULL + Sh::kVStages,
                 DRAIN = V_EMPTY + Sh::kVStages, N_BARS = DRAIN + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(&bars[N_BARS]);
@@ -467,13 +522,13 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
       mbar_init(gbar(Q_FULL, grp), 1);
       mbar_init(gbar(Q_EMPTY, grp), 1);
       mbar_init(gbar(P_FULL, grp), 4);
-      mbar_init(gbar(P_EMPTY, grp), 1);
       mbar_init(gbar(O_FULL, grp), 1);
       mbar_init(gbar(O_EMPTY, grp), 4);
+      mbar_init(gbar(PV_DONE, grp), 1);
     }
-    for (int i = 0; i < Sh::kSBufs; ++i) {
+    for (int i = 0; i < Sh::kBufs; ++i) {
       mbar_init(bar(S_FULL + i), 1);
-      mbar_init(bar(S_EMPTY + i), 4);
+      mbar_init(bar(BUF_EMPTY + i), 1);
     }
     for (int i = 0; i < Sh::kKStages; ++i) {
       mbar_init(bar(K_FULL + i), 1);
@@ -505,11 +560,13 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
     atomicExch(s_abort, 1);
   };
   auto wait = [&](uint32_t b, uint32_t parity) {
+    if (mbar_try_wait(b, parity)) return true;
     if (aborted(s_abort)) return false;
     if (mbar_wait(b, parity)) return true;
     if (!aborted(s_abort)) fail();
     return false;
   };
+  auto wwait = [&](uint32_t b, uint32_t parity) { return warp_wait(b, parity, s_abort, p.status); };  // by a whole warp
   auto unit_of = [&](int64_t unit) {
     const Rec r = read_rec(p, int(unit / p.n_heads));
     if (!r.ok) {
@@ -520,9 +577,11 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
     if (r.nk == 0) return Unit{r.q0, r.nq, 0, 1, r.tile, 2};
     return Unit{r.q0, r.nq, r.k0, r.nk, r.tile, 0};
   };
-  // group grp takes the CTA's units 2k + grp
-  using Cur = Cursor<kKeys>;
-  auto start = [&](Cur& c, int grp) {
+  // Round i gives every group of every CTA one unit, in the records' order (most keys
+  // first), the order of the groups turned round from round to round: a group that had a
+  // longer unit gets a shorter one next.
+  const int64_t n_slots = int64_t(kGroups) * gridDim.x;
+  auto start = [&](Cursor& c, int grp) {
     c.unit = blockIdx.x + int64_t(grp) * gridDim.x;
     c.u = c.t = c.j = 0;
     if (c.unit < n_units) {
@@ -530,64 +589,73 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
       c.n_kv = (c.it.nk + kKeys - 1) / kKeys;
     }
   };
-  auto advance = [&](Cur& c) {
+  auto advance = [&](Cursor& c) {
     ++c.t;
     if (++c.j < c.n_kv) return;
-    c.unit += int64_t(kGroups) * gridDim.x;
+    const int64_t in_round = c.unit - c.u * n_slots;
     ++c.u;
+    c.unit = c.u * n_slots + (n_slots - 1 - in_round);
     c.j = 0;
     if (c.unit < n_units) {
       c.it = unit_of(c.unit);
       c.n_kv = (c.it.nk + kKeys - 1) / kKeys;
     }
   };
-  auto live = [&](const Cur& c) { return c.unit < n_units; };
+  auto live = [&](const Cursor& c) { return c.unit < n_units; };
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      Cur c[kGroups];
+  if (warp < 4) {
+    set_max_regs_dec<kRegsIssue>();
+    if (warp == 0) {
+      // ------------------------------------------------------------ producer
+      Cursor c[kGroups];
       for (int grp = 0; grp < kGroups; ++grp) start(c[grp], grp);
       int kc = 0, nq[kGroups] = {0, 0};
       bool stop = false;
       while (!stop && (live(c[0]) || live(c[1]))) {
-        for (int grp = 0; grp < kGroups && !stop; ++grp) {
-          Cur& cg = c[grp];
-          if (!live(cg)) continue;
+#pragma unroll
+        for (int grp = 0; grp < kGroups; ++grp) {
+          Cursor& cg = c[grp];
+          if (stop || !live(cg)) continue;
           const int h = int(cg.unit % p.n_heads), hk = h / p.group;
           if (cg.j == 0) {  // the unit's Q tile, once the group's previous unit has no S left to issue
-            if (!wait(gbar(Q_EMPTY, grp), (cg.u & 1) ^ 1)) {
+            if (!wwait(gbar(Q_EMPTY, grp), (cg.u & 1) ^ 1)) {
               stop = true;
-              break;
+              continue;
             }
-            mbar_arrive_expect_tx(gbar(Q_FULL, grp), Sh::kQBytes);
-            for (int b = 0; b < Sh::kBlocks; ++b)
-              tma_load_3d(sQ + grp * Sh::kQBytes + b * (kRows * 128), &p.q_map, gbar(Q_FULL, grp), b * 64, h,
-                          cg.it.q0 + cg.it.tile * kRows);
+            if (elect_one()) {
+              mbar_arrive_expect_tx(gbar(Q_FULL, grp), Sh::kQBytes);
+              for (int b = 0; b < Sh::kBlocks; ++b)
+                tma_load_3d(sQ + grp * Sh::kQBytes + b * (kRows * 128), &p.q_map, gbar(Q_FULL, grp), b * 64, h,
+                            cg.it.q0 + cg.it.tile * kRows);
+            }
             ++nq[grp];
           }
           const int sk = kc % Sh::kKStages, sv = kc % Sh::kVStages;
           const int32_t krow = cg.it.k0 + cg.j * kKeys;
-          if (!wait(bar(K_EMPTY + sk), ((kc / Sh::kKStages) & 1) ^ 1)) {
+          if (!wwait(bar(K_EMPTY + sk), ((kc / Sh::kKStages) & 1) ^ 1)) {
             stop = true;
-            break;
+            continue;
           }
-          mbar_arrive_expect_tx(bar(K_FULL + sk), kKvBytes);
-          for (int b = 0; b < Sh::kBlocks; ++b)
-            tma_load_3d(sK + sk * kKvBytes + b * (kKeys * 128), &p.k_map, bar(K_FULL + sk), b * 64, hk, krow);
-          if (!wait(bar(V_EMPTY + sv), ((kc / Sh::kVStages) & 1) ^ 1)) {
+          if (elect_one()) {
+            mbar_arrive_expect_tx(bar(K_FULL + sk), kKvBytes);
+            for (int b = 0; b < Sh::kBlocks; ++b)
+              tma_load_3d(sK + sk * kKvBytes + b * (kKeys * 128), &p.k_map, bar(K_FULL + sk), b * 64, hk, krow);
+          }
+          if (!wwait(bar(V_EMPTY + sv), ((kc / Sh::kVStages) & 1) ^ 1)) {
             stop = true;
-            // this tile's K has been issued and its V has not: drained below as one more K
-            mbar_wait(bar(K_FULL + sk), (kc / Sh::kKStages) & 1);
-            break;
+            mbar_wait(bar(K_FULL + sk), (kc / Sh::kKStages) & 1);  // this tile's K lands; its V was not issued
+            continue;
           }
-          mbar_arrive_expect_tx(bar(V_FULL + sv), kKvBytes);
-          for (int b = 0; b < Sh::kBlocks; ++b)
-            tma_load_3d(sV + sv * kKvBytes + b * (kKeys * 128), &p.v_map, bar(V_FULL + sv), b * 64, hk, krow);
+          if (elect_one()) {
+            mbar_arrive_expect_tx(bar(V_FULL + sv), kKvBytes);
+            for (int b = 0; b < Sh::kBlocks; ++b)
+              tma_load_3d(sV + sv * kKvBytes + b * (kKeys * 128), &p.v_map, bar(V_FULL + sv), b * 64, hk, krow);
+          }
           ++kc;
           advance(cg);
         }
       }
+      __syncwarp();
       if (aborted(s_abort)) {  // loads nobody consumed must land before the CTA exits (bounded)
         for (int q = (kc > Sh::kKStages ? kc - Sh::kKStages : 0); q < kc; ++q)
           mbar_wait(bar(K_FULL + q % Sh::kKStages), (q / Sh::kKStages) & 1);
@@ -596,14 +664,12 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
         for (int grp = 0; grp < kGroups; ++grp)  // only a group's latest Q can be unconsumed
           if (nq[grp] > 0) mbar_wait(gbar(Q_FULL, grp), (nq[grp] - 1) & 1);
       }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer
       const int nks = (p.d + 15) / 16;  // 16-column steps of a head's row
       const uint32_t idesc_o = umma_idesc_f16(DT<T>::umma_fmt, kRows, uint32_t(nks) * 16, /*a_mn=*/0, /*b_mn=*/1);
-      struct Prev { bool valid, first, last; int t, u, kv, nk; };  // nk: 16-key steps of O += P V
-      Cur c[kGroups];
+      struct Prev { bool valid, first, last; int t, u, kv, n16; };  // n16: 16-key steps of O += P V
+      Cursor c[kGroups];
       Prev prev[kGroups];
       for (int grp = 0; grp < kGroups; ++grp) {
         start(c[grp], grp);
@@ -611,83 +677,94 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
       }
       int kc = 0;
       bool stop = false;
-      // O_grp += P V for the group's previous tile
+      // O_grp += P V for the group's previous tile, P in the tile's score buffer
       auto pv = [&](int grp, const Prev& e) -> bool {
-        const int sv = e.kv % Sh::kVStages;
-        if (!wait(gbar(P_FULL, grp), e.t & 1)) return false;
-        if (!wait(bar(V_FULL + sv), (e.kv / Sh::kVStages) & 1)) return false;
-        if (e.first && !wait(gbar(O_EMPTY, grp), (e.u & 1) ^ 1)) return false;
+        const int sv = e.kv % Sh::kVStages, sb = e.kv % Sh::kBufs;
+        if (!wwait(bar(V_FULL + sv), (e.kv / Sh::kVStages) & 1)) return false;
+        if (e.first && !wwait(gbar(O_EMPTY, grp), (e.u & 1) ^ 1)) return false;
+        if (!wwait(gbar(P_FULL, grp), e.t & 1)) return false;
         tc_fence_after();
-        const uint32_t pb = sP + grp * Sh::kPBytes;
-        const uint32_t vb = sV + sv * kKvBytes;
+        const uint64_t vd = smem_desc(sV + sv * kKvBytes, kKeys * 128, 1024, 2);
+        const uint32_t d = tmem + Sh::kOCol + kD * grp, a = tmem + kKeys * sb;
+        if (elect_one()) {
 #pragma unroll
-        for (int t = 0; t < kKeys / 16; ++t) {
-          if (t >= e.nk) break;
-          umma_f16(tmem + Sh::kOCol + kD * grp, smem_desc(pb + (t >> 2) * (kRows * 128) + (t & 3) * 32, 16, 1024, 2),
-                   smem_desc(vb + t * 2048, kKeys * 128, 1024, 2), idesc_o, (e.first && t == 0) ? 0u : 1u);
+          for (int t = 0; t < kKeys / 16; ++t) {  // 16 value rows are 2,048 bytes
+            if (t < e.n16) umma_f16_ta(d, a + t * 8, vd + uint64_t(t * 128), idesc_o, (e.first && t == 0) ? 0u : 1u);
+          }
+          umma_commit(bar(BUF_EMPTY + sb));
+          umma_commit(bar(V_EMPTY + sv));
+          umma_commit(gbar(PV_DONE, grp));
+          if (e.last) umma_commit(gbar(O_FULL, grp));
         }
-        umma_commit(gbar(P_EMPTY, grp));
-        umma_commit(bar(V_EMPTY + sv));
-        if (e.last) umma_commit(gbar(O_FULL, grp));
+        __syncwarp();
         return true;
       };
       while (!stop && (live(c[0]) || live(c[1]) || prev[0].valid || prev[1].valid)) {
-        for (int grp = 0; grp < kGroups && !stop; ++grp) {
-          Cur& cg = c[grp];
+#pragma unroll
+        for (int grp = 0; grp < kGroups; ++grp) {
+          if (stop) continue;
+          Cursor& cg = c[grp];
           Prev cur{false, false, false, 0, 0, 0, 0};
           if (live(cg)) {
-            const int sk = kc % Sh::kKStages, sb = kc % Sh::kSBufs;
-            if ((cg.j == 0 && !wait(gbar(Q_FULL, grp), cg.u & 1)) ||
-                !wait(bar(K_FULL + sk), (kc / Sh::kKStages) & 1) ||
-                !wait(bar(S_EMPTY + sb), ((kc / Sh::kSBufs) & 1) ^ 1)) {
+            const int sk = kc % Sh::kKStages, sb = kc % Sh::kBufs;
+            if ((cg.j == 0 && !wwait(gbar(Q_FULL, grp), cg.u & 1)) ||
+                !wwait(bar(K_FULL + sk), (kc / Sh::kKStages) & 1) ||
+                !wwait(bar(BUF_EMPTY + sb), ((kc / Sh::kBufs) & 1) ^ 1)) {
               stop = true;
-              break;
+              continue;
             }
             tc_fence_after();
-            const uint32_t qa = sQ + grp * Sh::kQBytes, kb = sK + sk * kKvBytes;
+            const uint64_t qd = smem_desc(sQ + grp * Sh::kQBytes, 16, 1024, 2);
+            const uint64_t kd = smem_desc(sK + sk * kKvBytes, 16, 1024, 2);
             // S over the tile's keys, to the next multiple of 16
             const int n16 = (min(kKeys, cg.it.nk - cg.j * kKeys) + 15) / 16;
             const uint32_t idesc = umma_idesc_f16(DT<T>::umma_fmt, kRows, uint32_t(n16) * 16, 0, 0);
+            const bool last = cg.j == cg.n_kv - 1;
+            if (elect_one()) {
 #pragma unroll
-            for (int t = 0; t < kD / 16; ++t) {
-              if (t >= nks) break;
-              umma_f16(tmem + kKeys * sb, smem_desc(qa + (t >> 2) * (kRows * 128) + (t & 3) * 32, 16, 1024, 2),
-                       smem_desc(kb + (t >> 2) * (kKeys * 128) + (t & 3) * 32, 16, 1024, 2), idesc, t > 0 ? 1u : 0u);
+              for (int t = 0; t < kD / 16; ++t) {  // 16 columns are 32 bytes, 64 of them a block
+                if (t < nks)
+                  umma_f16(tmem + kKeys * sb, qd + uint64_t((t >> 2) * (kRows * 8) + (t & 3) * 2),
+                           kd + uint64_t((t >> 2) * (kKeys * 8) + (t & 3) * 2), idesc, t > 0 ? 1u : 0u);
+              }
+              umma_commit(bar(S_FULL + sb));
+              umma_commit(bar(K_EMPTY + sk));
+              if (last) umma_commit(gbar(Q_EMPTY, grp));
             }
-            umma_commit(bar(S_FULL + sb));
-            umma_commit(bar(K_EMPTY + sk));
-            if (cg.j == cg.n_kv - 1) umma_commit(gbar(Q_EMPTY, grp));
-            cur = Prev{true, cg.j == 0, cg.j == cg.n_kv - 1, cg.t, cg.u, kc, n16};
+            __syncwarp();
+            cur = Prev{true, cg.j == 0, last, cg.t, cg.u, kc, n16};
             ++kc;
             advance(cg);
           }
           if (prev[grp].valid && !pv(grp, prev[grp])) {
             stop = true;
-            break;
+            continue;
           }
           prev[grp] = cur;
         }
       }
+      __syncwarp();
       if (aborted(s_abort)) {  // every issued MMA must finish before TMEM is released (bounded)
-        umma_commit(bar(DRAIN));
+        if (elect_one()) umma_commit(bar(DRAIN));
+        __syncwarp();
         mbar_wait(bar(DRAIN), 0);
       }
     }
+    __syncwarp();
   } else {
-    // ------------------------------------------------------------ softmax groups (warps 2..9)
-    const int grp = (warp - 2) >> 2;
+    // ------------------------------------------------------------ softmax groups (warps 4..11)
+    set_max_regs_inc<kRegsSoftmax>();
+    const int grp = (warp - 4) >> 2;
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
     const uint32_t lane_addr = tmem + (uint32_t(quad * 32) << 16);
     const uint32_t o_addr = lane_addr + Sh::kOCol + kD * grp;   // this row of the group's O
-    const uint32_t prow = (row >> 3) * 1024 + (row & 7) * 128;  // this row in a SW128 block
-    const uint32_t pb = sP + grp * Sh::kPBytes - base;
     const float2 sl2 = f2(p.scale_log2);
     // The MMA warp issues the groups' S tiles round-robin (group 0 first), so this
     // group's n-th tile is global tile n + min(n + grp, tiles of the other group).
     int other_tiles = 0;
     {
-      Cur o;
+      Cursor o;
       start(o, grp ^ 1);
       while (live(o)) {
         other_tiles += o.n_kv;
@@ -695,131 +772,131 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
         advance(o);
       }
     }
-    Cur c;
+    Cursor c;
     start(c, grp);
     float m = -INFINITY, l = 0.f;
     while (live(c)) {
       const int t = c.t, j = c.j;
       const int kc = t + min(t + grp, other_tiles);
-      const int sb = kc % Sh::kSBufs;
+      const int sb = kc % Sh::kBufs;
       const uint32_t s_addr = lane_addr + kKeys * sb;
-      const Unit it = c.it;
-      const int64_t unit = c.unit;
-      const int uu = c.u;
       const bool last = j == c.n_kv - 1;
-      const int nvalid = min(kKeys, it.nk - j * kKeys);
+      const int nvalid = min(kKeys, c.it.nk - j * kKeys);
       // a warp whose 32 query rows all lie past the queries' end does no softmax (its P rows
       // only feed O rows that are never stored)
-      const bool rows_live = quad * 32 < it.nq - it.tile * kRows;
-      const int n_half = (nvalid + 63) / 64;
-      const bool work = __all_sync(0xffffffffu, wait(bar(S_FULL + sb), (kc / Sh::kSBufs) & 1));
+      const bool rows_live = quad * 32 < c.it.nq - c.it.tile * kRows;
+      const bool work = __all_sync(0xffffffffu, wait(bar(S_FULL + sb), (kc / Sh::kBufs) & 1));
       tc_fence_after();
-      // pass 1: the row max over the valid keys, 64 columns at a time
-      float mx = -INFINITY;
+      float sum = 0.f, m_new = m, alpha = 1.f;
       if (work && rows_live) {
-#pragma unroll 1
-        for (int hh = 0; hh < n_half; ++hh) {
-          uint32_t sv[64];
-          tmem_ld64(s_addr + hh * 64, sv);
-          if (nvalid < hh * 64 + 64) {  // warp-uniform: keys past the end do not count
+        // the row's scores, all in registers; a short tile reads its first 64 alone
+        uint32_t s[kKeys];
+        const bool wide = kKeys == 128 && nvalid > 64;
+        if constexpr (kKeys == 128) {
+          if (wide) {
+            tmem_ld128(s_addr, s);
+          } else {
+            uint32_t lo[64];
+            tmem_ld64(s_addr, lo);
 #pragma unroll
-            for (int q = 0; q < 64; ++q)
-              if (hh * 64 + q >= nvalid) sv[q] = __float_as_uint(-INFINITY);
+            for (int q = 0; q < 64; ++q) s[q] = lo[q], s[64 + q] = 0u;
           }
-          float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int q = 0; q < 64; q += 2)
-            mxs[(q >> 1) & 3] = max3(mxs[(q >> 1) & 3], __uint_as_float(sv[q]), __uint_as_float(sv[q + 1]));
-          mx = max3(mx, fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
+        } else {
+          tmem_ld64(s_addr, s);
         }
-        mx *= sl2.x;  // the scale is positive: max commutes with it
-      }
-      const float m_new = (j == 0 || mx > m + kMaxSlack) ? mx : m;
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;  // every score so far is -inf: p = 0
-      const float alpha = (j == 0) ? 1.f : sfu_ex2(m - m_use);
-      // the previous tile's O += P V has finished: P may be overwritten, O rescaled
-      const bool go = __all_sync(0xffffffffu, work && wait(gbar(P_EMPTY, grp), (t & 1) ^ 1));
-      if (go && rows_live && j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
-        tc_fence_after();
+        if (nvalid < kKeys) {  // warp-uniform: keys past the end score -inf, so they do not count
+#pragma unroll
+          for (int q = 0; q < kKeys; ++q)
+            if (q >= nvalid) s[q] = __float_as_uint(-INFINITY);
+        }
+        float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int q = 0; q < 64; q += 2)
+          mxs[(q >> 1) & 3] = max3(mxs[(q >> 1) & 3], __uint_as_float(s[q]), __uint_as_float(s[q + 1]));
+        if (wide) {
+#pragma unroll
+          for (int q = 64; q < kKeys; q += 2)
+            mxs[(q >> 1) & 3] = max3(mxs[(q >> 1) & 3], __uint_as_float(s[q]), __uint_as_float(s[q + 1]));
+        }
+        // the scale is positive: max commutes with it
+        const float mx = max3(fmaxf(mxs[0], mxs[1]), mxs[2], mxs[3]) * sl2.x;
+        m_new = (j == 0 || mx > m + kMaxSlack) ? mx : m;
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;  // every score so far is -inf: p = 0
+        alpha = (j == 0) ? 1.f : sfu_ex2(m - m_use);
+        if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          // O moves to the new maximum, once the previous tile's O += P V has finished
+          if (__all_sync(0xffffffffu, wait(gbar(PV_DONE, grp), (t & 1) ^ 1))) {
+            tc_fence_after();
 #pragma unroll 1
-        for (int b = 0; b < Sh::kBlocks; ++b) {
-          uint32_t ov[64];
-          tmem_ld64(o_addr + b * 64, ov);
+            for (int b = 0; b < 2 * Sh::kBlocks; ++b) {
+              uint32_t ov[32];
+              tmem_ld32(o_addr + b * 32, ov);
 #pragma unroll
-          for (int q = 0; q < 64; ++q) ov[q] = __float_as_uint(__uint_as_float(ov[q]) * alpha);
-          tmem_st64(o_addr + b * 64, ov);
+              for (int q = 0; q < 32; ++q) ov[q] = __float_as_uint(__uint_as_float(ov[q]) * alpha);
+              tmem_st32(o_addr + b * 32, ov);
+            }
+          }
         }
-      }
-      // pass 2: p = 2^(s - max), rounded to T into the group's SW128 K-major P tile
-      float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      if (go && rows_live) {
+        // p = 2^(s - max), rounded to T, over the scores' own TMEM columns (two keys a column)
+        float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         const float2 neg_m = f2(-m_use);
-#pragma unroll 1
-        for (int hh = 0; hh < n_half; ++hh) {
-          uint32_t sv[64];
-          tmem_ld64(s_addr + hh * 64, sv);
-          if (nvalid < hh * 64 + 64) {  // warp-uniform: keys past the end score -inf, so p = 0
 #pragma unroll
-            for (int q = 0; q < 64; ++q)
-              if (hh * 64 + q >= nvalid) sv[q] = __float_as_uint(-INFINITY);
-          }
+        for (int hh = 0; hh < kKeys / 64; ++hh) {
+          if (hh == 0 || wide) {
+            uint32_t w[32];
 #pragma unroll
-          for (int c8 = 0; c8 < 8; ++c8) {  // 16-byte chunks = 8 keys
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int col = c8 * 8 + 2 * i;
-              const float2 x = f2_fma(make_float2(__uint_as_float(sv[col]), __uint_as_float(sv[col + 1])), sl2, neg_m);
+            for (int i = 0; i < 32; ++i) {
+              const int col = hh * 64 + 2 * i;
+              const float2 x = f2_fma(make_float2(__uint_as_float(s[col]), __uint_as_float(s[col + 1])), sl2, neg_m);
               const float2 pr = make_float2(sfu_ex2(x.x), sfu_ex2(x.y));
               sums[i & 1] = f2_add(sums[i & 1], pr);
               w[i] = Pack2<T>::pack(pr.x, pr.y);
             }
-            *reinterpret_cast<uint4*>(gbase + pb + hh * (kRows * 128) + prow + ((c8 ^ (row & 7)) << 4)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
+            tmem_st32(s_addr + hh * 32, w);
           }
         }
+        sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(S_EMPTY + sb));  // S has been read: the buffer may take the next S
-      const float sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
       l = (j == 0) ? sum : l * alpha + sum;
       m = m_new;
       // the last 16-key step of a tile that ends inside it multiplies value rows past the
       // sequence's end by p = 0: those rows become zeros first (they may hold NaN)
       if ((nvalid & 15) != 0) {
         const int sv = kc % Sh::kVStages;
-        if (__all_sync(0xffffffffu, go && wait(bar(V_FULL + sv), (kc / Sh::kVStages) & 1))) {
+        if (__all_sync(0xffffffffu, work && wait(bar(V_FULL + sv), (kc / Sh::kVStages) & 1))) {
           const int n_zero = 16 - (nvalid & 15);
           uint8_t* vrow = gbase + (sV + sv * kKvBytes - base) + nvalid * 128;
           for (int i = row; i < n_zero * 8 * Sh::kBlocks; i += kRows) {
             const int b = i / (n_zero * 8), x = i % (n_zero * 8);
             *reinterpret_cast<uint4*>(vrow + b * (kKeys * 128) + x * 16) = make_uint4(0u, 0u, 0u, 0u);
           }
+          fence_proxy_async_smem();
         }
       }
-      fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(gbar(P_FULL, grp));
-      advance(c);
+      // The next S may already be there, so without a wait a warp could arrive for this tile
+      // before a slower one has for the last, or all of them before the MMA thread has seen
+      // the last tile's phase: PV_DONE of the last tile says that both have happened.
+      if (lane == 0 && wait(gbar(PV_DONE, grp), (t & 1) ^ 1)) mbar_arrive(gbar(P_FULL, grp));
+      __syncwarp();
       if (last) {
         // the unit's output: O / l, once its last O += P V has finished
-        if (__all_sync(0xffffffffu, wait(gbar(O_FULL, grp), uu & 1)) && rows_live) {
+        if (__all_sync(0xffffffffu, wait(gbar(O_FULL, grp), c.u & 1)) && rows_live) {
           tc_fence_after();
-          const int qr = it.tile * kRows + row;
-          const float inv = it.what == 2 || l == 0.f ? 0.f : 1.f / l;
-          T* dst = reinterpret_cast<T*>(p.out) + int64_t(it.q0 + qr) * p.ldo + int64_t(unit % p.n_heads) * p.d;
+          const int qr = c.it.tile * kRows + row, what = c.it.what;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          T* dst = reinterpret_cast<T*>(p.out) + int64_t(c.it.q0 + qr) * p.ldo + int64_t(c.unit % p.n_heads) * p.d;
 #pragma unroll 1
           for (int b = 0; b < Sh::kBlocks; ++b) {
             uint32_t ov[64];
             tmem_ld64(o_addr + b * 64, ov);
-            if (qr < it.nq && it.what != 1) {
+            if (qr < c.it.nq && what != 1) {
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
                 if (b * 64 + q * 8 >= p.d) break;
                 uint4 w;
-                if (it.what == 2) {  // no keys: zeros, whatever the key row read in their place holds
+                if (what == 2) {  // no keys: zeros, whatever the key row read in their place holds
                   w = make_uint4(0u, 0u, 0u, 0u);
                 } else {
                   w.x = Pack2<T>::pack(__uint_as_float(ov[8 * q + 0]) * inv, __uint_as_float(ov[8 * q + 1]) * inv);
@@ -836,6 +913,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive(gbar(O_EMPTY, grp));
       }
+      advance(c);
     }
   }
 
