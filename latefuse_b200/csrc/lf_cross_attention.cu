@@ -25,18 +25,19 @@
 // to even out long and short ones; the cluster joins its parts through distributed
 // shared memory in rank order, so there is no workspace, no second launch and no atomic.
 //
-// cross_prompt_kernel, for many query rows, on tcgen05: the schedule of the packed
-// self-attention (lf_attention.cu) with separate query and key tables.  Work unit =
-// (128 queries of a sequence, head); a persistent CTA per SM runs two units in ping-pong:
-//   warp 0      producer: Q, K and V tiles by TMA (SW128 blocks of 64 columns);
-//   warp 1      MMA issuer: S = Q K^T into shared TMEM S buffers, O += P V into the
-//               group's TMEM accumulator;
-//   warps 4-7,  softmax groups, one thread per query row.  The row's scores are read from
-//   8-11        TMEM once and stay in registers (the first warpgroup hands its registers
-//               over); the probabilities go back over the scores' columns, from where the
-//               second product takes them as its TMEM operand.
-// With 64 columns a key tile has 128 keys, with 128 columns 64, so that O of both groups
-// and three (four) score buffers fit TMEM's 512 columns.
+// cross_prompt_kernel, for many query rows, on tcgen05.  Work unit = (128 queries of a
+// sequence, head).  A persistent CTA per SM runs two groups side by side, each walking
+// units of its own with its own warps, rings, barriers and TMEM columns, so that one
+// group's exponentials fill the other's waits and neither waits for the other:
+//   warps 0-1   producers, one per group: Q, K and V tiles by TMA (SW128 blocks of 64 columns);
+//   warps 2-3   MMA issuers, one per group: S = Q K^T, then O += P V of the tile before;
+//   warps 4-7,  softmax, one thread per query row.  The row's scores are read from TMEM once
+//   8-11        into registers (the first warpgroup hands registers over) and the S buffer
+//               is free for the next tile at once; the probabilities go to TMEM columns of
+//               their own, from where the second product takes them as its operand.
+// With 64 columns a key tile has 128 keys, with 128 columns 64: S, P and O of a group take
+// 256 (224) TMEM columns.  A tile's exponentials take the SFU 1,024 (512) clocks, as long
+// as its products take the tensor cores: that is the bound.
 // Every wait is bounded: a timeout sets LF_STATUS_TIMEOUT and the roles unwind.
 #include <cmath>
 #include <cstring>
@@ -407,12 +408,12 @@ struct Shape {
   static constexpr int kBlocks = kD / 64;             // 64-column SW128 blocks of a head's row
   static constexpr int kQBytes = kRows * kD * 2;
   static constexpr int kKvBytes = kKeys * kD * 2;     // 16 KB
-  static constexpr int kKStages = kD == 64 ? 6 : 5;
-  static constexpr int kVStages = 5;
-  static constexpr int kBufs = kD == 64 ? 3 : 4;      // TMEM score buffers shared by the groups
-  static constexpr int kOCol = kBufs * kKeys;         // group g's O at TMEM column kOCol + kD g
-  static constexpr int kSmem = 1024 + kGroups * kQBytes + (kKStages + kVStages) * kKvBytes + 1024;
-  static_assert(kOCol + kGroups * kD <= 512, "TMEM columns");
+  static constexpr int kStages = kD == 64 ? 3 : 2;    // K stages and V stages of a group
+  // TMEM columns of a group: S, then P (two probabilities a column), then O
+  static constexpr int kPCol = kKeys, kOCol = kKeys + kKeys / 2;
+  static constexpr int kGroupBytes = kQBytes + 2 * kStages * kKvBytes;
+  static constexpr int kSmem = 1024 + kGroups * kGroupBytes + 1024;
+  static_assert(kOCol + kD <= 256, "TMEM columns of a group");
   static_assert(kSmem <= 232448, "above the 227 KB of shared memory a CTA may use");
 };
 
@@ -495,78 +496,54 @@ struct Cursor {
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_constant__ CrossParams p) {
   using Sh = Shape<kD>;
-  constexpr int kKeys = Sh::kKeys, kKvBytes = Sh::kKvBytes;
+  constexpr int kKeys = Sh::kKeys, kKvBytes = Sh::kKvBytes, kStages = Sh::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int grp = warp < 4 ? warp & 1 : (warp - 4) >> 2;  // the group this warp works for
 
-  const uint32_t sQ = base;
-  const uint32_t sK = sQ + kGroups * Sh::kQBytes;
-  const uint32_t sV = sK + Sh::kKStages * kKvBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(gbase + (sV + Sh::kVStages * kKvBytes - base));
-  auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  // per-group barriers at index (kind * kGroups + group)
-  constexpr int Q_FULL = 0, Q_EMPTY = 1, P_FULL = 2, O_FULL = 3, O_EMPTY = 4, PV_DONE = 5;
-  auto gbar = [&](int kind, int grp) { return bar(kind * kGroups + grp); };
-  constexpr int S_FULL = 6 * kGroups, BUF_EMPTY = S_FULL + Sh::kBufs, K_FULL = BUF_EMPTY + Sh::kBufs,
-                K_EMPTY = K_FULL + Sh::kKStages, V_FULL = K_EMPTY + Sh::kKStages, V_EMPTY = V_FULL + Sh::kVStages,
-                DRAIN = V_EMPTY + Sh::kVStages, N_BARS = DRAIN + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(&bars[N_BARS]);
+  const uint32_t sQ = base + grp * Sh::kGroupBytes;
+  const uint32_t sK = sQ + Sh::kQBytes;
+  const uint32_t sV = sK + kStages * kKvBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(gbase + kGroups * Sh::kGroupBytes);
+  constexpr int Q_FULL = 0, Q_EMPTY = 1, S_FULL = 2, S_EMPTY = 3, P_FULL = 4, PV_DONE = 5, O_FULL = 6, O_EMPTY = 7,
+                DRAIN = 8, K_FULL = 9, K_EMPTY = K_FULL + kStages, V_FULL = K_EMPTY + kStages, V_EMPTY = V_FULL + kStages,
+                N_BARS = V_EMPTY + kStages;  // of a group
+  auto bar = [&](int i) { return smem_u32(&bars[grp * N_BARS + i]); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(&bars[kGroups * N_BARS]);
   int32_t* s_abort = reinterpret_cast<int32_t*>(tmem_slot + 1);
   const int64_t n_units = int64_t(p.n_items) * p.n_heads;
 
-  if (tid == 0) {
-    for (int grp = 0; grp < kGroups; ++grp) {
-      mbar_init(gbar(Q_FULL, grp), 1);
-      mbar_init(gbar(Q_EMPTY, grp), 1);
-      mbar_init(gbar(P_FULL, grp), 4);
-      mbar_init(gbar(O_FULL, grp), 1);
-      mbar_init(gbar(O_EMPTY, grp), 4);
-      mbar_init(gbar(PV_DONE, grp), 1);
-    }
-    for (int i = 0; i < Sh::kBufs; ++i) {
-      mbar_init(bar(S_FULL + i), 1);
-      mbar_init(bar(BUF_EMPTY + i), 1);
-    }
-    for (int i = 0; i < Sh::kKStages; ++i) {
-      mbar_init(bar(K_FULL + i), 1);
-      mbar_init(bar(K_EMPTY + i), 1);
-    }
-    for (int i = 0; i < Sh::kVStages; ++i) {
-      mbar_init(bar(V_FULL + i), 1);
-      mbar_init(bar(V_EMPTY + i), 1);
-    }
-    mbar_init(bar(DRAIN), 1);
-    *s_abort = 0;
+  if (warp < kGroups && lane == 0) {  // each producer warp: its group's barriers
+    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i == S_EMPTY || i == P_FULL || i == O_EMPTY ? 4 : 1);
+    if (warp == 0) *s_abort = 0;
     fence_mbar_init();
     prefetch_tmap(&p.q_map);
     prefetch_tmap(&p.k_map);
     prefetch_tmap(&p.v_map);
   }
-  if (warp == 1) {
+  if (warp == 2) {
     __syncwarp();
     tmem_alloc(smem_u32(tmem_slot), 512);
   }
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = *tmem_slot + uint32_t(grp) * 256;
   pdl_wait();
   pdl_launch_dependents();
 
-  auto fail = [&]() {
-    set_status(p.status, LF_STATUS_TIMEOUT);
-    atomicExch(s_abort, 1);
-  };
+  // by a whole warp, and by one lane
+  auto wwait = [&](uint32_t b, uint32_t parity) { return warp_wait(b, parity, s_abort, p.status); };
   auto wait = [&](uint32_t b, uint32_t parity) {
     if (mbar_try_wait(b, parity)) return true;
     if (aborted(s_abort)) return false;
     if (mbar_wait(b, parity)) return true;
-    if (!aborted(s_abort)) fail();
+    set_status(p.status, LF_STATUS_TIMEOUT);
+    atomicExch(s_abort, 1);
     return false;
   };
-  auto wwait = [&](uint32_t b, uint32_t parity) { return warp_wait(b, parity, s_abort, p.status); };  // by a whole warp
   auto unit_of = [&](int64_t unit) {
     const Rec r = read_rec(p, int(unit / p.n_heads));
     if (!r.ok) {
@@ -581,13 +558,17 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
   // first), the order of the groups turned round from round to round: a group that had a
   // longer unit gets a shorter one next.
   const int64_t n_slots = int64_t(kGroups) * gridDim.x;
-  auto start = [&](Cursor& c, int grp) {
-    c.unit = blockIdx.x + int64_t(grp) * gridDim.x;
-    c.u = c.t = c.j = 0;
+  auto load = [&](Cursor& c) {
+    c.j = 0;
     if (c.unit < n_units) {
       c.it = unit_of(c.unit);
       c.n_kv = (c.it.nk + kKeys - 1) / kKeys;
     }
+  };
+  auto start = [&](Cursor& c) {
+    c.unit = blockIdx.x + int64_t(grp) * gridDim.x;
+    c.u = c.t = 0;
+    load(c);
   };
   auto advance = [&](Cursor& c) {
     ++c.t;
@@ -595,153 +576,132 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
     const int64_t in_round = c.unit - c.u * n_slots;
     ++c.u;
     c.unit = c.u * n_slots + (n_slots - 1 - in_round);
-    c.j = 0;
-    if (c.unit < n_units) {
-      c.it = unit_of(c.unit);
-      c.n_kv = (c.it.nk + kKeys - 1) / kKeys;
-    }
+    load(c);
   };
-  auto live = [&](const Cursor& c) { return c.unit < n_units; };
+  // A tile of at most 64 queries sits in the upper 64 rows for group 1, so that the two
+  // groups' busy warps lie on different schedulers.
+  auto shift_of = [&](const Unit& it) { return grp == 1 && it.nq - it.tile * kRows <= 64 ? 64 : 0; };
 
   if (warp < 4) {
     set_max_regs_dec<kRegsIssue>();
-    if (warp == 0) {
+    if (warp < 2) {
       // ------------------------------------------------------------ producer
-      Cursor c[kGroups];
-      for (int grp = 0; grp < kGroups; ++grp) start(c[grp], grp);
-      int kc = 0, nq[kGroups] = {0, 0};
+      Cursor c;
+      start(c);
       bool stop = false;
-      while (!stop && (live(c[0]) || live(c[1]))) {
-#pragma unroll
-        for (int grp = 0; grp < kGroups; ++grp) {
-          Cursor& cg = c[grp];
-          if (stop || !live(cg)) continue;
-          const int h = int(cg.unit % p.n_heads), hk = h / p.group;
-          if (cg.j == 0) {  // the unit's Q tile, once the group's previous unit has no S left to issue
-            if (!wwait(gbar(Q_EMPTY, grp), (cg.u & 1) ^ 1)) {
-              stop = true;
-              continue;
-            }
-            if (elect_one()) {
-              mbar_arrive_expect_tx(gbar(Q_FULL, grp), Sh::kQBytes);
-              for (int b = 0; b < Sh::kBlocks; ++b)
-                tma_load_3d(sQ + grp * Sh::kQBytes + b * (kRows * 128), &p.q_map, gbar(Q_FULL, grp), b * 64, h,
-                            cg.it.q0 + cg.it.tile * kRows);
-            }
-            ++nq[grp];
-          }
-          const int sk = kc % Sh::kKStages, sv = kc % Sh::kVStages;
-          const int32_t krow = cg.it.k0 + cg.j * kKeys;
-          if (!wwait(bar(K_EMPTY + sk), ((kc / Sh::kKStages) & 1) ^ 1)) {
-            stop = true;
-            continue;
-          }
+      while (!stop && c.unit < n_units) {
+        const int h = int(c.unit % p.n_heads), hk = h / p.group;
+        const int s = c.t % kStages;
+        const uint32_t ph = ((c.t / kStages) & 1) ^ 1;
+        if (c.j == 0) {  // the unit's Q tile, once the previous unit has no S left to issue
+          if (!wwait(bar(Q_EMPTY), (c.u & 1) ^ 1)) break;
           if (elect_one()) {
-            mbar_arrive_expect_tx(bar(K_FULL + sk), kKvBytes);
+            mbar_arrive_expect_tx(bar(Q_FULL), Sh::kQBytes);
             for (int b = 0; b < Sh::kBlocks; ++b)
-              tma_load_3d(sK + sk * kKvBytes + b * (kKeys * 128), &p.k_map, bar(K_FULL + sk), b * 64, hk, krow);
+              tma_load_3d(sQ + b * (kRows * 128), &p.q_map, bar(Q_FULL), b * 64, h,
+                          c.it.q0 + c.it.tile * kRows - shift_of(c.it));
           }
-          if (!wwait(bar(V_EMPTY + sv), ((kc / Sh::kVStages) & 1) ^ 1)) {
-            stop = true;
-            mbar_wait(bar(K_FULL + sk), (kc / Sh::kKStages) & 1);  // this tile's K lands; its V was not issued
-            continue;
-          }
-          if (elect_one()) {
-            mbar_arrive_expect_tx(bar(V_FULL + sv), kKvBytes);
-            for (int b = 0; b < Sh::kBlocks; ++b)
-              tma_load_3d(sV + sv * kKvBytes + b * (kKeys * 128), &p.v_map, bar(V_FULL + sv), b * 64, hk, krow);
-          }
-          ++kc;
-          advance(cg);
+          __syncwarp();
         }
+        const int32_t krow = c.it.k0 + c.j * kKeys;
+        stop = !wwait(bar(K_EMPTY + s), ph);
+        if (stop) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bar(K_FULL + s), kKvBytes);
+          for (int b = 0; b < Sh::kBlocks; ++b)
+            tma_load_3d(sK + s * kKvBytes + b * (kKeys * 128), &p.k_map, bar(K_FULL + s), b * 64, hk, krow);
+        }
+        __syncwarp();
+        stop = !wwait(bar(V_EMPTY + s), ph);
+        if (stop) {
+          mbar_wait(bar(K_FULL + s), ph ^ 1);  // this tile's K lands; its V was not issued
+          break;
+        }
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bar(V_FULL + s), kKvBytes);
+          for (int b = 0; b < Sh::kBlocks; ++b)
+            tma_load_3d(sV + s * kKvBytes + b * (kKeys * 128), &p.v_map, bar(V_FULL + s), b * 64, hk, krow);
+        }
+        __syncwarp();
+        advance(c);
       }
       __syncwarp();
       if (aborted(s_abort)) {  // loads nobody consumed must land before the CTA exits (bounded)
-        for (int q = (kc > Sh::kKStages ? kc - Sh::kKStages : 0); q < kc; ++q)
-          mbar_wait(bar(K_FULL + q % Sh::kKStages), (q / Sh::kKStages) & 1);
-        for (int q = (kc > Sh::kVStages ? kc - Sh::kVStages : 0); q < kc; ++q)
-          mbar_wait(bar(V_FULL + q % Sh::kVStages), (q / Sh::kVStages) & 1);
-        for (int grp = 0; grp < kGroups; ++grp)  // only a group's latest Q can be unconsumed
-          if (nq[grp] > 0) mbar_wait(gbar(Q_FULL, grp), (nq[grp] - 1) & 1);
+        for (int q = (c.t > kStages ? c.t - kStages : 0); q < c.t; ++q) {
+          mbar_wait(bar(K_FULL + q % kStages), (q / kStages) & 1);
+          mbar_wait(bar(V_FULL + q % kStages), (q / kStages) & 1);
+        }
+        const int nq = c.u + (c.unit < n_units && c.j > 0 ? 1 : 0);  // only the latest Q can be unconsumed
+        if (nq > 0) mbar_wait(bar(Q_FULL), (nq - 1) & 1);
       }
-    } else if (warp == 1) {
+    } else {
       // ------------------------------------------------------------ MMA issuer
       const int nks = (p.d + 15) / 16;  // 16-column steps of a head's row
       const uint32_t idesc_o = umma_idesc_f16(DT<T>::umma_fmt, kRows, uint32_t(nks) * 16, /*a_mn=*/0, /*b_mn=*/1);
-      struct Prev { bool valid, first, last; int t, u, kv, n16; };  // n16: 16-key steps of O += P V
-      Cursor c[kGroups];
-      Prev prev[kGroups];
-      for (int grp = 0; grp < kGroups; ++grp) {
-        start(c[grp], grp);
-        prev[grp].valid = false;
-      }
-      int kc = 0;
-      bool stop = false;
-      // O_grp += P V for the group's previous tile, P in the tile's score buffer
-      auto pv = [&](int grp, const Prev& e) -> bool {
-        const int sv = e.kv % Sh::kVStages, sb = e.kv % Sh::kBufs;
-        if (!wwait(bar(V_FULL + sv), (e.kv / Sh::kVStages) & 1)) return false;
-        if (e.first && !wwait(gbar(O_EMPTY, grp), (e.u & 1) ^ 1)) return false;
-        if (!wwait(gbar(P_FULL, grp), e.t & 1)) return false;
-        tc_fence_after();
-        const uint64_t vd = smem_desc(sV + sv * kKvBytes, kKeys * 128, 1024, 2);
-        const uint32_t d = tmem + Sh::kOCol + kD * grp, a = tmem + kKeys * sb;
-        if (elect_one()) {
+      const uint64_t q_desc = smem_desc(sQ, 16, 1024, 2), k_desc0 = smem_desc(sK, 16, 1024, 2),
+                     v_desc0 = smem_desc(sV, kKeys * 128, 1024, 2);
+      Cursor c;
+      start(c);
+      bool prev = false, prev_first = false, prev_last = false;  // the tile whose O += P V is still to be issued
+      int prev_n16 = 0, prev_t = 0, prev_u = 0;
+      while (true) {
+        const bool now = c.unit < n_units;
+        if (!now && !prev) break;
+        bool first = false, last = false;
+        int n16 = 0;
+        const int t = c.t, u = c.u;
+        if (now) {
+          const int s = t % kStages;
+          if ((c.j == 0 && !wwait(bar(Q_FULL), u & 1)) || !wwait(bar(K_FULL + s), (t / kStages) & 1) ||
+              !wwait(bar(S_EMPTY), (t & 1) ^ 1))
+            break;
+          tc_fence_after();
+          // S over the tile's keys, to the next multiple of 16
+          first = c.j == 0;
+          last = c.j == c.n_kv - 1;
+          n16 = (min(kKeys, c.it.nk - c.j * kKeys) + 15) / 16;
+          const uint32_t idesc = umma_idesc_f16(DT<T>::umma_fmt, kRows, uint32_t(n16) * 16, 0, 0);
+          const uint64_t kd = k_desc0 + uint64_t(s * (kKvBytes >> 4));
+          if (elect_one()) {
 #pragma unroll
-          for (int t = 0; t < kKeys / 16; ++t) {  // 16 value rows are 2,048 bytes
-            if (t < e.n16) umma_f16_ta(d, a + t * 8, vd + uint64_t(t * 128), idesc_o, (e.first && t == 0) ? 0u : 1u);
-          }
-          umma_commit(bar(BUF_EMPTY + sb));
-          umma_commit(bar(V_EMPTY + sv));
-          umma_commit(gbar(PV_DONE, grp));
-          if (e.last) umma_commit(gbar(O_FULL, grp));
-        }
-        __syncwarp();
-        return true;
-      };
-      while (!stop && (live(c[0]) || live(c[1]) || prev[0].valid || prev[1].valid)) {
-#pragma unroll
-        for (int grp = 0; grp < kGroups; ++grp) {
-          if (stop) continue;
-          Cursor& cg = c[grp];
-          Prev cur{false, false, false, 0, 0, 0, 0};
-          if (live(cg)) {
-            const int sk = kc % Sh::kKStages, sb = kc % Sh::kBufs;
-            if ((cg.j == 0 && !wwait(gbar(Q_FULL, grp), cg.u & 1)) ||
-                !wwait(bar(K_FULL + sk), (kc / Sh::kKStages) & 1) ||
-                !wwait(bar(BUF_EMPTY + sb), ((kc / Sh::kBufs) & 1) ^ 1)) {
-              stop = true;
-              continue;
+            for (int i = 0; i < kD / 16; ++i) {  // 16 columns are 32 bytes, 64 of them a block
+              if (i < nks)
+                umma_f16(tmem, q_desc + uint64_t((i >> 2) * (kRows * 8) + (i & 3) * 2),
+                         kd + uint64_t((i >> 2) * (kKeys * 8) + (i & 3) * 2), idesc, i > 0 ? 1u : 0u);
             }
-            tc_fence_after();
-            const uint64_t qd = smem_desc(sQ + grp * Sh::kQBytes, 16, 1024, 2);
-            const uint64_t kd = smem_desc(sK + sk * kKvBytes, 16, 1024, 2);
-            // S over the tile's keys, to the next multiple of 16
-            const int n16 = (min(kKeys, cg.it.nk - cg.j * kKeys) + 15) / 16;
-            const uint32_t idesc = umma_idesc_f16(DT<T>::umma_fmt, kRows, uint32_t(n16) * 16, 0, 0);
-            const bool last = cg.j == cg.n_kv - 1;
-            if (elect_one()) {
-#pragma unroll
-              for (int t = 0; t < kD / 16; ++t) {  // 16 columns are 32 bytes, 64 of them a block
-                if (t < nks)
-                  umma_f16(tmem + kKeys * sb, qd + uint64_t((t >> 2) * (kRows * 8) + (t & 3) * 2),
-                           kd + uint64_t((t >> 2) * (kKeys * 8) + (t & 3) * 2), idesc, t > 0 ? 1u : 0u);
-              }
-              umma_commit(bar(S_FULL + sb));
-              umma_commit(bar(K_EMPTY + sk));
-              if (last) umma_commit(gbar(Q_EMPTY, grp));
-            }
-            __syncwarp();
-            cur = Prev{true, cg.j == 0, last, cg.t, cg.u, kc, n16};
-            ++kc;
-            advance(cg);
+            umma_commit(bar(S_FULL));
+            umma_commit(bar(K_EMPTY + s));
+            if (last) umma_commit(bar(Q_EMPTY));
           }
-          if (prev[grp].valid && !pv(grp, prev[grp])) {
-            stop = true;
-            continue;
-          }
-          prev[grp] = cur;
+          __syncwarp();
+          advance(c);
         }
+        if (prev) {  // O += P V of the tile before
+          const int s = prev_t % kStages;
+          if (!wwait(bar(V_FULL + s), (prev_t / kStages) & 1) || (prev_first && !wwait(bar(O_EMPTY), (prev_u & 1) ^ 1)) ||
+              !wwait(bar(P_FULL), prev_t & 1))
+            break;
+          tc_fence_after();
+          const uint64_t vd = v_desc0 + uint64_t(s * (kKvBytes >> 4));
+          if (elect_one()) {
+#pragma unroll
+            for (int i = 0; i < kKeys / 16; ++i) {  // 16 value rows are 2,048 bytes
+              if (i < prev_n16)
+                umma_f16_ta(tmem + Sh::kOCol, tmem + Sh::kPCol + i * 8, vd + uint64_t(i * 128), idesc_o,
+                            (prev_first && i == 0) ? 0u : 1u);
+            }
+            umma_commit(bar(V_EMPTY + s));
+            umma_commit(bar(PV_DONE));
+            if (prev_last) umma_commit(bar(O_FULL));
+          }
+          __syncwarp();
+        }
+        prev = now;
+        prev_first = first;
+        prev_last = last;
+        prev_n16 = n16;
+        prev_t = t;
+        prev_u = u;
       }
       __syncwarp();
       if (aborted(s_abort)) {  // every issued MMA must finish before TMEM is released (bounded)
@@ -752,46 +712,31 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
     }
     __syncwarp();
   } else {
-    // ------------------------------------------------------------ softmax groups (warps 4..11)
+    // ------------------------------------------------------------ softmax (warps 4..11)
     set_max_regs_inc<kRegsSoftmax>();
-    const int grp = (warp - 4) >> 2;
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
-    const uint32_t lane_addr = tmem + (uint32_t(quad * 32) << 16);
-    const uint32_t o_addr = lane_addr + Sh::kOCol + kD * grp;   // this row of the group's O
+    const uint32_t s_addr = tmem + (uint32_t(quad * 32) << 16);  // this row of S
+    const uint32_t p_addr = s_addr + Sh::kPCol, o_addr = s_addr + Sh::kOCol;
     const float2 sl2 = f2(p.scale_log2);
-    // The MMA warp issues the groups' S tiles round-robin (group 0 first), so this
-    // group's n-th tile is global tile n + min(n + grp, tiles of the other group).
-    int other_tiles = 0;
-    {
-      Cursor o;
-      start(o, grp ^ 1);
-      while (live(o)) {
-        other_tiles += o.n_kv;
-        o.j = o.n_kv - 1;
-        advance(o);
-      }
-    }
     Cursor c;
-    start(c, grp);
+    start(c);
     float m = -INFINITY, l = 0.f;
-    while (live(c)) {
+    while (c.unit < n_units) {
       const int t = c.t, j = c.j;
-      const int kc = t + min(t + grp, other_tiles);
-      const int sb = kc % Sh::kBufs;
-      const uint32_t s_addr = lane_addr + kKeys * sb;
       const bool last = j == c.n_kv - 1;
       const int nvalid = min(kKeys, c.it.nk - j * kKeys);
-      // a warp whose 32 query rows all lie past the queries' end does no softmax (its P rows
-      // only feed O rows that are never stored)
-      const bool rows_live = quad * 32 < c.it.nq - c.it.tile * kRows;
-      const bool work = __all_sync(0xffffffffu, wait(bar(S_FULL + sb), (kc / Sh::kBufs) & 1));
+      // a warp whose 32 rows hold no query does no softmax (its P rows only feed O rows that
+      // are never stored)
+      const int shift = shift_of(c.it), n_rows = c.it.nq - c.it.tile * kRows;
+      const bool rows_live = quad * 32 + 31 >= shift && quad * 32 < shift + n_rows;
+      const bool work = wwait(bar(S_FULL), t & 1);
       tc_fence_after();
       float sum = 0.f, m_new = m, alpha = 1.f;
+      // the row's scores, all in registers; a short tile reads its first 64 alone
+      uint32_t s[kKeys];
+      const bool wide = kKeys == 128 && nvalid > 64;
       if (work && rows_live) {
-        // the row's scores, all in registers; a short tile reads its first 64 alone
-        uint32_t s[kKeys];
-        const bool wide = kKeys == 128 && nvalid > 64;
         if constexpr (kKeys == 128) {
           if (wide) {
             tmem_ld128(s_addr, s);
@@ -804,6 +749,12 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
         } else {
           tmem_ld64(s_addr, s);
         }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(S_EMPTY));  // S has been read: the next may be computed
+      bool go = work;  // the previous tile's O += P V has finished: P and O are this warp's
+      if (work && rows_live) {
         if (nvalid < kKeys) {  // warp-uniform: keys past the end score -inf, so they do not count
 #pragma unroll
           for (int q = 0; q < kKeys; ++q)
@@ -823,9 +774,9 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
         m_new = (j == 0 || mx > m + kMaxSlack) ? mx : m;
         const float m_use = m_new == -INFINITY ? 0.f : m_new;  // every score so far is -inf: p = 0
         alpha = (j == 0) ? 1.f : sfu_ex2(m - m_use);
-        if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
-          // O moves to the new maximum, once the previous tile's O += P V has finished
-          if (__all_sync(0xffffffffu, wait(gbar(PV_DONE, grp), (t & 1) ^ 1))) {
+        if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {  // O moves to the new maximum
+          go = wwait(bar(PV_DONE), (t & 1) ^ 1);
+          if (go) {
             tc_fence_after();
 #pragma unroll 1
             for (int b = 0; b < 2 * Sh::kBlocks; ++b) {
@@ -837,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
             }
           }
         }
-        // p = 2^(s - max), rounded to T, over the scores' own TMEM columns (two keys a column)
+        // p = 2^(s - max), rounded to T, two keys a column
         float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         const float2 neg_m = f2(-m_use);
 #pragma unroll
@@ -852,18 +803,21 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
               sums[i & 1] = f2_add(sums[i & 1], pr);
               w[i] = Pack2<T>::pack(pr.x, pr.y);
             }
-            tmem_st32(s_addr + hh * 32, w);
+            if (hh == 0) go = wwait(bar(PV_DONE), (t & 1) ^ 1);
+            if (go) tmem_st32(p_addr + hh * 32, w);
           }
         }
         sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+      } else {
+        go = work && wwait(bar(PV_DONE), (t & 1) ^ 1);
       }
       l = (j == 0) ? sum : l * alpha + sum;
       m = m_new;
       // the last 16-key step of a tile that ends inside it multiplies value rows past the
       // sequence's end by p = 0: those rows become zeros first (they may hold NaN)
       if ((nvalid & 15) != 0) {
-        const int sv = kc % Sh::kVStages;
-        if (__all_sync(0xffffffffu, work && wait(bar(V_FULL + sv), (kc / Sh::kVStages) & 1))) {
+        const int sv = t % kStages;
+        if (go && wwait(bar(V_FULL + sv), (t / kStages) & 1)) {
           const int n_zero = 16 - (nvalid & 15);
           uint8_t* vrow = gbase + (sV + sv * kKvBytes - base) + nvalid * 128;
           for (int i = row; i < n_zero * 8 * Sh::kBlocks; i += kRows) {
@@ -873,28 +827,27 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
           fence_proxy_async_smem();
         }
       }
+      // This warp has seen PV_DONE of the tile before, so every warp of the group has arrived
+      // for that tile and the MMA warp has seen it: this arrival counts for this tile only.
       tc_fence_before();
       __syncwarp();
-      // The next S may already be there, so without a wait a warp could arrive for this tile
-      // before a slower one has for the last, or all of them before the MMA thread has seen
-      // the last tile's phase: PV_DONE of the last tile says that both have happened.
-      if (lane == 0 && wait(gbar(PV_DONE, grp), (t & 1) ^ 1)) mbar_arrive(gbar(P_FULL, grp));
-      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(P_FULL));
       if (last) {
         // the unit's output: O / l, once its last O += P V has finished
-        if (__all_sync(0xffffffffu, wait(gbar(O_FULL, grp), c.u & 1)) && rows_live) {
+        if (wwait(bar(O_FULL), c.u & 1) && rows_live) {
           tc_fence_after();
-          const int qr = c.it.tile * kRows + row, what = c.it.what;
+          const int r = row - shift, what = c.it.what;  // row of the query tile
           const float inv = l == 0.f ? 0.f : 1.f / l;
-          T* dst = reinterpret_cast<T*>(p.out) + int64_t(c.it.q0 + qr) * p.ldo + int64_t(c.unit % p.n_heads) * p.d;
+          T* dst = reinterpret_cast<T*>(p.out) + (int64_t(c.it.q0) + c.it.tile * kRows + r) * p.ldo +
+                   int64_t(c.unit % p.n_heads) * p.d;
 #pragma unroll 1
-          for (int b = 0; b < Sh::kBlocks; ++b) {
-            uint32_t ov[64];
-            tmem_ld64(o_addr + b * 64, ov);
-            if (qr < c.it.nq && what != 1) {
+          for (int b = 0; b < 2 * Sh::kBlocks; ++b) {
+            uint32_t ov[32];
+            tmem_ld32(o_addr + b * 32, ov);
+            if (r >= 0 && r < n_rows && what != 1) {
 #pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                if (b * 64 + q * 8 >= p.d) break;
+              for (int q = 0; q < 4; ++q) {
+                if (b * 32 + q * 8 >= p.d) break;
                 uint4 w;
                 if (what == 2) {  // no keys: zeros, whatever the key row read in their place holds
                   w = make_uint4(0u, 0u, 0u, 0u);
@@ -904,14 +857,14 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
                   w.z = Pack2<T>::pack(__uint_as_float(ov[8 * q + 4]) * inv, __uint_as_float(ov[8 * q + 5]) * inv);
                   w.w = Pack2<T>::pack(__uint_as_float(ov[8 * q + 6]) * inv, __uint_as_float(ov[8 * q + 7]) * inv);
                 }
-                reinterpret_cast<uint4*>(dst + b * 64)[q] = w;
+                reinterpret_cast<uint4*>(dst + b * 32)[q] = w;
               }
             }
           }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(gbar(O_EMPTY, grp));
+        if (lane == 0) mbar_arrive(bar(O_EMPTY));
       }
       advance(c);
     }
@@ -919,9 +872,9 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
 
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) {
+  if (warp == 2) {
     __syncwarp();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(*tmem_slot, 512);
   }
 }
 
