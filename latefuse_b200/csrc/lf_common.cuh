@@ -201,6 +201,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
+// Whether the phase has completed, without ever suspending the thread.
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
 // try_wait that lets the hardware suspend the thread until the phase
 // completes or `hint_ns` passes, instead of returning at once: a waiting warp
 // then takes no issue slots from the warps sharing its scheduler.
@@ -235,6 +248,10 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is)::"memory");
   return is != 0;
 }
+
+// A value that is the same in every lane of a converged warp, marked so for the compiler.
+template <typename T>
+__device__ __forceinline__ T uniform(T v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // mbar_wait by a whole converged warp, whose lanes all get the same answer.  `abort` (a
 // shared word another role sets when it gives up) is looked at before a wait that would

@@ -112,8 +112,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t rank = cluster_ctarank();  // 0: the leader, which issues the MMAs
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
+  const uint32_t rank = uniform(cluster_ctarank());  // 0: the leader, which issues the MMAs
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
   constexpr int kOutBuf = out_buf(sizeof(T));
 
@@ -148,51 +148,45 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
   __syncthreads();
   cluster_sync();  // both CTAs' barriers exist before either signals the other's
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   pdl_wait();
   pdl_launch_dependents();
 
-  auto fail = [&]() {
-    set_status(p.status, LF_STATUS_TIMEOUT);
-    atomicExch(s_abort, 1);
-  };
-  auto wait = [&](uint32_t b, uint32_t parity) {
-    if (aborted(s_abort)) return false;
-    if (mbar_wait(b, parity)) return true;
-    if (!aborted(s_abort)) fail();
-    return false;
-  };
+  auto wait = [&](uint32_t b, uint32_t parity) { return warp_wait(b, parity, s_abort, p.status); };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer (both CTAs)
-    if (lane == 0) {
-      int kk = 0;
-      bool stop = false;
-      for (int64_t t = pair; t < p.n_tiles && !stop; t += n_pairs) {
-        const int32_t m0 = int32_t(t / p.n_tiles_n) * (2 * kBM) + int32_t(rank) * kBM;
-        const int32_t n0 = int32_t(t % p.n_tiles_n) * kBN + int32_t(rank) * (kBN / 2);
-        for (int kb = 0; kb < p.n_kb; ++kb, ++kk) {
-          const int s = kk % kStages;
-          if (!wait(bar(EMPTY + s), ((kk / kStages) & 1) ^ 1)) {
-            stop = true;
-            break;
-          }
+    int kk = 0;
+    bool stop = false;
+    for (int64_t t = pair; t < p.n_tiles && !stop; t += n_pairs) {
+      const int32_t m0 = int32_t(t / p.n_tiles_n) * (2 * kBM) + int32_t(rank) * kBM;
+      const int32_t n0 = int32_t(t % p.n_tiles_n) * kBN + int32_t(rank) * (kBN / 2);
+      for (int kb = 0; kb < p.n_kb; ++kb, ++kk) {
+        const int s = kk % kStages;
+        if (!wait(bar(EMPTY + s), ((kk / kStages) & 1) ^ 1)) {
+          stop = true;
+          break;
+        }
+        if (elect_one()) {
           const uint32_t st = base + s * kStageBytes;
           const uint32_t full = mapa_shared(bar(FULL + s), 0);
           if (rank == 0) mbar_arrive_expect_tx(bar(FULL + s), 2 * kStageBytes);
           tma_load_2d_pair(st, &p.x_map, full, kb * kBK, m0);
           tma_load_2d_pair(st + kABytes, &p.w_map, full, kb * kBK, n0);
         }
-      }
-      if (aborted(s_abort) && rank == 0) {  // loads nobody consumed land before the CTA exits (bounded)
-        for (int q = (kk > kStages ? kk - kStages : 0); q < kk; ++q)
-          mbar_wait(bar(FULL + q % kStages), (q / kStages) & 1);
+        __syncwarp();
       }
     }
+    if (aborted(s_abort) && rank == 0) {  // loads nobody consumed land before the CTA exits (bounded)
+      for (int q = (kk > kStages ? kk - kStages : 0); q < kk; ++q)
+        mbar_wait(bar(FULL + q % kStages), (q / kStages) & 1);
+    }
+    __syncwarp();
   } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer (the leader's lane 0)
-    if (lane == 0 && rank == 0) {
+    // ------------------------------------------------------------ MMA issuer (the leader)
+    if (rank == 0) {
       constexpr uint32_t idesc = umma_idesc_i8(2 * kBM, kBN);
+      const uint64_t a_desc = smem_desc(base, 16, 1024, 2), b_desc = smem_desc(base + kABytes, 16, 1024, 2);
       int kk = 0, n_it = 0;
       bool stop = false;
       for (int64_t t = pair; t < p.n_tiles && !stop; t += n_pairs, ++n_it) {
@@ -206,20 +200,25 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
             break;
           }
           tc_fence_after();
-          const uint32_t st = base + s * kStageBytes;
+          if (elect_one()) {
+            const uint64_t off = uint64_t(s * (kStageBytes >> 4));
 #pragma unroll
-          for (int q = 0; q < kBK / 32; ++q)
-            umma_i8_pair(tmem + a * kBN, smem_desc(st + q * 32, 16, 1024, 2),
-                         smem_desc(st + kABytes + q * 32, 16, 1024, 2), idesc, (kb | q) != 0 ? 1u : 0u);
-          umma_commit_pair(bar(EMPTY + s));
+            for (int q = 0; q < kBK / 32; ++q)  // 32 bytes of K a step
+              umma_i8_pair(tmem + a * kBN, a_desc + off + uint64_t(2 * q), b_desc + off + uint64_t(2 * q), idesc,
+                           (kb | q) != 0 ? 1u : 0u);
+            umma_commit_pair(bar(EMPTY + s));
+            if (kb == p.n_kb - 1) umma_commit_pair(bar(ACC_FULL + a));
+          }
+          __syncwarp();
         }
-        if (!stop) umma_commit_pair(bar(ACC_FULL + a));
       }
       if (aborted(s_abort)) {  // every issued MMA finishes before TMEM is released (bounded)
-        umma_commit_pair_local(bar(DRAIN));
+        if (elect_one()) umma_commit_pair_local(bar(DRAIN));
+        __syncwarp();
         mbar_wait(bar(DRAIN), 0);
       }
     }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
     const int quad = warp & 3;
@@ -237,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
       const int64_t m0 = (t / p.n_tiles_n) * (2 * kBM) + int64_t(rank) * kBM + quad * 32;  // this warp's 32 rows
       const int32_t n0 = int32_t(t % p.n_tiles_n) * kBN;
       const float xs = m0 + lane < p.m_rows ? __ldg(p.x_scale + m0 + lane) : 0.f;
-      if (!__all_sync(0xffffffffu, wait(bar(ACC_FULL + a), (n_it >> 1) & 1))) break;
+      if (!wait(bar(ACC_FULL + a), (n_it >> 1) & 1)) break;
       tc_fence_after();
       for (int c = c_begin; c < c_end; ++c) {
         const int col0 = n0 + c * kOutCols;
