@@ -16,7 +16,7 @@
 //   warp 0      TMA producer (both CTAs): an x box {128, 128} and a w box {128, 128} into
 //               a 6-stage ring, completing on the leader's barrier;
 //   warp 1      MMA issuer (leader only); TMEM holds two 256-column accumulators;
-//   warps 2-9   epilogue (both CTAs), two warps per TMEM lane quadrant, 128 columns each,
+//   warps 2-17  epilogue (both CTAs), four warps per TMEM lane quadrant, 64 columns each,
 //               32 at a time: staged per warp and written by TMA, or by the warp row by row
 //               where y's rows are not 16-byte aligned.
 //
@@ -52,6 +52,7 @@ struct alignas(64) LinearInt8Params {
   int64_t n_tiles;
   int32_t n, n_tiles_n, n_kb;
   int32_t tma_out;    // y's base and row stride are 16-byte aligned
+  int32_t vec_ch;     // w_scale and bias are aligned for pairs
   int32_t split;      // split kernel: CTAs of the cluster that share a tile's K
   int32_t* status;
 };
@@ -83,12 +84,73 @@ __host__ __device__ constexpr uint32_t umma_idesc_i8(uint32_t m, uint32_t n) {
 
 __device__ __forceinline__ bool aborted(const int32_t* f) { return *reinterpret_cast<const volatile int32_t*>(f) != 0; }
 
-// Two accumulators of one token: scaled, biased, activated (f32).
-template <int kAct>
+// The exact GELU of two values for a 16-bit result, v max(0, sign v) - |v| Phi(-|v|) with
+//     Phi(-z) = exp(-z^2 / 2) R(z),  R(z) = erfcx(z / sqrt 2) / 2,
+// R as a polynomial in min(z, 5) - 5/2 whose largest relative error is least: degree 8 for
+// bf16 (2^-13.0 of Phi(-z)), degree 10 for f16 (2^-16.8); beyond 5, where R is held, Phi
+// is below 3e-7 and still falls with the exponential.  One SFU operation a value where
+// gelu2_fast takes two: with K = 1024 the epilogue's GELU set the projection's time
+// (17,410 x 4,096: 92 us, the products alone about 45).
+template <typename T>
+__device__ __forceinline__ float2 gelu2_narrow(float2 v) {
+  const float2 z = make_float2(fminf(fabsf(v.x), 5.f), fminf(fabsf(v.y), 5.f));
+  const float2 l = f2_mul(f2_mul(v, f2(-0.72134752044448170f)), v);  // -v^2 / 2 to base 2
+  const float2 u = f2_add(z, f2(-2.5f));
+  float2 r;
+  if constexpr (DT<T>::umma_fmt == 1) {  // bf16
+    r = f2_fma(u, f2(5.790445356979035e-06f), f2(-2.9506778446375392e-05f));
+    r = f2_fma(r, u, f2(5.341164069250226e-05f));
+    r = f2_fma(r, u, f2(-0.00018099445151165128f));
+    r = f2_fma(r, u, f2(0.0010193546768277884f));
+    r = f2_fma(r, u, f2(-0.003963787574321032f));
+    r = f2_fma(r, u, f2(0.013666416518390179f));
+    r = f2_fma(r, u, f2(-0.04555509611964226f));
+    r = f2_fma(r, u, f2(0.14132584631443024f));
+  } else {
+    r = f2_fma(u, f2(2.788294750644127e-07f), f2(-1.515155076958763e-06f));
+    r = f2_fma(r, u, f2(2.5983151772379642e-06f));
+    r = f2_fma(r, u, f2(-8.94710683496669e-06f));
+    r = f2_fma(r, u, f2(6.310718163149431e-05f));
+    r = f2_fma(r, u, f2(-0.0002729224506765604f));
+    r = f2_fma(r, u, f2(0.0010191438486799598f));
+    r = f2_fma(r, u, f2(-0.003814229043200612f));
+    r = f2_fma(r, u, f2(0.013645598664879799f));
+    r = f2_fma(r, u, f2(-0.0456189326941967f));
+    r = f2_fma(r, u, f2(0.141331747174263f));
+  }
+  const float2 h = f2_mul(r, make_float2(-sfu_ex2(l.x), -sfu_ex2(l.y)));
+  return f2_fma(z, h, make_float2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f)));
+}
+
+// Two accumulators: scaled, biased, activated (f32).
+template <typename T, int kAct>
 __device__ __forceinline__ float2 finish2(int a0, int a1, float2 xs, float2 ws, float2 b) {
   const float2 y = f2_fma(f2_mul(make_float2(__int2float_rn(a0), __int2float_rn(a1)), xs), ws, b);
-  if constexpr (kAct == LF_ACT_GELU) return gelu2_fast(y);
+  if constexpr (kAct == LF_ACT_GELU) {
+    if constexpr (sizeof(T) == 2) return gelu2_narrow<T>(y);
+    else return gelu2_fast(y);
+  }
   return y;
+}
+
+// 32 rows x 32 columns of TMEM in the layout of an mma accumulator: lane 4 r + q holds, of
+// the 8-column group j, columns 8 j + 2 q and the next, of rows r and r + 8 (v[4 j .. 4 j + 3])
+// and of rows r + 16 and r + 24 (v[16 + 4 j ..]).  A lane then needs the scales of 8 columns
+// instead of 32: the epilogue's reads of scales from L1 were competing with the MMAs'
+// operand reads.
+__device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr), "r"(taddr + (16u << 16))
+      : "memory");
 }
 
 // ---------------------------------------------------------------------------
@@ -98,13 +160,51 @@ constexpr int kBM = 128, kBN = 256;
 constexpr int kABytes = kBM * kBK;         // 16 KB: this CTA's x rows
 constexpr int kBBytes = (kBN / 2) * kBK;   // 16 KB: this CTA's half of the w rows
 constexpr int kStageBytes = kABytes + kBBytes;
-constexpr int kStages = 6;
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;               // a multiple of 4: kEpiWarps / 4 warps per TMEM lane quadrant
+constexpr int kWarpCols = kBN / (kEpiWarps / 4);  // columns of the tile per epilogue warp
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kOutCols = 32;
-__host__ __device__ constexpr int out_buf(int es) { return 32 * kOutCols * es; }  // one warp's 32 x 32 staging tile
-constexpr int smem_bytes(int es) { return 1024 + kStages * kStageBytes + kEpiWarps * out_buf(es) + 1024; }
-static_assert(smem_bytes(4) <= 232448, "above the 227 KB of shared memory a CTA may use");
+__host__ __device__ constexpr int out_buf(int es) { return 32 * kOutCols * es; }  // one 32 x 32 staging tile
+// ring stages: what the staging tiles leave of the shared memory
+__host__ __device__ constexpr int stages(int es) {
+  const int n = (232448 - 2048 - kEpiWarps * out_buf(es)) / kStageBytes;
+  return n < 6 ? n : 6;
+}
+constexpr int smem_bytes(int es) { return 1024 + stages(es) * kStageBytes + kEpiWarps * out_buf(es) + 1024; }
+static_assert(smem_bytes(4) <= 232448 && smem_bytes(2) <= 232448, "above the 227 KB of shared memory a CTA may use");
+
+// A lane's columns of a 32-column chunk (8 j + 2 fq and the next): their scales and biases,
+// the biases as they lie in memory, 0 past n.  Loaded a chunk ahead of their use.
+template <typename T>
+struct Channels {
+  float2 ws[4];
+  T b[4][2];
+  __device__ __forceinline__ void load(const float* w_scale, const T* bias, int32_t col, int32_t n, bool vec) {
+    if (vec && col + 25 < n) {  // every pair exists and is aligned as a pair
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ws[j] = __ldg(reinterpret_cast<const float2*>(w_scale + col + 8 * j));
+        if (bias != nullptr) {
+          if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint32_t*>(b[j]) = __ldg(reinterpret_cast<const uint32_t*>(bias + col + 8 * j));
+          else
+            *reinterpret_cast<float2*>(b[j]) = __ldg(reinterpret_cast<const float2*>(bias + col + 8 * j));
+        } else {
+          b[j][0] = b[j][1] = DT<T>::from_f(0.f);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int32_t c = col + 8 * j;
+        ws[j] = make_float2(c < n ? __ldg(w_scale + c) : 0.f, c + 1 < n ? __ldg(w_scale + c + 1) : 0.f);
+        b[j][0] = bias != nullptr && c < n ? bias[c] : DT<T>::from_f(0.f);
+        b[j][1] = bias != nullptr && c + 1 < n ? bias[c + 1] : DT<T>::from_f(0.f);
+      }
+    }
+  }
+  __device__ __forceinline__ float2 bias_of(int j) const { return make_float2(DT<T>::to_f(b[j][0]), DT<T>::to_f(b[j][1])); }
+};
 
 template <typename T, int kAct>
 __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_constant__ LinearInt8Params p) {
@@ -115,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const uint32_t rank = uniform(cluster_ctarank());  // 0: the leader, which issues the MMAs
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
-  constexpr int kOutBuf = out_buf(sizeof(T));
+  constexpr int kOutBuf = out_buf(sizeof(T)), kStages = stages(sizeof(T));
 
   const uint32_t s_out0 = base + kStages * kStageBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(gbase + kStages * kStageBytes + kEpiWarps * kOutBuf);
@@ -222,54 +322,70 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
   } else {
     // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
     const int quad = warp & 3;
-    const int half = (warp - 2) >> 2;  // columns [128 half, 128 half + 128) of the tile
-    const uint32_t taddr = tmem + (uint32_t(quad * 32) << 16);
+    const int c0 = ((warp - 2) >> 2) * kWarpCols;  // this warp's columns of the tile
+    const uint32_t taddr = tmem + (uint32_t(quad * 32) << 16) + c0;
     const uint32_t my_out = s_out0 + (warp - 2) * kOutBuf;
     uint8_t* g_out = gbase + (my_out - base);
     const uint32_t acc_empty = mapa_shared(bar(ACC_EMPTY), 0);  // the leader's
     const T* bias = static_cast<const T*>(p.bias);
     T* y = static_cast<T*>(p.y);
-    const int c_begin = half * (kBN / kOutCols / 2), c_end = c_begin + kBN / kOutCols / 2;
+    const int fr = lane >> 2, fq = lane & 3;  // this lane's rows fr + 8 k and columns 8 j + 2 fq of a 32 x 32 block
+    const bool vec = p.vec_ch != 0;
+    // scales and biases come a chunk ahead, the rows' scales a tile ahead
+    Channels<T> next;
+    float xs_next[4];
+    auto col_of = [&](int64_t t) { return int32_t(t % p.n_tiles_n) * kBN + c0 + 2 * fq; };
+    auto row_of = [&](int64_t t) { return (t / p.n_tiles_n) * (2 * kBM) + int64_t(rank) * kBM + quad * 32; };
+    auto load_xs = [&](int64_t t) {
+      const int64_t m = row_of(t) + fr;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) xs_next[k] = m + 8 * k < p.m_rows ? __ldg(p.x_scale + m + 8 * k) : 0.f;
+    };
+    if (pair < p.n_tiles) {
+      next.load(p.w_scale, bias, col_of(pair), p.n, vec);
+      load_xs(pair);
+    }
     int n_it = 0;
     for (int64_t t = pair; t < p.n_tiles; t += n_pairs, ++n_it) {
       const int a = n_it & 1;
-      const int64_t m0 = (t / p.n_tiles_n) * (2 * kBM) + int64_t(rank) * kBM + quad * 32;  // this warp's 32 rows
-      const int32_t n0 = int32_t(t % p.n_tiles_n) * kBN;
-      const float xs = m0 + lane < p.m_rows ? __ldg(p.x_scale + m0 + lane) : 0.f;
+      const int64_t m0 = row_of(t);  // this warp's 32 rows
+      const int32_t n0 = int32_t(t % p.n_tiles_n) * kBN + c0;
+      const bool more = t + n_pairs < p.n_tiles;
+      float xs[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) xs[k] = xs_next[k];
+      if (more) load_xs(t + n_pairs);
       if (!wait(bar(ACC_FULL + a), (n_it >> 1) & 1)) break;
       tc_fence_after();
-      for (int c = c_begin; c < c_end; ++c) {
-        const int col0 = n0 + c * kOutCols;
-        if (col0 >= p.n) break;
-        // the columns' scales and biases: lane i holds column i's, handed out by shuffles
-        const bool in = col0 + lane < p.n;
-        const float ws_l = in ? __ldg(p.w_scale + col0 + lane) : 0.f;
-        const float b_l = in && bias != nullptr ? DT<T>::to_f(bias[col0 + lane]) : 0.f;
-        uint32_t v[32];
-        tmem_ld32(taddr + a * kBN + c * kOutCols, v);
-        float o[32];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 ws = make_float2(__shfl_sync(0xffffffffu, ws_l, 2 * i), __shfl_sync(0xffffffffu, ws_l, 2 * i + 1));
-          const float2 b = make_float2(__shfl_sync(0xffffffffu, b_l, 2 * i), __shfl_sync(0xffffffffu, b_l, 2 * i + 1));
-          const float2 r = finish2<kAct>(int(v[2 * i]), int(v[2 * i + 1]), f2(xs), ws, b);
-          o[2 * i] = r.x;
-          o[2 * i + 1] = r.y;
-        }
+      for (int c = 0; c < kWarpCols; c += kOutCols) {
+        const int32_t col0 = n0 + c;
+        const Channels<T> ch = next;
+        if (c + kOutCols < kWarpCols) next.load(p.w_scale, bias, col0 + kOutCols + 2 * fq, p.n, vec);
+        else if (more) next.load(p.w_scale, bias, col_of(t + n_pairs), p.n, vec);
+        if (col0 >= p.n) continue;
+        uint32_t v[32];
+        tmem_ld_frag32(taddr + a * kBN + c, v);
         // the store that last read this staging tile must be done with it
         if (lane == 0) tma_store_wait_read_all();
         __syncwarp();
-        if constexpr (sizeof(T) == 2) {
+        // rows of 64 bytes: SW64, 16-byte chunk q of row r at q ^ ((r >> 1) & 3); of 128
+        // bytes (f32): SW128, at q ^ (r & 7).  fr + 8 k has fr's swizzle.
+        constexpr int kRowBytes = kOutCols * sizeof(T);
+        const int swz = sizeof(T) == 2 ? (fr >> 1) & 3 : fr & 7;
 #pragma unroll
-          for (int q = 0; q < 4; ++q)  // SW64: 16-byte chunk q of row `lane` at q ^ ((lane >> 1) & 3)
-            *reinterpret_cast<uint4*>(g_out + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) =
-                make_uint4(Pack2<T>::pack(o[8 * q], o[8 * q + 1]), Pack2<T>::pack(o[8 * q + 2], o[8 * q + 3]),
-                           Pack2<T>::pack(o[8 * q + 4], o[8 * q + 5]), Pack2<T>::pack(o[8 * q + 6], o[8 * q + 7]));
-        } else {
+        for (int j = 0; j < 4; ++j) {
+          const float2 cb = ch.bias_of(j);
 #pragma unroll
-          for (int q = 0; q < 8; ++q)  // SW128: chunk q of row `lane` at q ^ (lane & 7)
-            *reinterpret_cast<float4*>(g_out + lane * 128 + ((q ^ (lane & 7)) << 4)) =
-                make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+          for (int k = 0; k < 4; ++k) {
+            const int i = (k >> 1) * 16 + j * 4 + (k & 1) * 2;
+            const float2 r = finish2<T, kAct>(int(v[i]), int(v[i + 1]), f2(xs[k]), ch.ws[j], cb);
+            uint8_t* dst = g_out + (fr + 8 * k) * kRowBytes;
+            if constexpr (sizeof(T) == 2)
+              *reinterpret_cast<uint32_t*>(dst + ((j ^ swz) << 4) + fq * 4) = Pack2<T>::pack(r.x, r.y);
+            else
+              *reinterpret_cast<float2*>(dst + (((2 * j + (fq >> 1)) ^ swz) << 4) + (fq & 1) * 8) = r;
+          }
         }
         if (p.tma_out) {
           fence_proxy_async_smem();
@@ -281,10 +397,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
         } else {  // rows that are not 16-byte aligned: 32 neighbouring columns of a row at a time
           __syncwarp();
           for (int r = 0; r < 32 && m0 + r < p.m_rows; ++r) {
-            const T w = sizeof(T) == 2
-                            ? *reinterpret_cast<const T*>(g_out + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2)
-                            : *reinterpret_cast<const T*>(g_out + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-            if (in) y[(m0 + r) * p.ldy + col0 + lane] = w;
+            const int rs = sizeof(T) == 2 ? (r >> 1) & 3 : r & 7, byte = lane * int(sizeof(T));
+            const T w = *reinterpret_cast<const T*>(g_out + r * kRowBytes + (((byte >> 4) ^ rs) << 4) + (byte & 15));
+            if (col0 + lane < p.n) y[(m0 + r) * p.ldy + col0 + lane] = w;
           }
           __syncwarp();
         }
@@ -457,8 +572,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_int8_split_kernel(con
         a.w += v.w;
       }
       const float xs = __ldg(p.x_scale + row);
-      const float2 lo = finish2<kAct>(a.x, a.y, f2(xs), make_float2(ws[0], ws[1]), make_float2(b[0], b[1]));
-      const float2 hi = finish2<kAct>(a.z, a.w, f2(xs), make_float2(ws[2], ws[3]), make_float2(b[2], b[3]));
+      const float2 lo = finish2<T, kAct>(a.x, a.y, f2(xs), make_float2(ws[0], ws[1]), make_float2(b[0], b[1]));
+      const float2 hi = finish2<T, kAct>(a.z, a.w, f2(xs), make_float2(ws[2], ws[3]), make_float2(b[2], b[3]));
       T* dst = y + row * p.ldy + ch;
       if (whole) {
         if constexpr (sizeof(T) == 2)
@@ -583,6 +698,7 @@ extern "C" int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t 
   p.n = n;
   p.n_kb = (k + kBK - 1) / kBK;
   p.tma_out = aligned16(y) && (ldy * es) % 16 == 0 ? 1 : 0;
+  p.vec_ch = (reinterpret_cast<uintptr_t>(w_scale) & 7u) == 0 && (reinterpret_cast<uintptr_t>(bias) & (2u * es - 1u)) == 0;
   p.status = status;
 
   // 256 x 256 tiles once they fill the CTA pairs; below that 128 channels x nt tokens

@@ -4,9 +4,18 @@ Quantisation is decided exactly, so its integers and scales are compared for equ
 The projection's integer sum is exact; what is left is f32: the sum becomes f32 (2^-24),
 times the token's scale (2^-24), times the channel's scale plus the bias (one FMA,
 2^-24 of the result), then one rounding to the output type (half a step, ``eps / 2``).
-The fused GELU is a fit of erfc within 1.2e-7 (2^-23) with the formula's own f32
-roundings: within |v| 2^-21 of the formula, and it passes its input's error on by at
-most 1.13 (the largest slope of GELU).
+The fused GELU passes its input's error on by at most 1.13 (the largest slope of GELU)
+and adds its own:
+  * f32 results: a fit of erfc within 1.2e-7 (2^-23) with the formula's own f32
+    roundings, within |v| 2^-21 of the formula;
+  * 16-bit results: max(0, v) - |v| Phi(-|v|) with Phi(-z) = exp(-z^2 / 2) R(z), R a
+    polynomial within 2^-13.0 (bf16, degree 8) or 2^-16.8 (f16, degree 10) of its value on
+    [0, 5].  The exponent -z^2 / 2 log2 e, at most 18.1, is rounded twice and the
+    exponential once (18.1 * 2^-23 + 2^-21 < 2^-18): 2^-12.9 or 2^-16.3 of |v| Phi(-|v|) in
+    all.  Past 5 R(5) stands for R(z) and 5 for |v|, which together are off by less than
+    their value there, |v| Phi(-|v|) <= 5 * 2.9e-7: by at most 1.5e-6 * exp((25 - v^2) / 2),
+    and since both err towards each other by under 2% of it (R falls as 1 / z while the
+    factor |v| grows as z): 3e-8.
 """
 
 from __future__ import annotations
@@ -49,7 +58,12 @@ def check_projection(y, q, xs, w, ws, bias, act):
     v = prod + (0.0 if bias is None else bias.double())
     tol = 2.0 ** -24 * (3 * prod.abs() + v.abs())
     if act == ACT_GELU:
-        tol = 1.13 * tol + v.abs() * 2.0 ** -21
+        if y.dtype == torch.float32:
+            own = v.abs() * 2.0 ** -21
+        else:
+            own = v.abs() * torch.special.ndtr(-v.abs()) * 2.0 ** (-12.9 if y.dtype == torch.bfloat16 else -16.3) + \
+                torch.where(v.abs() > 5, 3e-8, 0.0) + v.abs() * 2.0 ** -23
+        tol = 1.13 * tol + own
         v = v * torch.special.ndtr(v)
     fi = torch.finfo(y.dtype)
     tol = tol + (v.abs() + tol) * fi.eps / 2 + fi.smallest_normal * fi.eps  # the last: subnormal results
