@@ -49,8 +49,7 @@ struct alignas(64) LinearInt8Params {
   void* y;
   int64_t ldy;
   int64_t m_rows;
-  int64_t n_tiles;
-  int32_t n, n_tiles_n, n_kb;
+  int32_t n, n_tiles, n_tiles_n, n_kb;
   int32_t tma_out;    // y's base and row stride are 16-byte aligned
   int32_t vec_ch;     // w_scale and bias are aligned for pairs
   int32_t split;      // split kernel: CTAs of the cluster that share a tile's K
@@ -206,6 +205,33 @@ struct Channels {
   __device__ __forceinline__ float2 bias_of(int j) const { return make_float2(DT<T>::to_f(b[j][0]), DT<T>::to_f(b[j][1])); }
 };
 
+// A CTA pair's walk over the output tiles, every n_pairs-th in row-block order, without a
+// division a step.
+struct TileWalk {
+  int32_t t, rb, c;       // tile, row block, column tile
+  int32_t n_tiles, n_cols, step, step_rb, step_c;
+  __device__ __forceinline__ TileWalk(const LinearInt8Params& p, int pair, int n_pairs) {
+    t = pair;
+    n_tiles = p.n_tiles;
+    n_cols = p.n_tiles_n;
+    step = n_pairs;
+    rb = pair / n_cols;
+    c = pair % n_cols;
+    step_rb = n_pairs / n_cols;
+    step_c = n_pairs % n_cols;
+  }
+  __device__ __forceinline__ bool live() const { return t < n_tiles; }
+  __device__ __forceinline__ void next() {
+    t += step;
+    rb += step_rb;
+    c += step_c;
+    if (c >= n_cols) {
+      c -= n_cols;
+      ++rb;
+    }
+  }
+};
+
 template <typename T, int kAct>
 __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_constant__ LinearInt8Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -258,9 +284,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
     // ------------------------------------------------------------ producer (both CTAs)
     int kk = 0;
     bool stop = false;
-    for (int64_t t = pair; t < p.n_tiles && !stop; t += n_pairs) {
-      const int32_t m0 = int32_t(t / p.n_tiles_n) * (2 * kBM) + int32_t(rank) * kBM;
-      const int32_t n0 = int32_t(t % p.n_tiles_n) * kBN + int32_t(rank) * (kBN / 2);
+    for (TileWalk w(p, pair, n_pairs); w.live() && !stop; w.next()) {
+      const int32_t m0 = w.rb * (2 * kBM) + int32_t(rank) * kBM;
+      const int32_t n0 = w.c * kBN + int32_t(rank) * (kBN / 2);
       for (int kb = 0; kb < p.n_kb; ++kb, ++kk) {
         const int s = kk % kStages;
         if (!wait(bar(EMPTY + s), ((kk / kStages) & 1) ^ 1)) {
@@ -289,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
       const uint64_t a_desc = smem_desc(base, 16, 1024, 2), b_desc = smem_desc(base + kABytes, 16, 1024, 2);
       int kk = 0, n_it = 0;
       bool stop = false;
-      for (int64_t t = pair; t < p.n_tiles && !stop; t += n_pairs, ++n_it) {
+      for (TileWalk w(p, pair, n_pairs); w.live() && !stop; w.next(), ++n_it) {
         const int a = n_it & 1;
         if (!wait(bar(ACC_EMPTY + a), ((n_it >> 1) & 1) ^ 1)) break;
         tc_fence_after();
@@ -334,27 +360,27 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
     // scales and biases come a chunk ahead, the rows' scales a tile ahead
     Channels<T> next;
     float xs_next[4];
-    auto col_of = [&](int64_t t) { return int32_t(t % p.n_tiles_n) * kBN + c0 + 2 * fq; };
-    auto row_of = [&](int64_t t) { return (t / p.n_tiles_n) * (2 * kBM) + int64_t(rank) * kBM + quad * 32; };
-    auto load_xs = [&](int64_t t) {
-      const int64_t m = row_of(t) + fr;
+    auto col_of = [&](const TileWalk& w) { return w.c * kBN + c0 + 2 * fq; };
+    auto row_of = [&](const TileWalk& w) { return int64_t(w.rb) * (2 * kBM) + int64_t(rank) * kBM + quad * 32; };
+    auto load_xs = [&](const TileWalk& w) {
+      const int64_t m = row_of(w) + fr;
 #pragma unroll
       for (int k = 0; k < 4; ++k) xs_next[k] = m + 8 * k < p.m_rows ? __ldg(p.x_scale + m + 8 * k) : 0.f;
     };
-    if (pair < p.n_tiles) {
-      next.load(p.w_scale, bias, col_of(pair), p.n, vec);
-      load_xs(pair);
+    TileWalk w(p, pair, n_pairs);
+    if (w.live()) {
+      next.load(p.w_scale, bias, col_of(w), p.n, vec);
+      load_xs(w);
     }
-    int n_it = 0;
-    for (int64_t t = pair; t < p.n_tiles; t += n_pairs, ++n_it) {
+    for (int n_it = 0; w.live(); ++n_it) {
       const int a = n_it & 1;
-      const int64_t m0 = row_of(t);  // this warp's 32 rows
-      const int32_t n0 = int32_t(t % p.n_tiles_n) * kBN + c0;
-      const bool more = t + n_pairs < p.n_tiles;
+      const int64_t m0 = row_of(w);  // this warp's 32 rows
+      const int32_t n0 = w.c * kBN + c0;
       float xs[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) xs[k] = xs_next[k];
-      if (more) load_xs(t + n_pairs);
+      w.next();  // from here on the tile after
+      if (w.live()) load_xs(w);
       if (!wait(bar(ACC_FULL + a), (n_it >> 1) & 1)) break;
       tc_fence_after();
 #pragma unroll
@@ -362,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
         const int32_t col0 = n0 + c;
         const Channels<T> ch = next;
         if (c + kOutCols < kWarpCols) next.load(p.w_scale, bias, col0 + kOutCols + 2 * fq, p.n, vec);
-        else if (more) next.load(p.w_scale, bias, col_of(t + n_pairs), p.n, vec);
+        else if (w.live()) next.load(p.w_scale, bias, col_of(w), p.n, vec);
         if (col0 >= p.n) continue;
         uint32_t v[32];
         tmem_ld_frag32(taddr + a * kBN + c, v);
@@ -406,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(acc_empty + a * 8);  // this warp's TMEM reads of the tile are done
+      if (lane == 0) mbar_arrive_remote(acc_empty + a * 8);  // this warp's TMEM reads of the tile are done
     }
     if (lane == 0) tma_store_wait_all();
   }
@@ -640,8 +666,10 @@ int launch_cluster(const char* what, dim3 grid, int threads, int smem, int clust
 template <typename T, int kAct>
 int launch_batch(LinearInt8Params& p, int dev, cudaStream_t s) {
   p.n_tiles_n = (p.n + kBN - 1) / kBN;
-  p.n_tiles = (p.m_rows + 2 * kBM - 1) / (2 * kBM) * p.n_tiles_n;
-  const int64_t pairs = device_sms(dev) / 2;
+  const int64_t tiles = (p.m_rows + 2 * kBM - 1) / (2 * kBM) * p.n_tiles_n;
+  if (tiles > INT32_MAX / 2) return set_error(LF_ERR_UNSUPPORTED, "lf_linear_int8: %lld output tiles", (long long)tiles);
+  p.n_tiles = int32_t(tiles);
+  const int pairs = device_sms(dev) / 2;
   const unsigned grid = unsigned(2 * (p.n_tiles < pairs ? p.n_tiles : pairs));
   return launch_cluster<linear_int8_kernel<T, kAct>>("launch linear_int8", dim3(grid), kThreads, smem_bytes(sizeof(T)),
                                                      2, dev, s, p);

@@ -67,6 +67,14 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 
+// The same arrival with release only at CTA scope: for a barrier that hands back TMEM
+// columns, whose reads tcgen05.wait::ld and the tcgen05 fences order.  The cluster-scope
+// release also waits for every load and store of the thread still in flight (2,000 clocks
+// and more with loads issued ahead).
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+
 // Allocate / free `ncols` TMEM columns in both CTAs of the pair (the same warp of each).
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols)
