@@ -233,10 +233,7 @@ add_layernorm_kernel(const NormParams p, int full) {
     for (int c = 0; c < NC; ++c) {
       const int col = c * 256 + lane * 8;
       if (full || col < H) {
-        uint2 w;
-        w.x = rq.q4(v[c][0], v[c][1], v[c][2], v[c][3]);
-        w.y = rq.q4(v[c][4], v[c][5], v[c][6], v[c][7]);
-        *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) = w;
+        *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) = rq.q8(v[c]);
       }
     }
   }

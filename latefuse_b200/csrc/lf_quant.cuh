@@ -22,6 +22,7 @@ struct RowQuant {
   float top;    // the row's largest magnitude, times pre
   float inv;    // 127 / top; 0 for a row of zeros or a row that is not finite
   float scale;
+  float inv_raw;  // 127 / the row's largest magnitude, for rows well inside f32's range; else 0
   // top_bits: the largest mag_bits of the row
   __device__ __forceinline__ explicit RowQuant(uint32_t top_bits) {
     const float t = __uint_as_float(top_bits);
@@ -30,6 +31,7 @@ struct RowQuant {
     top = t * pre;
     inv = (top_bits == 0u || !finite) ? 0.f : __fdiv_rn(127.f, top);
     scale = finite ? __fdiv_rn(t, 127.f) : __uint_as_float(0x7fc00000u);
+    inv_raw = t > 0x1p-100f && t < 0x1p120f ? __fdiv_rn(127.f, t) : 0.f;  // NaN and infinity: 0
   }
   // v next to r + 1/2 or r - 1/2 (r = rint(v)), or not a number: 127 x - r top is exact
   // in two floats (the product 127 x splits exactly, and its head minus r top is a
@@ -54,6 +56,25 @@ struct RowQuant {
   // q of four values, the first in the low byte
   __device__ __forceinline__ uint32_t q4(float a, float b, float c, float d) const {
     return __byte_perm(__byte_perm(q(a), q(b), 0x0040), __byte_perm(q(c), q(d), 0x0040), 0x5410);
+  }
+  // q of eight values, the first in the low byte of x.  Pairs at a time, and one test for all
+  // eight: a value next to a half, or a row at the ends of f32's range, takes q4.
+  __device__ __forceinline__ uint2 q8(const float (&x)[8]) const {
+    uint32_t m[8];
+    float far = inv_raw == 0.f ? 1.f : 0.f;  // the largest distance to the nearest integer
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = f2_mul(make_float2(x[2 * i], x[2 * i + 1]), f2(inv_raw));
+      const float2 w = f2_add(v, f2(kMagic));
+      const float2 d = f2_add(v, f2_fma(w, f2(-1.f), f2(kMagic)));  // v - (w - magic), both exact
+      far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+      m[2 * i] = __float_as_uint(w.x);
+      m[2 * i + 1] = __float_as_uint(w.y);
+    }
+    if (far >= 0.499969482421875f) return make_uint2(q4(x[0], x[1], x[2], x[3]), q4(x[4], x[5], x[6], x[7]));
+    return make_uint2(
+        __byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410),
+        __byte_perm(__byte_perm(m[4], m[5], 0x0040), __byte_perm(m[6], m[7], 0x0040), 0x5410));
   }
 };
 

@@ -17,7 +17,6 @@ namespace lf {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunks = 4;  // 8 elements each, per lane
 
 struct QuantParams {
   const void* x;
@@ -28,62 +27,86 @@ struct QuantParams {
   float* scale;
 };
 
-// This lane's 8 elements of chunk c: neighbours (VEC), or 32 apart.
+// A lane's 8 elements of a 256-element chunk: neighbours (VEC), kept as they lie in memory
+// until they are rounded, or 32 apart.  Elements past the row read as 0.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int32_t base, int lane, int32_t cols, float (&v)[8]) {
-  if constexpr (VEC) {
-    const int32_t col = base + lane * 8;
-    if (col < cols) {
-      if constexpr (sizeof(T) == 2) {
-        const uint4 w = *reinterpret_cast<const uint4*>(row + col);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+struct Chunk {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* row, int32_t base, int lane, int32_t cols) {
+    if constexpr (VEC) {
+      const int32_t col = base + lane * 8;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = Pack2<T>::unpack(u[i]);
-          v[2 * i] = f.x;
-          v[2 * i + 1] = f.y;
-        }
-      } else {
-        const float4 a = *reinterpret_cast<const float4*>(row + col), b = *reinterpret_cast<const float4*>(row + col + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-      }
+      for (int i = 0; i < int(sizeof(T)) / 2; ++i)
+        w[i] = col < cols ? __ldg(reinterpret_cast<const uint4*>(row + col) + i) : make_uint4(0u, 0u, 0u, 0u);
     } else {
+      T e[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    }
-  } else {
+      for (int i = 0; i < 8; ++i) {
+        const int32_t col = base + i * 32 + lane;
+        e[i] = col < cols ? row[col] : DT<T>::from_f(0.f);
+      }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int32_t col = base + i * 32 + lane;
-      v[i] = col < cols ? DT<T>::to_f(row[col]) : 0.f;
+      for (int i = 0; i < int(sizeof(T)) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(e)[i];
     }
   }
-}
-
-template <bool VEC>
-__device__ __forceinline__ void store8(int8_t* row, int32_t base, int lane, int32_t cols, const RowQuant& rq,
-                                       const float (&v)[8]) {
-  if constexpr (VEC) {
-    const int32_t col = base + lane * 8;
-    if (col < cols) {
-      uint2 w;
-      w.x = rq.q4(v[0], v[1], v[2], v[3]);
-      w.y = rq.q4(v[4], v[5], v[6], v[7]);
-      *reinterpret_cast<uint2*>(row + col) = w;
-    }
-  } else {
+  // the largest magnitude as an integer that orders like it: two 16-bit halves, or 32 bits
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t t = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int32_t col = base + i * 32 + lane;
-      if (col < cols) row[col] = int8_t(rq.q(v[i]));
+    for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
+      const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 2) t = __vmaxu2(t, u[k] & 0x7fff7fffu);
+        else t = max(t, u[k] & 0x7fffffffu);
+      }
+    }
+    return t;
+  }
+  __device__ __forceinline__ void store(int8_t* row, int32_t base, int lane, int32_t cols, const RowQuant& rq) const {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
+      const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 2) {
+          const float2 f = Pack2<T>::unpack(u[k]);
+          v[2 * k] = f.x;
+          v[2 * k + 1] = f.y;
+        } else {
+          v[4 * i + k] = __uint_as_float(u[k]);
+        }
+      }
+    }
+    if constexpr (VEC) {
+      const int32_t col = base + lane * 8;
+      if (col < cols) *reinterpret_cast<uint2*>(row + col) = rq.q8(v);
+    } else {
+      const uint2 q = rq.q8(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int32_t col = base + i * 32 + lane;
+        if (col < cols) row[col] = int8_t((i < 4 ? q.x >> (8 * i) : q.y >> (8 * (i - 4))) & 0xffu);
+      }
     }
   }
+};
+
+// The f32 bits of a magnitude given by its type's bits.
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(uint32_t t) {
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t h = uint16_t(t);
+    return __float_as_uint(DT<T>::to_f(*reinterpret_cast<const T*>(&h)));
+  }
+  return t;
 }
 
-// WPR warps per row; rows of at most WPR * 1024 elements, or any length when LONG (WPR = 8).
-template <typename T, int WPR, bool VEC, bool LONG>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantParams p) {
+// WPR warps per row, each with kChunks chunks of 256 elements in registers; LONG: rows of
+// any length, the rest read twice.
+template <typename T, int WPR, int kChunks, bool VEC, bool LONG>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && VEC && !LONG ? 6 : 1) quantize_rows_kernel(const QuantParams p) {
   __shared__ uint32_t s_top[kThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = warp % WPR;
@@ -93,24 +116,22 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantPara
   pdl_launch_dependents();
   const T* x = static_cast<const T*>(p.x) + (live ? row : 0) * p.ldx;
   int8_t* q = p.q + (live ? row : 0) * p.ldq;
-  float v[kChunks][8];
+  Chunk<T, VEC> v[kChunks];
   uint32_t top = 0;
   if (live) {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) load8<T, VEC>(x, (c * WPR + sub) * 256, lane, p.cols, v[c]);
+    for (int c = 0; c < kChunks; ++c) v[c].load(x, (c * WPR + sub) * 256, lane, p.cols);
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, mag_bits(v[c][i]));
+    for (int c = 0; c < kChunks; ++c) top = sizeof(T) == 2 ? __vmaxu2(top, v[c].top()) : max(top, v[c].top());
     if constexpr (LONG) {
       for (int32_t base = (kChunks * WPR + sub) * 256; base < p.cols; base += WPR * 256) {
-        float w[8];
-        load8<T, VEC>(x, base, lane, p.cols, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, mag_bits(w[i]));
+        Chunk<T, VEC> w;
+        w.load(x, base, lane, p.cols);
+        top = sizeof(T) == 2 ? __vmaxu2(top, w.top()) : max(top, w.top());
       }
     }
   }
+  if constexpr (sizeof(T) == 2) top = max(top >> 16, top & 0xffffu);
   top = __reduce_max_sync(0xffffffffu, top);
   if constexpr (WPR > 1) {
     if (lane == 0) s_top[warp] = top;
@@ -119,35 +140,48 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantPara
     for (int i = 0; i < WPR; ++i) top = max(top, s_top[warp - sub + i]);
   }
   if (!live) return;
-  const RowQuant rq(top);
+  const RowQuant rq(top_bits<T>(top));
   if (sub == 0 && lane == 0) p.scale[row] = rq.scale;
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) store8<VEC>(q, (c * WPR + sub) * 256, lane, p.cols, rq, v[c]);
+  for (int c = 0; c < kChunks; ++c) v[c].store(q, (c * WPR + sub) * 256, lane, p.cols, rq);
   if constexpr (LONG) {
     for (int32_t base = (kChunks * WPR + sub) * 256; base < p.cols; base += WPR * 256) {
-      float w[8];
-      load8<T, VEC>(x, base, lane, p.cols, w);
-      store8<VEC>(q, base, lane, p.cols, rq, w);
+      Chunk<T, VEC> w;
+      w.load(x, base, lane, p.cols);
+      w.store(q, base, lane, p.cols, rq);
     }
   }
 }
 
-template <typename T>
-int launch_quantize(const QuantParams& p, bool vec, cudaStream_t s) {
-  const int wpr = p.cols <= 1024 ? 1 : p.cols <= 2048 ? 2 : p.cols <= 4096 ? 4 : 8;
-  const int rows = kThreads / 32 / wpr;
+template <typename T, int WPR, int kChunks, bool LONG>
+int launch_rows(const QuantParams& p, bool vec, cudaStream_t s) {
+  constexpr int rows = kThreads / 32 / WPR;
   const int64_t blocks = (p.n_rows + rows - 1) / rows;
   if (blocks > INT32_MAX) return set_error(LF_ERR_UNSUPPORTED, "lf_quantize_rows: %lld rows", (long long)p.n_rows);
-  const bool lng = p.cols > 8192;
-  auto kern = wpr == 1   ? (vec ? quantize_rows_kernel<T, 1, true, false> : quantize_rows_kernel<T, 1, false, false>)
-              : wpr == 2 ? (vec ? quantize_rows_kernel<T, 2, true, false> : quantize_rows_kernel<T, 2, false, false>)
-              : wpr == 4 ? (vec ? quantize_rows_kernel<T, 4, true, false> : quantize_rows_kernel<T, 4, false, false>)
-              : lng      ? (vec ? quantize_rows_kernel<T, 8, true, true> : quantize_rows_kernel<T, 8, false, true>)
-                         : (vec ? quantize_rows_kernel<T, 8, true, false> : quantize_rows_kernel<T, 8, false, false>);
-  const cudaError_t e = launch_pdl(kern, dim3(unsigned(blocks)), dim3(kThreads), 0, s, p);
+  const cudaError_t e = launch_pdl(vec ? quantize_rows_kernel<T, WPR, kChunks, true, LONG>
+                                       : quantize_rows_kernel<T, WPR, kChunks, false, LONG>,
+                                   dim3(unsigned(blocks)), dim3(kThreads), 0, s, p);
   if (e != cudaSuccess) return cuda_error(e, "launch quantize_rows");
   count_launch();
   return LF_OK;
+}
+
+// A row's 256-element chunks over 1, 2, 4 or 8 warps, three or four a warp (so that a row of
+// 2,560 leaves 2 of 12 empty, not 6 of 16).
+template <typename T>
+int launch_quantize(const QuantParams& p, bool vec, cudaStream_t s) {
+  const int n = (p.cols + 255) / 256;
+  if (n <= 1) return launch_rows<T, 1, 1, false>(p, vec, s);
+  if (n <= 2) return launch_rows<T, 1, 2, false>(p, vec, s);
+  if (n <= 3) return launch_rows<T, 1, 3, false>(p, vec, s);
+  if (n <= 4) return launch_rows<T, 1, 4, false>(p, vec, s);
+  if (n <= 6) return launch_rows<T, 2, 3, false>(p, vec, s);
+  if (n <= 8) return launch_rows<T, 2, 4, false>(p, vec, s);
+  if (n <= 12) return launch_rows<T, 4, 3, false>(p, vec, s);
+  if (n <= 16) return launch_rows<T, 4, 4, false>(p, vec, s);
+  if (n <= 24) return launch_rows<T, 8, 3, false>(p, vec, s);
+  if (n <= 32) return launch_rows<T, 8, 4, false>(p, vec, s);
+  return launch_rows<T, 8, 4, true>(p, vec, s);
 }
 
 }  // namespace
