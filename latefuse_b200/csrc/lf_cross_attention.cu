@@ -124,7 +124,9 @@ __device__ __forceinline__ float ld_dsmem_f32(uint32_t addr) {
   return v;
 }
 
-__host__ __device__ constexpr int decode_stages(int kd) { return kd == 64 ? 4 : 3; }
+// three stages a warp: with four, three CTAs of 64 columns fit an SM instead of four (64
+// sequences of 4,096 keys, 16 heads: 185 us against 159)
+__host__ __device__ constexpr int decode_stages(int) { return 3; }
 __host__ __device__ constexpr int decode_pitch(int kd) { return kd + 8; }  // f32 columns of a partial output row
 // [Q tile][ring, reused for the warps' partial outputs][warps' m and l][the CTA's m and l]
 __host__ __device__ constexpr int decode_q_bytes(int kd, int mt) { return 16 * mt * kd * 2; }
@@ -186,26 +188,54 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const _
   const int n_tiles = (rec.nk + kKeyTile - 1) / kKeyTile;
   const int t0 = int(int64_t(n_tiles) * rank / S), t1 = int(int64_t(n_tiles) * (rank + 1) / S);
   const int n_my = t1 - t0 > warp ? (t1 - t0 - warp + kDecodeWarps - 1) / kDecodeWarps : 0;
-  const T* kg = static_cast<const T*>(p.k) + int64_t(kvh) * p.d;
-  const T* vg = static_cast<const T*>(p.v) + int64_t(kvh) * p.d;
-  auto issue = [&](int i) {
-    if (i < n_my) {
-      const int key0 = (t0 + warp + kDecodeWarps * i) * kKeyTile;
-      const uint32_t st = ring + (i % kSt) * (2 * kTile);
+  // Addresses are kept as what changes from one copy to the next: a lane copies chunk
+  // lane % kCh of rows kRowsJ apart, whose swizzled places repeat every kPeriod copies.
+  constexpr int kRowsJ = 32 / kCh, kPeriod = 8 / kRowsJ, kCopies = kKeyTile / kRowsJ;
+  const int my_row = lane / kCh, my_ch = lane % kCh;
+  const bool my_col = my_ch < nch;  // a chunk past the head is never copied: zeros, written once
+  uint32_t cp_off[kPeriod];
 #pragma unroll
-      for (int j = 0; j < kKeyTile * kCh / 32; ++j) {
-        const int r = (j * 32 + lane) / kCh, c = (j * 32 + lane) % kCh;
-        const bool in = key0 + r < rec.nk && c < nch;  // rows past the end and columns past the head are zeros
-        const int64_t row = rec.k0 + (in ? key0 + r : 0);
-        const int col = (in ? c : 0) * 8;
-        cp_async16(at(st, r, c), kg + row * p.ldk + col, in ? 16u : 0u);
-        cp_async16(at(st + kTile, r, c), vg + row * p.ldv + col, in ? 16u : 0u);
+  for (int x = 0; x < kPeriod; ++x) cp_off[x] = at(0, x * kRowsJ + my_row, my_ch);
+  const T* kp = static_cast<const T*>(p.k) + (int64_t(rec.k0) + (t0 + warp) * kKeyTile + my_row) * p.ldk + int64_t(kvh) * p.d + my_ch * 8;
+  const T* vp = static_cast<const T*>(p.v) + (int64_t(rec.k0) + (t0 + warp) * kKeyTile + my_row) * p.ldv + int64_t(kvh) * p.d + my_ch * 8;
+  if (nch < kCh) {
+    for (int i = lane; i < kSt * 2 * kKeyTile * (kCh - nch); i += 32) {
+      const int r = i / (kCh - nch), c = nch + i % (kCh - nch);  // the stages' tiles lie one after the other
+      *reinterpret_cast<uint4*>(smem + (at(ring, r, c) - sQ)) = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  int issued = 0;
+  uint32_t st_issue = ring;
+  auto issue = [&]() {  // the next tile's copies into the next stage
+    if (issued < n_my) {
+      const int left = rec.nk - (t0 + warp + kDecodeWarps * issued) * kKeyTile;
+      if (my_col) {
+        if (left >= kKeyTile) {
+#pragma unroll
+          for (int j = 0; j < kCopies; ++j) {
+            const uint32_t dst = st_issue + cp_off[j % kPeriod] + (j / kPeriod) * (8 * kD * 2);
+            cp_async16(dst, kp + j * kRowsJ * p.ldk, 16u);
+            cp_async16(dst + kTile, vp + j * kRowsJ * p.ldv, 16u);
+          }
+        } else {  // rows past the end become zeros
+#pragma unroll
+          for (int j = 0; j < kCopies; ++j) {
+            const uint32_t dst = st_issue + cp_off[j % kPeriod] + (j / kPeriod) * (8 * kD * 2);
+            const bool in = j * kRowsJ + my_row < left;
+            cp_async16(dst, in ? kp + j * kRowsJ * p.ldk : static_cast<const T*>(p.k), in ? 16u : 0u);
+            cp_async16(dst + kTile, in ? vp + j * kRowsJ * p.ldv : static_cast<const T*>(p.v), in ? 16u : 0u);
+          }
+        }
+        kp += kDecodeWarps * kKeyTile * p.ldk;
+        vp += kDecodeWarps * kKeyTile * p.ldv;
       }
+      ++issued;
+      st_issue = st_issue == ring + (kSt - 1) * (2 * kTile) ? ring : st_issue + 2 * kTile;
     }
     cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < kSt - 1; ++i) issue(i);
+  for (int i = 0; i < kSt - 1; ++i) issue();
   cp_async_wait<kSt - 1>();  // Q has landed
   __syncthreads();
 
@@ -222,18 +252,24 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const _
 #pragma unroll
   for (int m = 0; m < MT; ++m) mrow[m][0] = mrow[m][1] = -INFINITY, lrow[m][0] = lrow[m][1] = 0.f;
 
-  const int k_row = (lane & 7) + (lane >> 4) * 8, k_chunk = (lane >> 3) & 1;  // K: {keys 0-7, 8-15} x {8 columns, next 8}
-  const int v_row = (lane & 7) + ((lane >> 3) & 1) * 8, v_chunk = lane >> 4;
+  // ldmatrix rows: K {keys 0-7, 8-15} x {8 columns, next 8}, V the other way round; chunk
+  // 2 ks + x of 16-column step ks repeats its swizzle every four steps (128 bytes)
+  uint32_t k_off[4], v_off[4];
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    k_off[ks] = at(0, (lane & 7) + (lane >> 4) * 8, ks * 2 + ((lane >> 3) & 1));
+    v_off[ks] = at(0, (lane & 7) + ((lane >> 3) & 1) * 8, ks * 2 + (lane >> 4)) + kTile;
+  }
+  uint32_t st = ring;
   for (int i = 0; i < n_my; ++i) {
     cp_async_wait<kSt - 2>();
     __syncwarp();
-    const uint32_t sK = ring + (i % kSt) * (2 * kTile), sV = sK + kTile;
-    float s[MT][2][4] = {};
+    float s[MT][2][4] = {}, s1[MT][2][4] = {};  // even and odd steps: half as long a chain of products
 #pragma unroll
     for (int ks = 0; ks < kD / 16; ++ks) {
       if (ks >= nks) break;
       uint32_t kf[4];
-      ldsm4(kf, at(sK, k_row, ks * 2 + k_chunk));
+      ldsm4(kf, st + k_off[ks & 3] + (ks >> 2) * 128);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         uint32_t a[4];
@@ -243,10 +279,16 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const _
         } else {
           ldsm4(a, at(sQ, m * 16 + q_row, ks * 2 + q_chunk));
         }
-        mma16816<T>(s[m][0], a, kf[0], kf[1]);
-        mma16816<T>(s[m][1], a, kf[2], kf[3]);
+        mma16816<T>(ks & 1 ? s1[m][0] : s[m][0], a, kf[0], kf[1]);
+        mma16816<T>(ks & 1 ? s1[m][1] : s[m][1], a, kf[2], kf[3]);
       }
     }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[m][n][x] += s1[m][n][x];
     const int left = rec.nk - (t0 + warp + kDecodeWarps * i) * kKeyTile;  // keys of the sequence from this tile on
     if (left < kKeyTile) {
 #pragma unroll
@@ -262,48 +304,47 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const _
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // rows lane / 4 and lane / 4 + 8
+        if (m * 16 + h * 8 >= rows) {  // eight rows without a query
+          pf[m][h] = pf[m][2 + h] = 0u;
+          continue;
+        }
         float mx = fmaxf(fmaxf(s[m][0][2 * h], s[m][0][2 * h + 1]), fmaxf(s[m][1][2 * h], s[m][1][2 * h + 1]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float m_new = fmaxf(mrow[m][h], mx * p.scale_log2);
         const float m_use = m_new == -INFINITY ? 0.f : m_new;  // every score so far is -inf: p = 0
-        const float alpha = sfu_ex2(mrow[m][h] - m_use);
-        mrow[m][h] = m_new;
-        float sum = 0.f;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float e = sfu_ex2(fmaf(s[m][n][2 * h + x], p.scale_log2, -m_use));
-            s[m][n][2 * h + x] = e;
-            sum += e;
-          }
-        lrow[m][h] = lrow[m][h] * alpha + sum;
-        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+        if (__any_sync(0xffffffffu, m_new != mrow[m][h])) {
+          const float alpha = sfu_ex2(mrow[m][h] - m_use);
+          mrow[m][h] = m_new;
+          lrow[m][h] *= alpha;
 #pragma unroll
           for (int n = 0; n < kD / 8; ++n) {
             o[m][n][2 * h] *= alpha;
             o[m][n][2 * h + 1] *= alpha;
           }
         }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float e0 = sfu_ex2(fmaf(s[m][n][2 * h], p.scale_log2, -m_use));
+          const float e1 = sfu_ex2(fmaf(s[m][n][2 * h + 1], p.scale_log2, -m_use));
+          lrow[m][h] += e0 + e1;
+          pf[m][2 * n + h] = Pack2<T>::pack(e0, e1);
+        }
       }
-      pf[m][0] = Pack2<T>::pack(s[m][0][0], s[m][0][1]);
-      pf[m][1] = Pack2<T>::pack(s[m][0][2], s[m][0][3]);
-      pf[m][2] = Pack2<T>::pack(s[m][1][0], s[m][1][1]);
-      pf[m][3] = Pack2<T>::pack(s[m][1][2], s[m][1][3]);
     }
 #pragma unroll
     for (int ks = 0; ks < kD / 16; ++ks) {
       if (ks >= nks) break;
       uint32_t vf[4];
-      ldsm4_t(vf, at(sV, v_row, ks * 2 + v_chunk));
+      ldsm4_t(vf, st + v_off[ks & 3] + (ks >> 2) * 128);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         mma16816<T>(o[m][2 * ks], pf[m], vf[0], vf[1]);
         mma16816<T>(o[m][2 * ks + 1], pf[m], vf[2], vf[3]);
       }
     }
-    issue(i + kSt - 1);  // into the slot of tile i - 1, which every lane has left
+    issue();  // into the stage of tile i - 1, which every lane has left
+    st = st == ring + (kSt - 1) * (2 * kTile) ? ring : st + 2 * kTile;
   }
   cp_async_wait<0>();
   __syncthreads();  // every warp is done with the ring
@@ -999,9 +1040,13 @@ extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q,
     const int64_t blocks = (rows + 16 * mt - 1) / (16 * mt);
     const int64_t units = int64_t(n_items) * n_kv_heads;
     if (units * 8 > INT32_MAX || blocks > 65535) return set_error(LF_ERR_UNSUPPORTED, "%s: too many records", fn);
+    // The keys are split only as far as it takes for the longest sequence not to outlast the
+    // others: a CTA costs 3 us beside its keys (64 sequences of 4,096 keys, 16 heads of 64, with four stages:
+    // 185 us whole, 172 in halves, 188 in quarters, 235 in eighths; 1 of 8,192: 92, 52, 30, 21).
+    const int64_t slots = int64_t(sms) * (head_dim <= 64 ? 4 : 2);  // CTAs that fit the GPU
+    const int64_t mean = units * blocks * (n_kv / n_items) / slots;  // keys for each of them
     p.split = 1;
-    while (p.split < 8 && max_kv / (2 * p.split) >= 64 && (units * blocks * p.split < 2 * sms || max_kv / p.split > 1024))
-      p.split *= 2;
+    while (p.split < 8 && max_kv / (2 * p.split) >= 64 && max_kv / p.split > mean + mean / 4) p.split *= 2;
     const unsigned rb = unsigned(blocks);
     if (head_dim <= 64) {
       if (mt == 1) return bf ? launch_decode<__nv_bfloat16, 64, 1>(p, rb, dev, s) : launch_decode<__half, 64, 1>(p, rb, dev, s);
