@@ -17,8 +17,9 @@
 //
 // cross_decode_kernel, for few query rows (single tokens), where reading K and V once at
 // HBM speed is the bound.  One CTA per (sequence, key head, block of query rows, share of
-// the keys): its rows are all of the group's heads and the sequence's queries (16 per
-// mma.sync tile), so K and V are read once for all of them.  Four warps take 16-key tiles
+// the keys): its rows are the group's heads and the sequence's queries, 16 of them (one
+// mma.sync tile; two tiles a CTA took 166 registers and measured slower than two CTAs side
+// by side, 59 against 46 us), so K and V are read once for all of them.  Four warps take 16-key tiles
 // in turn, each with its own ring of asynchronous copies and its own running maximum and
 // sum, merged at the end through shared memory.  The keys of a sequence are split over a
 // cluster of up to 8 CTAs when there are too few sequences and heads to fill the GPU, or
@@ -57,6 +58,7 @@ struct alignas(64) CrossParams {
   const int4* items;   // two per record: {q_start, q_len, kv_start, kv_len}, {q_tile, 0, 0, 0}
   int32_t n_items;
   int32_t max_q;       // decode: no record's q_len is above it
+  int32_t row_blocks;  // decode: CTAs that share a key head's query rows
   int32_t split;       // decode: CTAs of the cluster that share a sequence's keys
   float scale_log2;    // scale * log2(e)
   void* out;
@@ -82,6 +84,7 @@ __device__ __forceinline__ Rec read_rec(const CrossParams& p, int i) {
 // few query rows
 // ---------------------------------------------------------------------------
 constexpr int kDecodeWarps = 4;
+constexpr int kDecodeRows = 16;  // query rows of a CTA: one mma.sync tile
 constexpr int kKeyTile = 16;  // keys a warp takes at a time
 
 template <typename T>
@@ -129,30 +132,30 @@ __device__ __forceinline__ float ld_dsmem_f32(uint32_t addr) {
 __host__ __device__ constexpr int decode_stages(int) { return 3; }
 __host__ __device__ constexpr int decode_pitch(int kd) { return kd + 8; }  // f32 columns of a partial output row
 // [Q tile][ring, reused for the warps' partial outputs][warps' m and l][the CTA's m and l]
-__host__ __device__ constexpr int decode_q_bytes(int kd, int mt) { return 16 * mt * kd * 2; }
+__host__ __device__ constexpr int decode_q_bytes(int kd) { return kDecodeRows * kd * 2; }
 __host__ __device__ constexpr int decode_ring_bytes(int kd) {
   return kDecodeWarps * decode_stages(kd) * 2 * kKeyTile * kd * 2;
 }
-__host__ __device__ constexpr int decode_smem(int kd, int mt) {
-  return decode_q_bytes(kd, mt) + decode_ring_bytes(kd) + (kDecodeWarps + 1) * 16 * mt * 2 * 4;
+__host__ __device__ constexpr int decode_smem(int kd) {
+  return decode_q_bytes(kd) + decode_ring_bytes(kd) + (kDecodeWarps + 1) * kDecodeRows * 2 * 4;
 }
-static_assert(kDecodeWarps * 32 * decode_pitch(64) * 4 <= decode_ring_bytes(64), "partial outputs reuse the ring");
-static_assert(kDecodeWarps * 32 * decode_pitch(128) * 4 <= decode_ring_bytes(128), "partial outputs reuse the ring");
+static_assert(kDecodeWarps * kDecodeRows * decode_pitch(64) * 4 <= decode_ring_bytes(64), "partial outputs reuse the ring");
+static_assert(kDecodeWarps * kDecodeRows * decode_pitch(128) * 4 <= decode_ring_bytes(128), "partial outputs reuse the ring");
 
-template <typename T, int kD, int MT>
+template <typename T, int kD>
 __global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const __grid_constant__ CrossParams p) {
   constexpr int kSt = decode_stages(kD), kTile = kKeyTile * kD * 2, kCh = kD / 8, kPitch = decode_pitch(kD);
-  constexpr int kRowsMax = 16 * MT;
-  constexpr bool kQRegs = MT * kD <= 128;  // Q fragments stay in registers (else re-read from shared memory)
+  constexpr int kRowsMax = kDecodeRows;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int S = p.split;
   const int rank = S > 1 ? int(cluster_ctarank()) : 0;
-  const int unit = int(blockIdx.x) / S;
+  // a unit's row blocks lie side by side: they read the same keys at the same time
+  const int unit = int(blockIdx.x) / (S * p.row_blocks), row_block = int(blockIdx.x) / S % p.row_blocks;
   const int kvh = unit % p.n_kv_heads;
   const uint32_t sQ = smem_u32(smem);
-  const uint32_t ring = sQ + decode_q_bytes(kD, MT) + warp * (kSt * 2 * kTile);
-  float* s_part = reinterpret_cast<float*>(smem + decode_q_bytes(kD, MT));
+  const uint32_t ring = sQ + decode_q_bytes(kD) + warp * (kSt * 2 * kTile);
+  float* s_part = reinterpret_cast<float*>(smem + decode_q_bytes(kD));
   float* s_ml = s_part + decode_ring_bytes(kD) / 4;  // [warp][row]{m, l}, then the CTA's
 
   pdl_wait();
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const _
     if (tid == 0) set_status(p.status, LF_STATUS_BAD_SEGMENT);
     return;
   }
-  const int row0 = int(blockIdx.y) * kRowsMax;
+  const int row0 = row_block * kRowsMax;
   const int rows = min(kRowsMax, rec.nq * p.group - row0);  // row r: query (row0 + r) / group, head (row0 + r) % group
   if (rows <= 0) return;
   const int nch = p.d / 8;              // 16-byte chunks of a head's row
@@ -239,18 +242,11 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const _
   cp_async_wait<kSt - 1>();  // Q has landed
   __syncthreads();
 
-  uint32_t qf[kQRegs ? MT : 1][kQRegs ? kD / 16 : 1][4];
-  const int q_row = (lane & 7) + ((lane >> 3) & 1) * 8, q_chunk = lane >> 4;  // this lane's ldmatrix row of a Q tile
-  if constexpr (kQRegs) {
+  uint32_t qf[kD / 16][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int ks = 0; ks < kD / 16; ++ks) ldsm4(qf[m][ks], at(sQ, m * 16 + q_row, ks * 2 + q_chunk));
-  }
-  float o[MT][kD / 8][4] = {};
-  float mrow[MT][2], lrow[MT][2];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) mrow[m][0] = mrow[m][1] = -INFINITY, lrow[m][0] = lrow[m][1] = 0.f;
+  for (int ks = 0; ks < kD / 16; ++ks) ldsm4(qf[ks], at(sQ, (lane & 7) + ((lane >> 3) & 1) * 8, ks * 2 + (lane >> 4)));
+  float o[kD / 8][4] = {};
+  float mrow[2] = {-INFINITY, -INFINITY}, lrow[2] = {0.f, 0.f};
 
   // ldmatrix rows: K {keys 0-7, 8-15} x {8 columns, next 8}, V the other way round; chunk
   // 2 ks + x of 16-column step ks repeats its swizzle every four steps (128 bytes)
@@ -264,72 +260,51 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const _
   for (int i = 0; i < n_my; ++i) {
     cp_async_wait<kSt - 2>();
     __syncwarp();
-    float s[MT][2][4] = {}, s1[MT][2][4] = {};  // even and odd steps: half as long a chain of products
+    float s[2][4] = {}, s1[2][4] = {};  // even and odd steps: half as long a chain of products
 #pragma unroll
     for (int ks = 0; ks < kD / 16; ++ks) {
       if (ks >= nks) break;
       uint32_t kf[4];
       ldsm4(kf, st + k_off[ks & 3] + (ks >> 2) * 128);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        uint32_t a[4];
-        if constexpr (kQRegs) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) a[x] = qf[m][ks][x];
-        } else {
-          ldsm4(a, at(sQ, m * 16 + q_row, ks * 2 + q_chunk));
-        }
-        mma16816<T>(ks & 1 ? s1[m][0] : s[m][0], a, kf[0], kf[1]);
-        mma16816<T>(ks & 1 ? s1[m][1] : s[m][1], a, kf[2], kf[3]);
-      }
+      mma16816<T>(ks & 1 ? s1[0] : s[0], qf[ks], kf[0], kf[1]);
+      mma16816<T>(ks & 1 ? s1[1] : s[1], qf[ks], kf[2], kf[3]);
     }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) s[m][n][x] += s1[m][n][x];
     const int left = rec.nk - (t0 + warp + kDecodeWarps * i) * kKeyTile;  // keys of the sequence from this tile on
-    if (left < kKeyTile) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+      for (int x = 0; x < 4; ++x) {
+        s[n][x] += s1[n][x];
+        if (n * 8 + (lane & 3) * 2 + (x & 1) >= left) s[n][x] = -INFINITY;
+      }
+    uint32_t pf[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (n * 8 + (lane & 3) * 2 + (x & 1) >= left) s[m][n][x] = -INFINITY;
-    }
-    uint32_t pf[MT][4];
+    for (int h = 0; h < 2; ++h) {  // rows lane / 4 and lane / 4 + 8
+      if (h * 8 >= rows) {  // eight rows without a query
+        pf[h] = pf[2 + h] = 0u;
+        continue;
+      }
+      float mx = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float m_new = fmaxf(mrow[h], mx * p.scale_log2);
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;  // every score so far is -inf: p = 0
+      if (__any_sync(0xffffffffu, m_new != mrow[h])) {
+        const float alpha = sfu_ex2(mrow[h] - m_use);
+        mrow[h] = m_new;
+        lrow[h] *= alpha;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // rows lane / 4 and lane / 4 + 8
-        if (m * 16 + h * 8 >= rows) {  // eight rows without a query
-          pf[m][h] = pf[m][2 + h] = 0u;
-          continue;
+        for (int n = 0; n < kD / 8; ++n) {
+          o[n][2 * h] *= alpha;
+          o[n][2 * h + 1] *= alpha;
         }
-        float mx = fmaxf(fmaxf(s[m][0][2 * h], s[m][0][2 * h + 1]), fmaxf(s[m][1][2 * h], s[m][1][2 * h + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(mrow[m][h], mx * p.scale_log2);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;  // every score so far is -inf: p = 0
-        if (__any_sync(0xffffffffu, m_new != mrow[m][h])) {
-          const float alpha = sfu_ex2(mrow[m][h] - m_use);
-          mrow[m][h] = m_new;
-          lrow[m][h] *= alpha;
+      }
 #pragma unroll
-          for (int n = 0; n < kD / 8; ++n) {
-            o[m][n][2 * h] *= alpha;
-            o[m][n][2 * h + 1] *= alpha;
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float e0 = sfu_ex2(fmaf(s[m][n][2 * h], p.scale_log2, -m_use));
-          const float e1 = sfu_ex2(fmaf(s[m][n][2 * h + 1], p.scale_log2, -m_use));
-          lrow[m][h] += e0 + e1;
-          pf[m][2 * n + h] = Pack2<T>::pack(e0, e1);
-        }
+      for (int n = 0; n < 2; ++n) {
+        const float e0 = sfu_ex2(fmaf(s[n][2 * h], p.scale_log2, -m_use));
+        const float e1 = sfu_ex2(fmaf(s[n][2 * h + 1], p.scale_log2, -m_use));
+        lrow[h] += e0 + e1;
+        pf[2 * n + h] = Pack2<T>::pack(e0, e1);
       }
     }
 #pragma unroll
@@ -337,11 +312,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const _
       if (ks >= nks) break;
       uint32_t vf[4];
       ldsm4_t(vf, st + v_off[ks & 3] + (ks >> 2) * 128);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        mma16816<T>(o[m][2 * ks], pf[m], vf[0], vf[1]);
-        mma16816<T>(o[m][2 * ks + 1], pf[m], vf[2], vf[3]);
-      }
+      mma16816<T>(o[2 * ks], pf, vf[0], vf[1]);
+      mma16816<T>(o[2 * ks + 1], pf, vf[2], vf[3]);
     }
     issue();  // into the stage of tile i - 1, which every lane has left
     st = st == ring + (kSt - 1) * (2 * kTile) ? ring : st + 2 * kTile;
@@ -351,21 +323,19 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const _
 
   // the warps' parts: output rows, maximum and sum
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int h = 0; h < 2; ++h) {
+    const int r = h * 8 + (lane >> 2);
+    float l = lrow[h];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    float* dst = s_part + (warp * kRowsMax + r) * kPitch + (lane & 3) * 2;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = m * 16 + h * 8 + (lane >> 2);
-      float l = lrow[m][h];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      float* dst = s_part + (warp * kRowsMax + r) * kPitch + (lane & 3) * 2;
-#pragma unroll
-      for (int n = 0; n < kD / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[m][n][2 * h], o[m][n][2 * h + 1]);
-      if ((lane & 3) == 0) {
-        s_ml[(warp * kRowsMax + r) * 2] = mrow[m][h];
-        s_ml[(warp * kRowsMax + r) * 2 + 1] = l;
-      }
+    for (int n = 0; n < kD / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+    if ((lane & 3) == 0) {
+      s_ml[(warp * kRowsMax + r) * 2] = mrow[h];
+      s_ml[(warp * kRowsMax + r) * 2 + 1] = l;
     }
+  }
   __syncthreads();
   T* out = static_cast<T*>(p.out);
   auto store = [&](int r, int c4, float4 v, float l) {
@@ -940,10 +910,10 @@ int encode_rows(CUtensorMap* map, int dtype, const void* base, int64_t ld, int64
   return LF_OK;
 }
 
-template <typename T, int kD, int MT>
-int launch_decode(const CrossParams& p, unsigned row_blocks, int dev, cudaStream_t s) {
-  constexpr auto kern = cross_decode_kernel<T, kD, MT>;
-  constexpr int smem = decode_smem(kD, MT);
+template <typename T, int kD>
+int launch_decode(const CrossParams& p, int dev, cudaStream_t s) {
+  constexpr auto kern = cross_decode_kernel<T, kD>;
+  constexpr int smem = decode_smem(kD);
   cudaError_t e = allow_smem<kern>(dev, smem);
   if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute(cross_decode)");
   cudaLaunchAttribute attr[2];
@@ -954,7 +924,7 @@ int launch_decode(const CrossParams& p, unsigned row_blocks, int dev, cudaStream
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(p.n_items) * unsigned(p.n_kv_heads) * unsigned(p.split), row_blocks);
+  cfg.gridDim = dim3(unsigned(p.n_items) * unsigned(p.n_kv_heads) * unsigned(p.row_blocks) * unsigned(p.split));
   cfg.blockDim = dim3(32 * kDecodeWarps);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -1033,29 +1003,40 @@ extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q,
   const int dev = current_device(), sms = device_sms(dev);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == LF_DTYPE_BF16;
-  const int64_t rows = int64_t(max_q) * p.group;
-  const bool decode = max_q <= kRows && rows <= 32;
-  if (decode) {
-    const int mt = rows <= 16 ? 1 : 2;
-    const int64_t blocks = (rows + 16 * mt - 1) / (16 * mt);
-    const int64_t units = int64_t(n_items) * n_kv_heads;
-    if (units * 8 > INT32_MAX || blocks > 65535) return set_error(LF_ERR_UNSUPPORTED, "%s: too many records", fn);
-    // The keys are split only as far as it takes for the longest sequence not to outlast the
-    // others: a CTA costs 3 us beside its keys (64 sequences of 4,096 keys, 16 heads of 64, with four stages:
-    // 185 us whole, 172 in halves, 188 in quarters, 235 in eighths; 1 of 8,192: 92, 52, 30, 21).
-    const int64_t slots = int64_t(sms) * (head_dim <= 64 ? 4 : 2);  // CTAs that fit the GPU
-    const int64_t mean = units * blocks * (n_kv / n_items) / slots;  // keys for each of them
-    p.split = 1;
-    while (p.split < 8 && max_kv / (2 * p.split) >= 64 && max_kv / p.split > mean + mean / 4) p.split *= 2;
-    const unsigned rb = unsigned(blocks);
-    if (head_dim <= 64) {
-      if (mt == 1) return bf ? launch_decode<__nv_bfloat16, 64, 1>(p, rb, dev, s) : launch_decode<__half, 64, 1>(p, rb, dev, s);
-      return bf ? launch_decode<__nv_bfloat16, 64, 2>(p, rb, dev, s) : launch_decode<__half, 64, 2>(p, rb, dev, s);
-    }
-    if (mt == 1) return bf ? launch_decode<__nv_bfloat16, 128, 1>(p, rb, dev, s) : launch_decode<__half, 128, 1>(p, rb, dev, s);
-    return bf ? launch_decode<__nv_bfloat16, 128, 2>(p, rb, dev, s) : launch_decode<__half, 128, 2>(p, rb, dev, s);
+  // Which kernel: both times in us as measured on this GPU (launch and first loads aside),
+  // keys a sequence by their mean.  The few-row kernel passes 1.8 (64 columns) or 0.95
+  // million 16-row x 16-key tiles a second, a warp alone one a microsecond, and reads K and
+  // V at 6.3 TB/s at best; the other takes 1.25 us a tile of 128 keys with one group of an SM
+  // at work, 2.0 with two (64 keys at 128 columns: 0.95 and 1.05), and 2 us a unit.
+  // Measured at 8 sequences of 4,096 keys, 16 heads of 64: 16 queries 32 and 50 us, 32: 46
+  // and 50, 64: 79 and 50; 1 of 8,192: 128 queries 46 and 87; 64 of 272: 32 queries 38 and 32.
+  const int64_t blocks = (int64_t(max_q) * p.group + kDecodeRows - 1) / kDecodeRows;
+  const int64_t units = int64_t(n_items) * n_kv_heads;
+  const int64_t mean_kv = n_kv / n_items < max_kv ? n_kv / n_items : max_kv;
+  const bool narrow = head_dim <= 64;
+  // The keys are split only as far as it takes for the longest sequence not to outlast the
+  // others: a CTA costs 3 us beside its keys (64 sequences of 4,096 keys, 16 heads of 64, with
+  // four stages: 185 us whole, 172 in halves, 188 in quarters, 235 in eighths; 1 of 8,192: 92,
+  // 52, 30, 21).
+  const int64_t slots = int64_t(sms) * (narrow ? 4 : 2);  // CTAs that fit the GPU
+  const int64_t share = units * blocks * mean_kv / slots;  // keys for each of them
+  int split = 1;
+  while (split < 8 && max_kv / (2 * split) >= 64 && max_kv / split > share + share / 4) split *= 2;
+  const double tiles16 = double(units) * double(blocks) * double(mean_kv) / 16.0;
+  const double t_few = std::fmax(std::fmax(tiles16 / (narrow ? 1800.0 : 950.0), double(max_kv) / (64.0 * split)),
+                                 double(units) * double(mean_kv) * head_dim * 4.0 / 6.3e6);
+  const int64_t p_units = int64_t(n_items) * n_heads;
+  const double p_keys = narrow ? 128.0 : 64.0, p_one = narrow ? 1.25 : 0.95, p_two = narrow ? 2.0 : 1.05;
+  const double rounds = std::ceil(double(p_units) / (2.0 * sms));
+  const double t_many = std::fmax(p_units <= sms ? 0.0 : rounds * (std::ceil(double(mean_kv) / p_keys) * p_two + 2.0),
+                                  std::ceil(double(max_kv) / p_keys) * p_one + 2.0);
+  if (max_q <= kRows && t_few <= t_many && units * blocks * 8 <= INT32_MAX) {
+    p.row_blocks = int32_t(blocks);
+    p.split = split;
+    if (narrow) return bf ? launch_decode<__nv_bfloat16, 64>(p, dev, s) : launch_decode<__half, 64>(p, dev, s);
+    return bf ? launch_decode<__nv_bfloat16, 128>(p, dev, s) : launch_decode<__half, 128>(p, dev, s);
   }
-  const int key_tile = head_dim <= 64 ? Shape<64>::kKeys : Shape<128>::kKeys;
+  const int key_tile = narrow ? Shape<64>::kKeys : Shape<128>::kKeys;
   int rc;
   if ((rc = encode_rows(&p.q_map, dtype, q, ldq, n_q, n_heads, head_dim, kRows, "q"))) return rc;
   // no keys at all: the row read in the place of one (its result is not used) is a query row
@@ -1063,6 +1044,6 @@ extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q,
   const int64_t kv_rows = n_kv > 0 ? n_kv : n_q;
   if ((rc = encode_rows(&p.k_map, dtype, kb, n_kv > 0 ? ldk : ldq, kv_rows, n_kv_heads, head_dim, key_tile, "k"))) return rc;
   if ((rc = encode_rows(&p.v_map, dtype, vb, n_kv > 0 ? ldv : ldq, kv_rows, n_kv_heads, head_dim, key_tile, "v"))) return rc;
-  if (head_dim <= 64) return bf ? launch_prompt<__nv_bfloat16, 64>(p, dev, s) : launch_prompt<__half, 64>(p, dev, s);
+  if (narrow) return bf ? launch_prompt<__nv_bfloat16, 64>(p, dev, s) : launch_prompt<__half, 64>(p, dev, s);
   return bf ? launch_prompt<__nv_bfloat16, 128>(p, dev, s) : launch_prompt<__half, 128>(p, dev, s);
 }

@@ -99,7 +99,7 @@ def test_prompts(cuda, dtype, heads, kv_heads, d):
 
 
 @pytest.mark.parametrize("heads,kv_heads,d", [(4, 4, 64), (4, 2, 128), (2, 2, 80)])
-@pytest.mark.parametrize("q", [[1, 1, 1], [3, 1, 5], [9, 16, 2], [17, 32, 8], [40, 3, 150]])
+@pytest.mark.parametrize("q", [[1, 1, 1], [3, 1, 5], [9, 16, 2], [17, 32, 8], [100, 128, 1], [40, 3, 150]])
 def test_long_keys_and_a_moving_max(cuda, heads, kv_heads, d, q):
     """Up to 8,192 keys: every split of the few-row kernel, many tiles of the other, with
     scores that grow along the keys."""
@@ -124,7 +124,7 @@ def test_scale_and_one_hot_scores(cuda):
     run(cuda, [140, 1], [100, 500], 2, 1, 128, torch.float16, scale=1e-6)
 
 
-@pytest.mark.parametrize("q_len", [1, 70])
+@pytest.mark.parametrize("q_len", [1, 70, 150])
 def test_no_keys_at_all(cuda, q_len):
     q = torch.randn(2 * q_len, 128, device=cuda, dtype=torch.bfloat16)
     k = torch.empty(0, 128, device=cuda, dtype=torch.bfloat16)
@@ -134,7 +134,7 @@ def test_no_keys_at_all(cuda, q_len):
     assert none.shape == (0, 128)
 
 
-@pytest.mark.parametrize("q_len", [2, 90])
+@pytest.mark.parametrize("q_len", [2, 90, 150])
 def test_infinities_stay_in_their_sequence_and_scores(cuda, q_len):
     """A key of -inf scores (its probability is 0) changes nothing but its own weight; a NaN
     value makes its sequence NaN and no other."""
@@ -154,7 +154,7 @@ def test_infinities_stay_in_their_sequence_and_scores(cuda, q_len):
     assert torch.equal(got[:q_len], want[:q_len]) and torch.equal(got[2 * q_len:], want[2 * q_len:])
 
 
-@pytest.mark.parametrize("q_len", [1, 50])
+@pytest.mark.parametrize("q_len", [1, 50, 140])
 def test_shared_states(cuda, q_len):
     """Beams: sequences whose key ranges coincide or overlap read the same states."""
     q = torch.randn(4 * q_len, 256, device=cuda, dtype=torch.float16)
@@ -173,7 +173,7 @@ def test_far_rows(cuda):
     tail = torch.randn(2100, 256, device=cuda, dtype=torch.bfloat16)
     kv[rows - 2100:, 3840:] = tail
     k, v = kv[:, 3840:3968], kv[:, 3968:]
-    for q_len in (1, 100):
+    for q_len in (1, 100, 140):
         q = torch.randn(2 * q_len, 128, device=cuda, dtype=torch.bfloat16)
         batch = cross_batch([q_len] * 2, [2100, 70], cuda, kv_starts=[rows - 2100, rows - 70])
         out = cross_attention_varlen(q, k, v, batch, 2)
@@ -182,7 +182,7 @@ def test_far_rows(cuda):
     del kv, k, v
 
 
-@pytest.mark.parametrize("q_len", [1, 100])
+@pytest.mark.parametrize("q_len", [1, 100, 140])
 def test_capture_replay_and_streams(cuda, q_len):
     kv = torch.randn(1500, 512, device=cuda, dtype=torch.bfloat16)
     k, v = kv[:, :256], kv[:, 256:]
@@ -215,7 +215,7 @@ def test_capture_replay_and_streams(cuda, q_len):
         assert torch.equal(o, want[n % 4])
 
 
-@pytest.mark.parametrize("q_len", [2, 80])
+@pytest.mark.parametrize("q_len", [2, 80, 140])
 def test_records_outside_the_tensors_store_nothing(cuda, q_len):
     """Records past the queries or the keys, with a negative start or a tile past their
     queries, are reported and write no row; the others are as without them."""
