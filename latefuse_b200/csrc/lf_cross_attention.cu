@@ -522,8 +522,8 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
   const uint32_t sK = sQ + Sh::kQBytes;
   const uint32_t sV = sK + kStages * kKvBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(gbase + kGroups * Sh::kGroupBytes);
-  constexpr int Q_FULL = 0, Q_EMPTY = 1, S_FULL = 2, S_EMPTY = 3, P_FULL = 4, PV_DONE = 5, O_FULL = 6, O_EMPTY = 7,
-                DRAIN = 8, K_FULL = 9, K_EMPTY = K_FULL + kStages, V_FULL = K_EMPTY + kStages, V_EMPTY = V_FULL + kStages,
+  constexpr int Q_FULL = 0, Q_EMPTY = 1, S_FULL = 2, S_EMPTY = 3, P_FULL = 4, PV_DONE = 5, O_EMPTY = 6, DRAIN = 7,
+                K_FULL = 8, K_EMPTY = K_FULL + kStages, V_FULL = K_EMPTY + kStages, V_EMPTY = V_FULL + kStages,
                 N_BARS = V_EMPTY + kStages;  // of a group
   auto bar = [&](int i) { return smem_u32(&bars[grp * N_BARS + i]); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(&bars[kGroups * N_BARS]);
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
                      v_desc0 = smem_desc(sV, kKeys * 128, 1024, 2);
       Cursor c;
       start(c);
-      bool prev = false, prev_first = false, prev_last = false;  // the tile whose O += P V is still to be issued
+      bool prev = false, prev_first = false;  // the tile whose O += P V is still to be issued
       int prev_n16 = 0, prev_t = 0, prev_u = 0;
       while (true) {
         const bool now = c.unit < n_units;
@@ -707,13 +707,11 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
             }
             umma_commit(bar(V_EMPTY + s));
             umma_commit(bar(PV_DONE));
-            if (prev_last) umma_commit(bar(O_FULL));
           }
           __syncwarp();
         }
         prev = now;
         prev_first = first;
-        prev_last = last;
         prev_n16 = n16;
         prev_t = t;
         prev_u = u;
@@ -737,6 +735,42 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
     Cursor c;
     start(c);
     float m = -INFINITY, l = 0.f;
+    // A unit's output O / l is stored during the next unit's first tile, whose wait for
+    // PV_DONE is the wait for the unit's last O += P V: 1 nothing, 2 zeros (no keys), 0 O / l.
+    bool pend = false, pend_rows = false;
+    int pend_mode = 1;
+    float pend_inv = 0.f;
+    T* pend_dst = nullptr;
+    auto store_pending = [&](bool done) {
+      if (done && pend_rows) {
+        tc_fence_after();
+#pragma unroll 1
+        for (int b = 0; b < 2 * Sh::kBlocks; ++b) {
+          uint32_t ov[32];
+          tmem_ld32(o_addr + b * 32, ov);
+          if (pend_mode != 1) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              if (b * 32 + q * 8 >= p.d) break;
+              uint4 w;
+              if (pend_mode == 2) {  // no keys: zeros, whatever the key row read in their place holds
+                w = make_uint4(0u, 0u, 0u, 0u);
+              } else {
+                w.x = Pack2<T>::pack(__uint_as_float(ov[8 * q + 0]) * pend_inv, __uint_as_float(ov[8 * q + 1]) * pend_inv);
+                w.y = Pack2<T>::pack(__uint_as_float(ov[8 * q + 2]) * pend_inv, __uint_as_float(ov[8 * q + 3]) * pend_inv);
+                w.z = Pack2<T>::pack(__uint_as_float(ov[8 * q + 4]) * pend_inv, __uint_as_float(ov[8 * q + 5]) * pend_inv);
+                w.w = Pack2<T>::pack(__uint_as_float(ov[8 * q + 6]) * pend_inv, __uint_as_float(ov[8 * q + 7]) * pend_inv);
+              }
+              reinterpret_cast<uint4*>(pend_dst + b * 32)[q] = w;
+            }
+          }
+        }
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(O_EMPTY));
+      pend = false;
+    };
     while (c.unit < n_units) {
       const int t = c.t, j = c.j;
       const bool last = j == c.n_kv - 1;
@@ -826,6 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
       } else {
         go = work && wwait(bar(PV_DONE), (t & 1) ^ 1);
       }
+      if (pend) store_pending(go);  // PV_DONE was that of the unit before's last tile
       l = (j == 0) ? sum : l * alpha + sum;
       m = m_new;
       // the last 16-key step of a tile that ends inside it multiplies value rows past the
@@ -847,42 +882,17 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(P_FULL));
-      if (last) {
-        // the unit's output: O / l, once its last O += P V has finished
-        if (wwait(bar(O_FULL), c.u & 1) && rows_live) {
-          tc_fence_after();
-          const int r = row - shift, what = c.it.what;  // row of the query tile
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          T* dst = reinterpret_cast<T*>(p.out) + (int64_t(c.it.q0) + c.it.tile * kRows + r) * p.ldo +
-                   int64_t(c.unit % p.n_heads) * p.d;
-#pragma unroll 1
-          for (int b = 0; b < 2 * Sh::kBlocks; ++b) {
-            uint32_t ov[32];
-            tmem_ld32(o_addr + b * 32, ov);
-            if (r >= 0 && r < n_rows && what != 1) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                if (b * 32 + q * 8 >= p.d) break;
-                uint4 w;
-                if (what == 2) {  // no keys: zeros, whatever the key row read in their place holds
-                  w = make_uint4(0u, 0u, 0u, 0u);
-                } else {
-                  w.x = Pack2<T>::pack(__uint_as_float(ov[8 * q + 0]) * inv, __uint_as_float(ov[8 * q + 1]) * inv);
-                  w.y = Pack2<T>::pack(__uint_as_float(ov[8 * q + 2]) * inv, __uint_as_float(ov[8 * q + 3]) * inv);
-                  w.z = Pack2<T>::pack(__uint_as_float(ov[8 * q + 4]) * inv, __uint_as_float(ov[8 * q + 5]) * inv);
-                  w.w = Pack2<T>::pack(__uint_as_float(ov[8 * q + 6]) * inv, __uint_as_float(ov[8 * q + 7]) * inv);
-                }
-                reinterpret_cast<uint4*>(dst + b * 32)[q] = w;
-              }
-            }
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(O_EMPTY));
+      if (last) {  // the unit's output waits for its last O += P V
+        const int r = row - shift;  // row of the query tile
+        pend = true;
+        pend_rows = rows_live;
+        pend_mode = r >= 0 && r < n_rows ? c.it.what : 1;
+        pend_inv = l == 0.f ? 0.f : 1.f / l;
+        pend_dst = static_cast<T*>(p.out) + (int64_t(c.it.q0) + c.it.tile * kRows + r) * p.ldo + int64_t(c.unit % p.n_heads) * p.d;
       }
       advance(c);
     }
+    if (pend) store_pending(wwait(bar(PV_DONE), (c.t - 1) & 1));
   }
 
   __syncthreads();

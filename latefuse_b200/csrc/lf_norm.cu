@@ -233,7 +233,7 @@ add_layernorm_kernel(const NormParams p, int full) {
     for (int c = 0; c < NC; ++c) {
       const int col = c * 256 + lane * 8;
       if (full || col < H) {
-        *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) = rq.q8(v[c]);
+        *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) = rq.q8<T>(v[c]);
       }
     }
   }

@@ -1,11 +1,16 @@
 // Symmetric 8-bit quantisation of a row: with top = max |x| over the row,
 //     scale = top / 127                 (rounded to f32)
 //     q     = round_half_even(127 x / top)          in [-127, 127]
-// The quotient is decided exactly: it is formed in f32 as v = x * (127 / top), which is
-// off by at most 127.5 * 2^-23 < 2^-15, and where v lies nearer than 2^-15 to a half the
-// remainder decides (RowQuant::settle).  So q does not depend on how a caller rounds, and
-// ties (frequent with 16-bit inputs: top = 254 * 2^e makes every second integer one) go
-// to the even step.  A row of zeros gives q = 0, scale = 0.  A row with an infinity or
+// The quotient is decided exactly.  For f32 rows it is formed as v = x * (127 / top), which
+// is off by at most 127.5 * 2^-23 < 2^-15, and where v lies nearer than 2^-15 to a half the
+// remainder decides (quant_settle).  With 16-bit values exact halves are frequent (0.5% of
+// bf16's: one or more in most warps' 32), so their quotients are divided out instead
+// (RowQuant::q8): v = v0 + (p - v0 top) / top with p = 127 x and v0 = p * (1 / top), where
+// the FMA makes p - v0 top exact, is the quotient itself whenever f32 holds it, as it
+// holds every half; and a quotient of two values of at most 11 bits that is not a half is
+// 2^(k - 12) or more away from one (k the exponent of x less that of top) where v is
+// 2^(k - 16) off.  So q does not depend on how a caller rounds, and ties go to the even
+// step.  A row of zeros gives q = 0, scale = 0.  A row with an infinity or
 // NaN gives q = 0 and scale = NaN, so that whatever is computed from the row is NaN.
 #pragma once
 
@@ -16,13 +21,29 @@ namespace lf {
 // |x| as an integer that orders like the magnitude, NaN above infinity (fmaxf would drop NaN).
 __device__ __forceinline__ uint32_t mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// Rounds 127 x / top where v = x * (127 / top) lies next to r + 1/2 or r - 1/2 (r = rint(v)),
+// or is not a number: 127 x - r top is exact in two floats (the product 127 x splits
+// exactly, and its head minus r top is a multiple of ulp(top) / 2 below 2^24 of them), so
+// comparing it with top / 2 is exact.  Rare, and out of line: inlined for each of a lane's
+// 32 values it doubled the kernels' code and time.
+__device__ __noinline__ static float quant_settle(float x, float r, float top, float inv) {
+  if (!(fabsf(r) <= 128.f) || inv == 0.f) return 0.f;  // only rows that are not finite (or all 0) come here so
+  const float p = 127.f * x, e = fmaf(127.f, x, -p), rem = fmaf(-r, top, p);
+  const float sgn = rem < 0.f ? -1.f : 1.f;
+  const float over = (fabsf(rem) - 0.5f * top) + sgn * e;  // its sign is exact: the difference is
+  const bool odd = (int(r) & 1) != 0;
+  return over > 0.f || (over == 0.f && odd) ? r + sgn : r;
+}
+
 struct RowQuant {
   static constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, ties to even
   float pre;    // a power of two that keeps top and 127 x clear of f32's ends
   float top;    // the row's largest magnitude, times pre
   float inv;    // 127 / top; 0 for a row of zeros or a row that is not finite
   float scale;
-  float inv_raw;  // 127 / the row's largest magnitude, for rows well inside f32's range; else 0
+  float raw;      // the row's largest magnitude where it is well inside f32's range; else 0
+  float rcp;      // 1 / raw, inv_raw = 127 / raw (0 where raw is)
+  float inv_raw;
   // top_bits: the largest mag_bits of the row
   __device__ __forceinline__ explicit RowQuant(uint32_t top_bits) {
     const float t = __uint_as_float(top_bits);
@@ -31,18 +52,9 @@ struct RowQuant {
     top = t * pre;
     inv = (top_bits == 0u || !finite) ? 0.f : __fdiv_rn(127.f, top);
     scale = finite ? __fdiv_rn(t, 127.f) : __uint_as_float(0x7fc00000u);
-    inv_raw = t > 0x1p-100f && t < 0x1p120f ? __fdiv_rn(127.f, t) : 0.f;  // NaN and infinity: 0
-  }
-  // v next to r + 1/2 or r - 1/2 (r = rint(v)), or not a number: 127 x - r top is exact
-  // in two floats (the product 127 x splits exactly, and its head minus r top is a
-  // multiple of ulp(top) / 2 below 2^24 of them), so comparing it with top / 2 is exact.
-  __device__ __forceinline__ float settle(float x, float r) const {
-    if (!(fabsf(r) <= 128.f) || inv == 0.f) return 0.f;  // only rows that are not finite (or all 0) come here so
-    const float p = 127.f * x, e = fmaf(127.f, x, -p), rem = fmaf(-r, top, p);
-    const float sgn = rem < 0.f ? -1.f : 1.f;
-    const float over = (fabsf(rem) - 0.5f * top) + sgn * e;  // its sign is exact: the difference is
-    const bool odd = (__float_as_int(r + kMagic) & 1) != 0;
-    return over > 0.f || (over == 0.f && odd) ? r + sgn : r;
+    raw = t > 0x1p-100f && t < 0x1p100f ? t : 0.f;  // NaN and infinity: 0
+    rcp = raw != 0.f ? __frcp_rn(raw) : 0.f;
+    inv_raw = raw != 0.f ? __fdiv_rn(127.f, raw) : 0.f;
   }
   // q in the low byte (two's complement) of the result
   __device__ __forceinline__ uint32_t q(float x) const {
@@ -50,28 +62,43 @@ struct RowQuant {
     const float v = x * inv;
     float m = v + kMagic;
     const float r = m - kMagic;
-    if (!(fabsf(v - r) < 0.499969482421875f)) m = settle(x, r) + kMagic;
+    if (!(fabsf(v - r) < 0.499969482421875f)) m = quant_settle(x, r, top, inv) + kMagic;
     return __float_as_uint(m);
   }
   // q of four values, the first in the low byte
   __device__ __forceinline__ uint32_t q4(float a, float b, float c, float d) const {
     return __byte_perm(__byte_perm(q(a), q(b), 0x0040), __byte_perm(q(c), q(d), 0x0040), 0x5410);
   }
-  // q of eight values, the first in the low byte of x.  Pairs at a time, and one test for all
-  // eight: a value next to a half, or a row at the ends of f32's range, takes q4.
+  // q of eight values of type T, the first in the low byte of x.  Rows at the ends of f32's
+  // range take q4, and of f32 rows any eight with a value next to a half.
+  template <typename T>
   __device__ __forceinline__ uint2 q8(const float (&x)[8]) const {
     uint32_t m[8];
-    float far = inv_raw == 0.f ? 1.f : 0.f;  // the largest distance to the nearest integer
+    bool slow = raw == 0.f;
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 v = f2_mul(make_float2(x[2 * i], x[2 * i + 1]), f2(inv_raw));
-      const float2 w = f2_add(v, f2(kMagic));
-      const float2 d = f2_add(v, f2_fma(w, f2(-1.f), f2(kMagic)));  // v - (w - magic), both exact
-      far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
-      m[2 * i] = __float_as_uint(w.x);
-      m[2 * i + 1] = __float_as_uint(w.y);
+      for (int i = 0; i < 4; ++i) {
+        const float2 p = f2_mul(make_float2(x[2 * i], x[2 * i + 1]), f2(127.f));
+        const float2 v0 = f2_mul(p, f2(rcp));
+        const float2 v = f2_fma(f2_fma(v0, f2(-raw), p), f2(rcp), v0);
+        const float2 w = f2_add(v, f2(kMagic));
+        m[2 * i] = __float_as_uint(w.x);
+        m[2 * i + 1] = __float_as_uint(w.y);
+      }
+    } else {
+      float far = 0.f;  // the largest distance to the nearest integer
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = f2_mul(make_float2(x[2 * i], x[2 * i + 1]), f2(inv_raw));
+        const float2 w = f2_add(v, f2(kMagic));
+        const float2 d = f2_add(v, f2_fma(w, f2(-1.f), f2(kMagic)));  // v - (w - magic), both exact
+        far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+        m[2 * i] = __float_as_uint(w.x);
+        m[2 * i + 1] = __float_as_uint(w.y);
+      }
+      slow |= far >= 0.499969482421875f;
     }
-    if (far >= 0.499969482421875f) return make_uint2(q4(x[0], x[1], x[2], x[3]), q4(x[4], x[5], x[6], x[7]));
+    if (slow) return make_uint2(q4(x[0], x[1], x[2], x[3]), q4(x[4], x[5], x[6], x[7]));
     return make_uint2(
         __byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410),
         __byte_perm(__byte_perm(m[4], m[5], 0x0040), __byte_perm(m[6], m[7], 0x0040), 0x5410));

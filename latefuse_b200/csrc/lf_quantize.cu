@@ -81,9 +81,9 @@ struct Chunk {
     }
     if constexpr (VEC) {
       const int32_t col = base + lane * 8;
-      if (col < cols) *reinterpret_cast<uint2*>(row + col) = rq.q8(v);
+      if (col < cols) *reinterpret_cast<uint2*>(row + col) = rq.q8<T>(v);
     } else {
-      const uint2 q = rq.q8(v);
+      const uint2 q = rq.q8<T>(v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int32_t col = base + i * 32 + lane;

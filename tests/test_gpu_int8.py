@@ -104,6 +104,25 @@ def test_quantize_rows_ties_and_ends(cuda, dtype):
         assert torch.equal(r.q.double(), q) and torch.equal(r.scale, scale)
 
 
+@pytest.mark.parametrize("dtype,digits", [(torch.bfloat16, 8), (torch.float16, 11)])
+def test_quantize_rows_every_quotient(cuda, dtype, digits):
+    """Every pair of significands of the type (f16: every seventh of the largest's), at every
+    distance of exponents that leaves a quotient of 1/2 or more: the halves among them,
+    and the quotients next to halves, are rounded as the definition says."""
+    lo, hi = 2 ** (digits - 1), 2 ** digits
+    tops = torch.arange(lo, hi, 1 if digits == 8 else 7, device=cuda)
+    sig = torch.arange(lo, hi, device=cuda)
+    x = torch.cat([sig * 2.0 ** -k for k in range(9)] + [torch.zeros(1, device=cuda)])
+    rows = x.repeat(tops.numel(), 1)
+    rows[rows > tops[:, None]] = 1.0
+    rows[:, -1] = tops
+    rows[:, ::2] *= -1
+    rows = (rows * 2.0 ** -6).to(dtype)
+    r = quantize_rows(rows)
+    q, scale = ref_rows(rows)
+    assert torch.equal(r.q.double(), q) and torch.equal(r.scale, scale)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_of_zeros_infinities_and_nan(cuda, dtype):
     x = torch.randn(6, 72, device=cuda).to(dtype)
