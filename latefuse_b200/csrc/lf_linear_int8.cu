@@ -449,7 +449,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
 // ---------------------------------------------------------------------------
 // few tokens: 128 channels x NT tokens per CTA, K split over a cluster
 // ---------------------------------------------------------------------------
-constexpr int kSplitThreads = 64 + 128;
+constexpr int kSplitEpiWarps = 8;  // two per TMEM lane quadrant
+constexpr int kSplitThreads = 64 + 32 * kSplitEpiWarps;
 __host__ __device__ constexpr int split_stages(int nt) { return nt <= 32 ? 8 : 6; }
 __host__ __device__ constexpr int split_stage_bytes(int nt) { return 128 * kBK + nt * kBK; }
 constexpr int split_smem_bytes(int nt) { return 1024 + split_stages(nt) * split_stage_bytes(nt) + 512; }
@@ -474,9 +475,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_int8_split_kernel(con
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const int S = p.split;
-  const int rank = int(cluster_ctarank());
+  const int rank = int(uniform(cluster_ctarank()));
   const int32_t n0 = int32_t(blockIdx.x / unsigned(S)) * 128;
   const int64_t m0 = int64_t(blockIdx.y) * NT;
   const int kb0 = int(int64_t(p.n_kb) * rank / S), kb1 = int(int64_t(p.n_kb) * (rank + 1) / S);
@@ -503,68 +504,57 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_int8_split_kernel(con
   }
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   pdl_wait();
   pdl_launch_dependents();
 
-  auto wait = [&](uint32_t b, uint32_t parity) {
-    if (aborted(s_abort)) return false;
-    if (mbar_wait(b, parity)) return true;
-    set_status(p.status, LF_STATUS_TIMEOUT);
-    atomicExch(s_abort, 1);
-    return false;
-  };
-
   if (warp == 0) {
-    if (lane == 0) {
-      int kk = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++kk) {
-        const int s = kk % kSt;
-        if (!wait(bar(EMPTY + s), ((kk / kSt) & 1) ^ 1)) break;
+    int kk = 0;
+    for (int kb = kb0; kb < kb1; ++kb, ++kk) {
+      const int s = kk % kSt;
+      if (!warp_wait(bar(EMPTY + s), ((kk / kSt) & 1) ^ 1, s_abort, p.status)) break;
+      if (elect_one()) {
         const uint32_t st = base + s * kSb;
         mbar_arrive_expect_tx(bar(FULL + s), kSb);
         tma_load_2d(st, &p.w_map, bar(FULL + s), kb * kBK, n0);
         tma_load_2d(st + 128 * kBK, &p.x_map, bar(FULL + s), kb * kBK, int32_t(m0));
       }
-      if (aborted(s_abort))  // loads nobody consumed land before the CTA exits (bounded)
-        for (int q = (kk > kSt ? kk - kSt : 0); q < kk; ++q) mbar_wait(bar(FULL + q % kSt), (q / kSt) & 1);
+      __syncwarp();
     }
+    if (aborted(s_abort))  // loads nobody consumed land before the CTA exits (bounded)
+      for (int q = (kk > kSt ? kk - kSt : 0); q < kk; ++q) mbar_wait(bar(FULL + q % kSt), (q / kSt) & 1);
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = umma_idesc_i8(128, NT);
-      int kk = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++kk) {
-        const int s = kk % kSt;
-        if (!wait(bar(FULL + s), (kk / kSt) & 1)) break;
-        tc_fence_after();
-        const uint32_t st = base + s * kSb;
+    constexpr uint32_t idesc = umma_idesc_i8(128, NT);
+    const uint64_t a_desc = smem_desc(base, 16, 1024, 2), b_desc = smem_desc(base + 128 * kBK, 16, 1024, 2);
+    int kk = 0;
+    for (int kb = kb0; kb < kb1; ++kb, ++kk) {
+      const int s = kk % kSt;
+      if (!warp_wait(bar(FULL + s), (kk / kSt) & 1, s_abort, p.status)) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t off = uint64_t(s * (kSb >> 4));
 #pragma unroll
         for (int q = 0; q < kBK / 32; ++q)
-          umma_i8(tmem, smem_desc(st + q * 32, 16, 1024, 2), smem_desc(st + 128 * kBK + q * 32, 16, 1024, 2), idesc,
-                  (kk | q) != 0 ? 1u : 0u);
+          umma_i8(tmem, a_desc + off + uint64_t(2 * q), b_desc + off + uint64_t(2 * q), idesc, (kk | q) != 0 ? 1u : 0u);
         umma_commit(bar(EMPTY + s));
       }
-      umma_commit(bar(ACC));  // also when unwinding: every issued MMA finishes before TMEM is released
+      __syncwarp();
     }
+    if (elect_one()) umma_commit(bar(ACC));  // also when unwinding: every issued MMA finishes before TMEM is released
     __syncwarp();
   } else {
     // the CTA's partial sums, (token, channel) int32, into the ring once every MMA has read it
-    const int quad = warp & 3;
-    const bool ok = mbar_wait(bar(ACC), 0);
-    if (!ok) {
-      set_status(p.status, LF_STATUS_TIMEOUT);
-      atomicExch(s_abort, 1);
-    }
-    if (__all_sync(0xffffffffu, ok && !aborted(s_abort))) {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    if (warp_wait(bar(ACC), 0, s_abort, p.status)) {
       tc_fence_after();
-      int32_t* acc = reinterpret_cast<int32_t*>(gbase);
+      int32_t* acc = reinterpret_cast<int32_t*>(gbase) + quad * 32 + lane;
 #pragma unroll
-      for (int c = 0; c < NT / 16; ++c) {
+      for (int c = half; c < NT / 16; c += 2) {
         float v[16];
         tmem_ld16(tmem + (uint32_t(quad * 32) << 16) + c * 16, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[(c * 16 + i) * 128 + quad * 32 + lane] = __float_as_int(v[i]);
+        for (int i = 0; i < 16; ++i) acc[(c * 16 + i) * 128] = __float_as_int(v[i]);
       }
       tc_fence_before();
     }
@@ -573,7 +563,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_int8_split_kernel(con
   const bool bad = aborted(s_abort);
   cluster_sync();  // every CTA's partial sums are in place
   if (warp >= 2 && !bad) {
-    // tokens [NT rank / S, NT (rank + 1) / S), one per warp at a time, four channels a lane
+    // tokens [NT rank / S, NT (rank + 1) / S), two per warp at a time, four channels a lane;
+    // all parts of both are on their way before the first is added
     const T* bias = static_cast<const T*>(p.bias);
     T* y = static_cast<T*>(p.y);
     const int32_t ch = n0 + lane * 4;
@@ -585,32 +576,48 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_int8_split_kernel(con
       b[i] = in && bias != nullptr ? DT<T>::to_f(bias[ch + i]) : 0.f;
     }
     const bool whole = ch + 3 < p.n && p.tma_out;
-#pragma unroll 2
-    for (int t = NT * rank / S + (warp - 2); t < NT * (rank + 1) / S; t += 4) {
-      const int64_t row = m0 + t;
-      if (row >= p.m_rows) break;
-      int4 a = make_int4(0, 0, 0, 0);
-      for (int r = 0; r < S; ++r) {
-        const int4 v = ld_dsmem_i4(mapa_shared(base + uint32_t(t * 128 + lane * 4) * 4u, uint32_t(r)));
-        a.x += v.x;
-        a.y += v.y;
-        a.z += v.z;
-        a.w += v.w;
-      }
-      const float xs = __ldg(p.x_scale + row);
-      const float2 lo = finish2<T, kAct>(a.x, a.y, f2(xs), make_float2(ws[0], ws[1]), make_float2(b[0], b[1]));
-      const float2 hi = finish2<T, kAct>(a.z, a.w, f2(xs), make_float2(ws[2], ws[3]), make_float2(b[2], b[3]));
-      T* dst = y + row * p.ldy + ch;
-      if (whole) {
-        if constexpr (sizeof(T) == 2)
-          *reinterpret_cast<uint2*>(dst) = make_uint2(Pack2<T>::pack(lo.x, lo.y), Pack2<T>::pack(hi.x, hi.y));
-        else
-          *reinterpret_cast<float4*>(dst) = make_float4(lo.x, lo.y, hi.x, hi.y);
-      } else {
-        const float o[4] = {lo.x, lo.y, hi.x, hi.y};
+    const int t_end = NT * (rank + 1) / S;
+    uint32_t part[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (ch + i < p.n) dst[i] = DT<T>::from_f(o[i]);
+    for (int r = 0; r < 8; ++r) part[r] = mapa_shared(base + uint32_t(lane) * 16u, uint32_t(r < S ? r : 0));
+    for (int t = NT * rank / S + (warp - 2); t < t_end && m0 + t < p.m_rows; t += 2 * kSplitEpiWarps) {
+      const int t2 = t + kSplitEpiWarps;
+      const bool two = t2 < t_end && m0 + t2 < p.m_rows;
+      int4 v[2][8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        v[0][r] = v[1][r] = make_int4(0, 0, 0, 0);
+        if (r < S) {
+          v[0][r] = ld_dsmem_i4(part[r] + uint32_t(t) * 512u);
+          if (two) v[1][r] = ld_dsmem_i4(part[r] + uint32_t(t2) * 512u);
+        }
+      }
+      const float xs[2] = {__ldg(p.x_scale + m0 + t), two ? __ldg(p.x_scale + m0 + t2) : 0.f};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (k == 1 && !two) break;
+        int4 a = v[k][0];
+#pragma unroll
+        for (int r = 1; r < 8; ++r) {
+          a.x += v[k][r].x;
+          a.y += v[k][r].y;
+          a.z += v[k][r].z;
+          a.w += v[k][r].w;
+        }
+        const float2 lo = finish2<T, kAct>(a.x, a.y, f2(xs[k]), make_float2(ws[0], ws[1]), make_float2(b[0], b[1]));
+        const float2 hi = finish2<T, kAct>(a.z, a.w, f2(xs[k]), make_float2(ws[2], ws[3]), make_float2(b[2], b[3]));
+        T* dst = y + (m0 + (k == 0 ? t : t2)) * p.ldy + ch;
+        if (whole) {
+          if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint2*>(dst) = make_uint2(Pack2<T>::pack(lo.x, lo.y), Pack2<T>::pack(hi.x, hi.y));
+          else
+            *reinterpret_cast<float4*>(dst) = make_float4(lo.x, lo.y, hi.x, hi.y);
+        } else {
+          const float o[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (ch + i < p.n) dst[i] = DT<T>::from_f(o[i]);
+        }
       }
     }
   }
