@@ -35,6 +35,7 @@ from latefuse_b200.lora import (FactorCache, SegmentTable, blocked_u, fused_shri
                                  lora_apply_into, lora_shrink_blocked, per_row_cache, workspace_bytes)
 from latefuse_b200.encoder_ops import (ACT_GELU, add_layernorm, attention_varlen, embed_layernorm, gelu, linear,
                                        linear_accumulate)
+from latefuse_b200.int8_ops import Int8Weight, add_layernorm_int8, ffn_int8, linear_int8
 from latefuse_b200.packing import PackedBatch, pack_rows
 
 # Per-layer module paths (relative to "encoder.layer.{i}.") for each logical target.
@@ -339,6 +340,8 @@ class EncoderWithLora(nn.Module):
         #: pair leaves 73% full (98 vs 103-109 us alone), and the serving step measured
         #: 0.45 ms faster with cuBLAS here.
         self.native_ffn_down = False
+        #: the layers' FFN weights in 8-bit integers (:meth:`quantize_ffn`)
+        self._ffn8: list[tuple[Int8Weight, Int8Weight]] | None = None
         targets = serving_config.target_modules
         self._qkv_targets = [(m, _QKV.index(m)) for m in targets if m in _QKV]
         self._dense_target = "dense" in targets
@@ -350,7 +353,9 @@ class EncoderWithLora(nn.Module):
     # -- construction ----------------------------------------------------------
     @torch.no_grad()
     def load_hf_state_dict(self, sd: dict[str, Tensor]) -> None:
-        """Copy weights from a HuggingFace BERT-family state dict (strict)."""
+        """Copy weights from a HuggingFace BERT-family state dict (strict).  8-bit FFN weights
+        of earlier ones are dropped."""
+        self._ffn8 = None
         sd = {k.removeprefix("bert.").removeprefix("roberta."): v for k, v in sd.items()}
         used: set[str] = set()
 
@@ -421,6 +426,17 @@ class EncoderWithLora(nn.Module):
         if hf_config.pad_token_id is not None:
             model.word_embeddings.weight[hf_config.pad_token_id].zero_()
         return model.eval()
+
+    @torch.no_grad()
+    def quantize_ffn(self, enabled: bool = True) -> None:
+        """Run the FFN projections (two thirds of a layer's products, and the part without a
+        LoRA delta) in 8-bit integers: weights with a scale per output channel, quantised
+        here, activations with a scale per token (:mod:`latefuse_b200.int8_ops`).  The
+        attention projections and their deltas stay in the model's dtype.  Call it once the
+        model is on its GPU, and again if FFN weights change; ``False`` goes back to the
+        model's own weights, which are kept."""
+        self._ffn8 = [(Int8Weight.from_float(layer.wi), Int8Weight.from_float(layer.wo2))
+                      for layer in self.layers] if enabled else None
 
     # -- forward -------------------------------------------------------------
     def position_ids(self, input_ids: Tensor) -> Tensor:
@@ -509,17 +525,21 @@ class EncoderWithLora(nn.Module):
                 else:
                     cache = _DeltaRunner.layerwise_cache(lora_weights[l], "dense")
                     lora_apply(ctx, ao, cache, segs, [0], [0], ws, status)
-            h = self._ffn(layer, ao, h)
+            h = self._ffn(l, ao, h)
         return h.view(B, S, H)
 
-    def _ffn(self, layer: _Layer, ao: Tensor, h: Tensor | None) -> Tensor:
+    def _ffn(self, idx: int, ao: Tensor, h: Tensor | None) -> Tensor:
         """``h1 = LN1(ao + h)`` (``LN1(ao)`` when ``h`` is None: the residual is already
         in ``ao``), then ``LN2(W2 act(W1 h1) + b2 + h1)``, on the native add+LayerNorm and
         GELU kernels.  For bf16/f16 the up projection and its exact GELU run as one launch
         of this library's tcgen05 GEMM (the GELU in its epilogue), the down projection
         accumulates onto ``h1`` in place (beta = 1: cuBLAS, or this library's GEMM when
         ``native_ffn_down``; ``h1`` is not read again) and LayerNorm adds ``b2``, so the
-        residual is not read a second time."""
+        residual is not read a second time.  With :meth:`quantize_ffn` both projections run
+        in 8-bit integers."""
+        layer = self.layers[idx]
+        if self._ffn8 is not None:
+            return self._ffn_int8(layer, self._ffn8[idx], ao, h)
         h1 = add_layernorm(ao, h, layer.ln1.weight, layer.ln1.bias, self.eps)
         if self._native_gelu and self._gemm_ok(h1.dtype, layer.wi.shape):
             mid = linear(h1, layer.wi, layer.bi, act=ACT_GELU)
@@ -533,6 +553,15 @@ class EncoderWithLora(nn.Module):
                 h1.view(-1, h1.shape[-1]).addmm_(mid.view(-1, mid.shape[-1]), layer.wo2.t())
             return add_layernorm(h1, None, layer.ln2.weight, layer.ln2.bias, self.eps, out=h1, vec=layer.bo2)
         o = F.linear(mid, layer.wo2, layer.bo2)
+        return add_layernorm(o, h1, layer.ln2.weight, layer.ln2.bias, self.eps, out=o)
+
+    def _ffn_int8(self, layer: _Layer, weights: tuple[Int8Weight, Int8Weight], ao: Tensor, h: Tensor | None) -> Tensor:
+        up, down = weights
+        if self._native_gelu:
+            h1, o = ffn_int8(ao, h, layer.ln1.weight, layer.ln1.bias, self.eps, up, layer.bi, down, layer.bo2)
+        else:
+            h1, rows = add_layernorm_int8(ao, h, layer.ln1.weight, layer.ln1.bias, self.eps)
+            o = linear_int8(self.act(linear_int8(rows, up, layer.bi)), down, layer.bo2)
         return add_layernorm(o, h1, layer.ln2.weight, layer.ln2.bias, self.eps, out=o)
 
     def _transposed(self, w: Tensor) -> Tensor | None:
@@ -670,7 +699,7 @@ class EncoderWithLora(nn.Module):
                                  shrink=fuse_dense_shrink, weight_t=self._transposed(layer.wo))
                 if ev is not None:
                     ev[1].record()
-                h = self._ffn(layer, ao, h)
+                h = self._ffn(l, ao, h)
             elif fuse_dense:
                 # The delta, bias and residual go first, into a fresh output that
                 # the projection GEMM accumulates onto (beta = 1); the LayerNorm
@@ -682,7 +711,7 @@ class EncoderWithLora(nn.Module):
                 if ev is not None:
                     ev[1].record()
                 ao.addmm_(ctx, layer.wo.t())
-                h = self._ffn(layer, ao, None)
+                h = self._ffn(l, ao, None)
             else:
                 ao = F.linear(ctx, layer.wo, layer.bo)
                 if do_lora and self._dense_target:
@@ -690,7 +719,7 @@ class EncoderWithLora(nn.Module):
                     lora_apply(ctx, ao, store.factor_cache(l), segs, dense_idx, [0], ws, status)
                     if ev is not None:
                         ev[1].record()
-                h = self._ffn(layer, ao, h)
+                h = self._ffn(l, ao, h)
         return h
 
     def encode_pooled_packed(self, pb: PackedBatch, store, pooling: str = "auto",
