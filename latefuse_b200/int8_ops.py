@@ -105,9 +105,9 @@ def quantize_rows(x: Tensor) -> Int8Rows:
 def _bias(bias: Tensor | None, n: int, dtype: torch.dtype) -> Tensor | None:
     if bias is None:
         return None
-    if bias.shape != (n,):
+    if bias.dim() != 1 or bias.numel() != n:
         raise ValueError(f"bias must have {n} entries, got {tuple(bias.shape)}")
-    if bias.dtype != dtype:
+    if bias.dtype is not dtype:
         bias = bias.to(dtype)
     return bias if bias.is_contiguous() else bias.contiguous()
 
@@ -198,8 +198,7 @@ def ffn_int8(a: Tensor, residual: Tensor | None, ln_weight: Tensor, ln_bias: Ten
     m = a2.shape[0]
     w, bb = _bias(ln_weight, hidden, dtype), _bias(ln_bias, hidden, dtype)
     ub, db = _bias(up_bias, inner, dtype), _bias(down_bias, hidden, dtype)
-    both = torch.empty(2, m, hidden, dtype=dtype, device=dev)
-    h, o = both.unbind(0)
+    h, o = (torch.empty(m, hidden, dtype=dtype, device=dev) for _ in range(2))
     lib, code = nat.lib(), nat.dtype_code(dtype)
     size = lib.lf_ffn_int8_workspace_bytes(code, m, hidden, inner)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
