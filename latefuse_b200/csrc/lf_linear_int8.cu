@@ -88,8 +88,8 @@ __device__ __forceinline__ bool aborted(const int32_t* f) { return *reinterpret_
 // R as a polynomial in min(z, 5) - 5/2 whose largest relative error is least: degree 8 for
 // bf16 (2^-13.0 of Phi(-z)), degree 10 for f16 (2^-16.8); beyond 5, where R is held, Phi
 // is below 3e-7 and still falls with the exponential.  One SFU operation a value where
-// gelu2_fast takes two: with K = 1024 the epilogue's GELU set the projection's time
-// (17,410 x 4,096: 92 us, the products alone about 45).
+// gelu2_fast takes two: with K = 1024 the epilogue's GELU sets the projection's time
+// (17,410 x 4,096: 92 us with gelu2_fast, 62 to 68 with this, 57 without an activation).
 template <typename T>
 __device__ __forceinline__ float2 gelu2_narrow(float2 v) {
   const float2 z = make_float2(fminf(fabsf(v.x), 5.f), fminf(fabsf(v.y), 5.f));
@@ -736,7 +736,12 @@ extern "C" int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t 
   p.vec_ch = (reinterpret_cast<uintptr_t>(w_scale) & 7u) == 0 && (reinterpret_cast<uintptr_t>(bias) & (2u * es - 1u)) == 0;
   p.status = status;
 
-  // 256 x 256 tiles once they fill the CTA pairs; below that 128 channels x nt tokens
+  // 256 x 256 tiles once a quarter as many as SMs; below that 128 channels x nt tokens.
+  // Measured with the few-token kernel and with the other (us, bf16, no activation):
+  //   n 1,024, k 4,096: 512 tokens (8 tiles) 14.3 and 20.5; 2,048 (32) 18.5 and 20.5;
+  //     3,000 (48) 32.8 and 20.5
+  //   n 4,096, k 1,024: 256 tokens (16) 12.3 both; 512 (32) 14.3 both; 1,024 (64) 24.6 and 14.3
+  //   n 10,240, k 2,560: 128 tokens (40) 18.4 and 16.4; 256 (40) 26.6 and 16.4
   const int dev = current_device(), sms = device_sms(dev);
   const int64_t big = ((m + 255) / 256) * ((n + 255) / 256);
   const bool batch = big > sms / 4;
@@ -744,7 +749,11 @@ extern "C" int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t 
   p.split = 1;
   if (!batch) {
     const int64_t tiles = ((m + nt - 1) / nt) * ((n + 127) / 128);
-    while (p.split < 8 && tiles * p.split * 2 <= sms && p.split * 2 <= p.n_kb) p.split *= 2;
+    // K is split while every cluster still has its place at once: the GPU's processing clusters
+    // leave room for 33 clusters of four such CTAs and 15 of eight on 148 SMs (16 of eight: 20.5 us,
+    // as 8 with K whole in a quarter each 14.3; 256 tokens, n 1,024, k 4,096).
+    const int64_t room[3] = {sms, int64_t(sms) * 9 / 10, int64_t(sms) * 13 / 16};  // in CTAs, clusters of 2, 4, 8
+    for (int i = 0; i < 3 && tiles * p.split * 2 <= room[i] && p.split * 2 <= p.n_kb; ++i) p.split *= 2;
   }
   int rc;
   if ((rc = encode(&p.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, k, m, ldx, kBK, nt, CU_TENSOR_MAP_SWIZZLE_128B, "x")))
