@@ -1013,34 +1013,48 @@ extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q,
   const int dev = current_device(), sms = device_sms(dev);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == LF_DTYPE_BF16;
-  // Which kernel: both times in us as measured on this GPU (launch and first loads aside),
-  // keys a sequence by their mean.  The few-row kernel passes 1.8 (64 columns) or 0.95
-  // million 16-row x 16-key tiles a second, a warp alone one a microsecond, and reads K and
-  // V at 6.3 TB/s at best; the other takes 1.25 us a tile of 128 keys with one group of an SM
-  // at work, 2.0 with two (64 keys at 128 columns: 0.95 and 1.05), and 2 us a unit.
-  // Measured at 8 sequences of 4,096 keys, 16 heads of 64: 16 queries 32 and 50 us, 32: 46
-  // and 50, 64: 79 and 50; 1 of 8,192: 128 queries 46 and 87; 64 of 272: 32 queries 38 and 32.
+  // Which kernel, and in how many parts the few-row kernel takes a sequence's keys: by their
+  // times in us as measured on this GPU (launch aside), keys a sequence by their mean, the
+  // longest sequence from the start on (the records' order).
+  // A few-row CTA takes 10.5 ns a key (64 columns; 13 at 128) alone and 20.5 with every place
+  // taken (four or two an SM), between them by the square of the share taken, and 3 us beside
+  // its keys, of which the first CTA's pass within the launch; clusters of four find nine
+  // tenths of the places, of eight seven eighths.  Measured with the keys whole, in 2, 4 and 8
+  // parts (64 columns, 16,384 keys each): 16 sequences x heads 172, 92, 51 and 33 us; 80: 174,
+  // 102, 66 and 77; 192: 195, 128, 148 and 132; 320: 228, 275, 228 and 217; 512: 306, 316, 324
+  // and 343; where 64 sequences of 20 to 10,668 keys, 935 on average, with 16 heads take 102 us
+  // in eighths, 68 in quarters.
+  // The other kernel takes 1.25 us a tile of 128 keys with one group of an SM at work, 2.0 with
+  // two (64 keys at 128 columns: 0.95 and 1.05), and 2 us a unit.  Both, with launch, 16 heads
+  // of 64: 8 sequences of 4,096 keys with 16 queries 32 and 50 us, 32: 46 and 50, 64: 79 and 50;
+  // 1 of 8,192: 128 queries 46 and 87; 64 of 272: 32 queries 37 and 31; 200 of 100: 33 queries 82
+  // and 43.
   const int64_t blocks = (int64_t(max_q) * p.group + kDecodeRows - 1) / kDecodeRows;
   const int64_t units = int64_t(n_items) * n_kv_heads;
   const int64_t mean_kv = n_kv / n_items < max_kv ? n_kv / n_items : max_kv;
   const bool narrow = head_dim <= 64;
-  // The keys are split only as far as it takes for the longest sequence not to outlast the
-  // others: a CTA costs 3 us beside its keys (64 sequences of 4,096 keys, 16 heads of 64, with
-  // four stages: 185 us whole, 172 in halves, 188 in quarters, 235 in eighths; 1 of 8,192: 92,
-  // 52, 30, 21).
-  const int64_t slots = int64_t(sms) * (narrow ? 4 : 2);  // CTAs that fit the GPU
-  const int64_t share = units * blocks * mean_kv / slots;  // keys for each of them
+  const double alone = narrow ? 0.0105 : 0.013, full = 0.0205, places = double(sms) * (narrow ? 4.0 : 2.0);
   int split = 1;
-  while (split < 8 && max_kv / (2 * split) >= 64 && max_kv / split > share + share / 4) split *= 2;
-  const double tiles16 = double(units) * double(blocks) * double(mean_kv) / 16.0;
-  const double t_few = std::fmax(std::fmax(tiles16 / (narrow ? 1800.0 : 950.0), double(max_kv) / (64.0 * split)),
-                                 double(units) * double(mean_kv) * head_dim * 4.0 / 6.3e6);
+  double t_few = 0.0;
+  for (int n = 1; n <= 8; n *= 2) {
+    if (n > 1 && max_kv / n < 64) break;
+    const double cap = places * (n <= 2 ? 1.0 : n == 4 ? 0.9 : 7.0 / 8.0);
+    const double ctas = double(units) * double(blocks) * n, waves = std::floor(ctas / cap), rest = ctas / cap - waves;
+    const double rate = alone + (full - alone) * std::fmin(1.0, ctas / cap * ctas / cap);  // of the first wave
+    const double part = double(mean_kv) / n;
+    const double last = rest > 0.0 ? part * (alone + (full - alone) * rest * rest) + 3.0 : 0.0;
+    const double t = std::fmax(waves * (part * full + 3.0) + last, double(max_kv) / n * rate + 3.0);
+    if (n == 1 || t < t_few) {
+      t_few = t;
+      split = n;
+    }
+  }
   const int64_t p_units = int64_t(n_items) * n_heads;
   const double p_keys = narrow ? 128.0 : 64.0, p_one = narrow ? 1.25 : 0.95, p_two = narrow ? 2.0 : 1.05;
   const double rounds = std::ceil(double(p_units) / (2.0 * sms));
-  const double t_many = std::fmax(p_units <= sms ? 0.0 : rounds * (std::ceil(double(mean_kv) / p_keys) * p_two + 2.0),
+  const double t_many = std::fmax(p_units <= sms ? 0.0 : rounds * (double(mean_kv) / p_keys * p_two + 2.0),
                                   std::ceil(double(max_kv) / p_keys) * p_one + 2.0);
-  if (max_q <= kRows && t_few <= t_many && units * blocks * 8 <= INT32_MAX) {
+  if (max_q <= kRows && t_few - 3.0 <= t_many && units * blocks * 8 <= INT32_MAX) {
     p.row_blocks = int32_t(blocks);
     p.split = split;
     if (narrow) return bf ? launch_decode<__nv_bfloat16, 64>(p, dev, s) : launch_decode<__half, 64>(p, dev, s);
