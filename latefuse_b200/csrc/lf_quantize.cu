@@ -4,10 +4,12 @@
 //
 // The bound is HBM: each element is read once and one byte is written.  So a row stays
 // in registers between the search for its largest magnitude and the rounding: 1, 2, 4 or
-// 8 warps share a row (32 elements a lane, rows up to 8,192), 16-byte loads, all of a
-// row's loads in flight before the first is used.  Longer rows are read a second time
-// (from L2), and rows that are not 16-byte aligned or whose length is not a multiple of
-// 8 take one element per load, 32 neighbours to a warp.
+// 8 warps share a row (8 to 32 elements a lane, rows up to 8,192), 16-byte loads, all of a
+// row's loads in flight before the first is used; six CTAs of 8 warps an SM.  Longer rows
+// are read a second time (from L2), and rows that are not 16-byte aligned or whose length
+// is not a multiple of 8 take one element per load, 32 neighbours to a warp.
+// Measured, bf16: 17,410 rows of 4,096 36.8 us (5.8 TB/s), of 1,024 14.3 us with launch;
+// 16,384 of 10,240, read twice, 100 us (5.0 TB/s counted once).
 #include "lf_common.cuh"
 #include "lf_internal.h"
 #include "lf_quant.cuh"
