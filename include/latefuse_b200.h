@@ -460,7 +460,8 @@ int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t ldx, const 
                    void* y, int64_t ldy, int64_t m, int n, int k, int act, int32_t* status);
 
 /* lf_quantize_rows of x (m, k) into the workspace, then lf_linear_int8: the 8-bit projection
- * of float rows in one call of two launches.  The workspace (256-byte aligned, at least
+ * of float rows in one call of two launches; up to 16 rows of up to 4,096, 16,384 elements in all, take one launch
+ * and no workspace (0 bytes).  x and y must not overlap.  The workspace (256-byte aligned, at least
  * lf_linear_rows_int8_workspace_bytes) is free again when the launches have run, so calls
  * that may overlap on the GPU need one each. */
 size_t lf_linear_rows_int8_workspace_bytes(int64_t m, int k);
@@ -473,7 +474,7 @@ int lf_linear_rows_int8(void* stream, int dtype, const void* x, int64_t ldx, con
  *     o = down(round(act(up(h))))
  * up (inner, hidden) and down (hidden, inner) int8 with a scale per row, h and the middle
  * activations quantised per token as lf_quantize_rows does; biases may be NULL.  One call
- * of four launches over one workspace (rules as for lf_linear_rows_int8).  Alignment of a, r,
+ * of four launches (or three, few rows) over one workspace (rules as for lf_linear_rows_int8).  Alignment of a, r,
  * gamma, beta and h as lf_add_layernorm, of up and down as lf_linear_int8; hidden a
  * multiple of 8 up to 4096, inner up to 131072. */
 size_t lf_ffn_int8_workspace_bytes(int dtype, int64_t m, int hidden, int inner);

@@ -32,7 +32,7 @@ using namespace lf;
 extern "C" {
 
 size_t lf_linear_rows_int8_workspace_bytes(int64_t m, int k) {
-  return sizes_ok(LF_DTYPE_F32, m, k, 1) ? RowsAt(0, m, k).end : 0;
+  return sizes_ok(LF_DTYPE_F32, m, k, 1) && !linear_int8_takes_rows(m, k) ? RowsAt(0, m, k).end : 0;
 }
 
 int lf_linear_rows_int8(void* stream, int dtype, const void* x, int64_t ldx, const int8_t* w, int64_t ldw,
@@ -41,6 +41,8 @@ int lf_linear_rows_int8(void* stream, int dtype, const void* x, int64_t ldx, con
   if (!sizes_ok(dtype, m, k, 1))
     return set_error(LF_ERR_INVALID, "lf_linear_rows_int8: dtype %d, m %lld, k %d (k up to 131072)", dtype, (long long)m, k);
   if (m == 0) return LF_OK;
+  if (linear_int8_takes_rows(m, k))
+    return linear_int8_rows(stream, dtype, x, ldx, w, ldw, w_scale, bias, y, ldy, m, n, k, act, status);
   const RowsAt at(0, m, k);
   if (workspace == nullptr || workspace_bytes < at.end || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
     return set_error(LF_ERR_WORKSPACE, "lf_linear_rows_int8: %zu bytes of 256-byte aligned workspace needed, %zu given", at.end,
@@ -81,6 +83,9 @@ int lf_ffn_int8(void* stream, int dtype, const void* a, int64_t lda, const void*
   if (rc) return rc;
   rc = lf_linear_int8(stream, dtype, q1, first.ld, s1, up, ld_up, up_scale, up_bias, mid, ld_mid, m, inner, hidden, act, status);
   if (rc) return rc;
+  if (linear_int8_takes_rows(m, inner))
+    return linear_int8_rows(stream, dtype, mid, ld_mid, down, ld_down, down_scale, down_bias, o, ldo, m, hidden, inner,
+                            LF_ACT_NONE, status);
   rc = lf_quantize_rows(stream, dtype, mid, ld_mid, m, inner, q2, second.ld, s2);
   if (rc) return rc;
   return lf_linear_int8(stream, dtype, q2, second.ld, s2, down, ld_down, down_scale, down_bias, o, ldo, m, hidden, inner,

@@ -267,6 +267,12 @@ cudaError_t allow_smem(int dev, int bytes) {
   return e;
 }
 
+// lf_linear_rows_int8 in one launch without a workspace, for the rows that it takes.
+bool linear_int8_takes_rows(int64_t m, int k);
+int linear_int8_rows(void* stream, int dtype, const void* x, int64_t ldx, const int8_t* w, int64_t ldw,
+                     const float* w_scale, const void* bias, void* y, int64_t ldy, int64_t m, int n, int k, int act,
+                     int32_t* status);
+
 // options
 int option_force_simt();
 int option_shrink_cluster();

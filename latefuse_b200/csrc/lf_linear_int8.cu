@@ -24,7 +24,9 @@
 // tiles would leave most SMs without work: w's rows are the MMA's M (128 channels per
 // CTA), the tokens its N (16 to 128), and K is split over a cluster of up to 8 CTAs whose
 // integer partial sums meet in distributed shared memory (each CTA finishes a share of
-// the tokens).  Integer addition is exact, so the split changes no bit.
+// the tokens).  Integer addition is exact, so the split changes no bit.  Up to 16 float rows
+// of up to 4,096 are quantised in the same launch, by the warps that finish later on: a
+// launch of their own takes the host 2 us and a workspace.
 //
 // Every wait is bounded: a timeout sets LF_STATUS_TIMEOUT and the roles unwind.
 #include <cstring>
@@ -32,6 +34,7 @@
 #include "lf_common.cuh"
 #include "lf_internal.h"
 #include "lf_pair.cuh"
+#include "lf_quant.cuh"
 
 namespace lf {
 
@@ -53,6 +56,10 @@ struct alignas(64) LinearInt8Params {
   int32_t tma_out;    // y's base and row stride are 16-byte aligned
   int32_t vec_ch;     // w_scale and bias are aligned for pairs
   int32_t split;      // split kernel: CTAs of the cluster that share a tile's K
+  const void* rows;   // float rows, quantised on chip (m_rows <= kRowsM), or null
+  int64_t ld_rows;
+  int32_t k;
+  int32_t vec_rows;   // they are aligned for 8 elements a load
   int32_t* status;
 };
 
@@ -455,6 +462,10 @@ __host__ __device__ constexpr int split_stages(int nt) { return nt <= 32 ? 8 : 6
 __host__ __device__ constexpr int split_stage_bytes(int nt) { return 128 * kBK + nt * kBK; }
 constexpr int split_smem_bytes(int nt) { return 1024 + split_stages(nt) * split_stage_bytes(nt) + 512; }
 static_assert(split_smem_bytes(128) <= 232448 && split_smem_bytes(32) <= 232448, "shared memory");
+// float rows: up to 16 of 4,096, whose integers (NT x 128 bytes a K block) stay beside the ring
+constexpr int kRowsM = 16, kRowsK = 4096;
+constexpr int rows_smem_bytes() { return split_smem_bytes(kRowsM) + kRowsM * kRowsK; }
+static_assert(rows_smem_bytes() <= 232448, "shared memory");
 // the partial sums (NT x 128 int32) reuse the ring
 static_assert(128 * 128 * 4 <= 6 * split_stage_bytes(128) && 16 * 128 * 4 <= 8 * split_stage_bytes(16), "ring");
 
@@ -467,9 +478,58 @@ __device__ __forceinline__ int4 ld_dsmem_i4(uint32_t addr) {
   return v;
 }
 
-template <typename T, int NT, int kAct>
+// kRows, the finishing warps before the product: p.rows' scales, and their integers of this
+// CTA's K blocks [kb0, kb1) in the layout that a TMA load of them would have (K-major SW128,
+// NT rows a block).  Every CTA finds the rows' largest magnitudes for itself, from L2.
+template <typename T, bool VEC>
+__device__ __forceinline__ void quantize_share(const LinearInt8Params& p, uint8_t* blocks, uint32_t* s_top, float* s_scale,
+                                               int kb0, int kb1, int w, int lane) {
+  const int m = int(p.m_rows), share = m <= 1 ? 8 : m <= 2 ? 4 : m <= 4 ? 2 : 1;  // warps a row
+  const T* x = static_cast<const T*>(p.rows);
+  for (int r = w / share; r < m; r += kSplitEpiWarps / share) {
+    uint32_t top = 0;
+    for (int32_t base = (w % share) * 256; base < p.k; base += 4 * share * 256) {
+      QuantChunk<T, VEC> c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i].load(x + r * p.ld_rows, base + i * share * 256, lane, p.k);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = sizeof(T) == 2 ? __vmaxu2(top, c[i].top()) : max(top, c[i].top());
+    }
+    if constexpr (sizeof(T) == 2) top = max(top >> 16, top & 0xffffu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) atomicMax(&s_top[r], top);
+  }
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * kSplitEpiWarps) : "memory");  // every row's largest magnitude is known
+  const int chunks = (kb1 - kb0 + 1) / 2;
+  for (int r = w / share; r < m; r += kSplitEpiWarps / share) {
+    const RowQuant rq(top_bits<T>(s_top[r]));
+    if (lane == 0 && w % share == 0) s_scale[r] = rq.scale;
+    uint8_t* row = blocks + (r >> 3) * 1024 + (r & 7) * 128;
+    for (int c = w % share; c < chunks; c += share) {
+      QuantChunk<T, VEC> v;
+      v.load(x + r * p.ld_rows, kb0 * kBK + c * 256, lane, p.k);
+      const uint2 q = v.steps(rq);
+      if constexpr (VEC) {  // bytes 8 l .. 8 l + 7 of two blocks, 16 lanes a block
+        const int kb = 2 * c + (lane >> 4), piece = (lane & 15) >> 1;
+        if (kb < kb1 - kb0)
+          *reinterpret_cast<uint2*>(row + kb * (kRowsM * kBK) + ((piece ^ (r & 7)) << 4) + (lane & 1) * 8) = q;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int at = i * 32 + lane, kb = 2 * c + (at >> 7), piece = (at & 127) >> 4;
+          if (kb < kb1 - kb0)
+            row[kb * (kRowsM * kBK) + ((piece ^ (r & 7)) << 4) + (at & 15)] =
+                uint8_t((i < 4 ? q.x >> (8 * i) : q.y >> (8 * (i - 4))) & 0xffu);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int NT, int kAct, bool kRows>
 __global__ void __launch_bounds__(kSplitThreads, 1) linear_int8_split_kernel(const __grid_constant__ LinearInt8Params p) {
   constexpr int kSt = split_stages(NT), kSb = split_stage_bytes(NT);
+  constexpr int kLoad = kRows ? 128 * kBK : kSb;  // bytes that arrive in a stage
   constexpr uint32_t kTmemCols = NT < 32 ? 32 : NT;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -482,22 +542,27 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_int8_split_kernel(con
   const int64_t m0 = int64_t(blockIdx.y) * NT;
   const int kb0 = int(int64_t(p.n_kb) * rank / S), kb1 = int(int64_t(p.n_kb) * (rank + 1) / S);
 
-  uint64_t* bars = reinterpret_cast<uint64_t*>(gbase + kSt * kSb);
+  uint8_t* blocks = gbase + kSt * kSb;  // kRows: the rows' integers
+  uint64_t* bars = reinterpret_cast<uint64_t*>(blocks + (kRows ? kRowsM * kRowsK : 0));
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  constexpr int FULL = 0, EMPTY = kSt, ACC = 2 * kSt, N_BARS = ACC + 1;
+  constexpr int FULL = 0, EMPTY = kSt, ACC = 2 * kSt, ROWS = ACC + 1, N_BARS = ROWS + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(&bars[N_BARS]);
   int32_t* s_abort = reinterpret_cast<int32_t*>(tmem_slot + 1);
+  uint32_t* s_top = tmem_slot + 2;
+  float* s_scale = reinterpret_cast<float*>(s_top + kRowsM);
   if (tid == 0) {
     for (int i = 0; i < kSt; ++i) {
       mbar_init(bar(FULL + i), 1);
       mbar_init(bar(EMPTY + i), 1);
     }
     mbar_init(bar(ACC), 1);
+    mbar_init(bar(ROWS), kSplitEpiWarps);
     *s_abort = 0;
     fence_mbar_init();
-    prefetch_tmap(&p.x_map);
+    if constexpr (!kRows) prefetch_tmap(&p.x_map);
     prefetch_tmap(&p.w_map);
   }
+  if (kRows && warp == 2 && lane < kRowsM) s_top[lane] = 0;
   if (warp == 1) {
     __syncwarp();
     tmem_alloc(smem_u32(tmem_slot), kTmemCols);
@@ -515,9 +580,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_int8_split_kernel(con
       if (!warp_wait(bar(EMPTY + s), ((kk / kSt) & 1) ^ 1, s_abort, p.status)) break;
       if (elect_one()) {
         const uint32_t st = base + s * kSb;
-        mbar_arrive_expect_tx(bar(FULL + s), kSb);
+        mbar_arrive_expect_tx(bar(FULL + s), kLoad);
         tma_load_2d(st, &p.w_map, bar(FULL + s), kb * kBK, n0);
-        tma_load_2d(st + 128 * kBK, &p.x_map, bar(FULL + s), kb * kBK, int32_t(m0));
+        if constexpr (!kRows) tma_load_2d(st + 128 * kBK, &p.x_map, bar(FULL + s), kb * kBK, int32_t(m0));
       }
       __syncwarp();
     }
@@ -526,17 +591,21 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_int8_split_kernel(con
     __syncwarp();
   } else if (warp == 1) {
     constexpr uint32_t idesc = umma_idesc_i8(128, NT);
-    const uint64_t a_desc = smem_desc(base, 16, 1024, 2), b_desc = smem_desc(base + 128 * kBK, 16, 1024, 2);
+    const uint64_t a_desc = smem_desc(base, 16, 1024, 2);
+    const uint64_t b_desc = smem_desc(kRows ? smem_u32(blocks) : base + 128 * kBK, 16, 1024, 2);
     int kk = 0;
-    for (int kb = kb0; kb < kb1; ++kb, ++kk) {
+    bool go = true;
+    if constexpr (kRows) go = warp_wait(bar(ROWS), 0, s_abort, p.status);
+    for (int kb = kb0; go && kb < kb1; ++kb, ++kk) {
       const int s = kk % kSt;
       if (!warp_wait(bar(FULL + s), (kk / kSt) & 1, s_abort, p.status)) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t off = uint64_t(s * (kSb >> 4));
+        const uint64_t a = a_desc + uint64_t(s * (kSb >> 4));
+        const uint64_t b = b_desc + uint64_t(kRows ? kk * (kRowsM * kBK >> 4) : s * (kSb >> 4));
 #pragma unroll
         for (int q = 0; q < kBK / 32; ++q)
-          umma_i8(tmem, a_desc + off + uint64_t(2 * q), b_desc + off + uint64_t(2 * q), idesc, (kk | q) != 0 ? 1u : 0u);
+          umma_i8(tmem, a + uint64_t(2 * q), b + uint64_t(2 * q), idesc, (kk | q) != 0 ? 1u : 0u);
         umma_commit(bar(EMPTY + s));
       }
       __syncwarp();
@@ -544,6 +613,13 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_int8_split_kernel(con
     if (elect_one()) umma_commit(bar(ACC));  // also when unwinding: every issued MMA finishes before TMEM is released
     __syncwarp();
   } else {
+    if constexpr (kRows) {
+      if (p.vec_rows) quantize_share<T, true>(p, blocks, s_top, s_scale, kb0, kb1, warp - 2, lane);
+      else quantize_share<T, false>(p, blocks, s_top, s_scale, kb0, kb1, warp - 2, lane);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(ROWS));
+    }
     // the CTA's partial sums, (token, channel) int32, into the ring once every MMA has read it
     const int quad = warp & 3, half = (warp - 2) >> 2;
     if (warp_wait(bar(ACC), 0, s_abort, p.status)) {
@@ -592,7 +668,14 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_int8_split_kernel(con
           if (two) v[1][r] = ld_dsmem_i4(part[r] + uint32_t(t2) * 512u);
         }
       }
-      const float xs[2] = {__ldg(p.x_scale + m0 + t), two ? __ldg(p.x_scale + m0 + t2) : 0.f};
+      float xs[2];
+      if constexpr (kRows) {
+        xs[0] = s_scale[t];
+        xs[1] = two ? s_scale[t2] : 0.f;
+      } else {
+        xs[0] = __ldg(p.x_scale + m0 + t);
+        xs[1] = two ? __ldg(p.x_scale + m0 + t2) : 0.f;
+      }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         if (k == 1 && !two) break;
@@ -682,17 +765,19 @@ int launch_batch(LinearInt8Params& p, int dev, cudaStream_t s) {
                                                      2, dev, s, p);
 }
 
-template <typename T, int NT, int kAct>
+template <typename T, int NT, int kAct, bool kRows = false>
 int launch_split(LinearInt8Params& p, int dev, cudaStream_t s) {
   p.n_tiles_n = (p.n + 127) / 128;
   const dim3 grid(unsigned(p.n_tiles_n) * unsigned(p.split), unsigned((p.m_rows + NT - 1) / NT));
-  return launch_cluster<linear_int8_split_kernel<T, NT, kAct>>("launch linear_int8_split", grid, kSplitThreads,
-                                                               split_smem_bytes(NT), p.split, dev, s, p);
+  return launch_cluster<linear_int8_split_kernel<T, NT, kAct, kRows>>("launch linear_int8_split", grid, kSplitThreads,
+                                                                      kRows ? rows_smem_bytes() : split_smem_bytes(NT),
+                                                                      p.split, dev, s, p);
 }
 
 template <typename T, int kAct>
 int launch(LinearInt8Params& p, bool batch, int nt, int dev, cudaStream_t s) {
   if (batch) return launch_batch<T, kAct>(p, dev, s);
+  if (p.rows != nullptr) return launch_split<T, kRowsM, kAct, true>(p, dev, s);
   if (nt == 16) return launch_split<T, 16, kAct>(p, dev, s);
   if (nt == 32) return launch_split<T, 32, kAct>(p, dev, s);
   if (nt == 64) return launch_split<T, 64, kAct>(p, dev, s);
@@ -705,10 +790,12 @@ int launch(LinearInt8Params& p, bool batch, int nt, int dev, cudaStream_t s) {
 
 using namespace lf;
 
-extern "C" int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t ldx, const float* x_scale,
-                              const int8_t* w, int64_t ldw, const float* w_scale, const void* bias, void* y,
-                              int64_t ldy, int64_t m, int n, int k, int act, int32_t* status) {
-  const char* fn = "lf_linear_int8";
+namespace {
+
+// x in 8-bit integers with x_scale, or (float_rows) rows of dtype that one launch quantises too.
+int run(const char* fn, void* stream, int dtype, const void* x, int64_t ldx, const float* x_scale, bool float_rows,
+        const int8_t* w, int64_t ldw, const float* w_scale, const void* bias, void* y, int64_t ldy, int64_t m, int n,
+        int k, int act, int32_t* status) {
   if (dtype != LF_DTYPE_BF16 && dtype != LF_DTYPE_F16 && dtype != LF_DTYPE_F32)
     return set_error(LF_ERR_INVALID, "%s: unknown dtype %d", fn, dtype);
   if (act != LF_ACT_NONE && act != LF_ACT_GELU) return set_error(LF_ERR_INVALID, "%s: unknown act %d", fn, act);
@@ -716,11 +803,11 @@ extern "C" int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t 
     return set_error(LF_ERR_INVALID, "%s: m %lld, n %d, k %d", fn, (long long)m, n, k);
   if (k > 131072) return set_error(LF_ERR_UNSUPPORTED, "%s: k %d above 131072 (the sum could leave 32 bits)", fn, k);
   if (m == 0) return LF_OK;
-  if (x == nullptr || x_scale == nullptr || w == nullptr || w_scale == nullptr || y == nullptr)
+  if (x == nullptr || (x_scale == nullptr && !float_rows) || w == nullptr || w_scale == nullptr || y == nullptr)
     return set_error(LF_ERR_INVALID, "%s: null x, w, scales or y", fn);
   if (ldx < k || ldw < k || ldy < n) return set_error(LF_ERR_INVALID, "%s: a row stride is below its row", fn);
-  if (!aligned16(x) || !aligned16(w) || ldx % 16 != 0 || ldw % 16 != 0)
-    return set_error(LF_ERR_INVALID, "%s: x and w need 16-byte aligned rows", fn);
+  if (!aligned16(w) || ldw % 16 != 0 || (!float_rows && (!aligned16(x) || ldx % 16 != 0)))
+    return set_error(LF_ERR_INVALID, "%s: 8-bit x and w need 16-byte aligned rows", fn);
   const int es = dtype == LF_DTYPE_F32 ? 4 : 2;
   LinearInt8Params p;
   memset(&p, 0, sizeof(p));
@@ -735,16 +822,25 @@ extern "C" int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t 
   p.tma_out = aligned16(y) && (ldy * es) % 16 == 0 ? 1 : 0;
   p.vec_ch = (reinterpret_cast<uintptr_t>(w_scale) & 7u) == 0 && (reinterpret_cast<uintptr_t>(bias) & (2u * es - 1u)) == 0;
   p.status = status;
+  if (float_rows) {
+    p.rows = x;
+    p.ld_rows = ldx;
+    p.k = k;
+    p.vec_rows = k % 8 == 0 && aligned16(x) && (ldx * es) % 16 == 0;
+  }
 
-  // 256 x 256 tiles once a quarter as many as SMs; below that 128 channels x nt tokens.
+  // 256 x 256 tiles once a quarter as many as SMs, unless few tokens leave them mostly empty
+  // and 128 channels a CTA still find an SM each; below that 128 channels x nt tokens.
   // Measured with the few-token kernel and with the other (us, bf16, no activation):
   //   n 1,024, k 4,096: 512 tokens (8 tiles) 14.3 and 20.5; 2,048 (32) 18.5 and 20.5;
   //     3,000 (48) 32.8 and 20.5
   //   n 4,096, k 1,024: 256 tokens (16) 12.3 both; 512 (32) 14.3 both; 1,024 (64) 24.6 and 14.3
-  //   n 10,240, k 2,560: 128 tokens (40) 18.4 and 16.4; 256 (40) 26.6 and 16.4
+  //   n 10,240, k 2,560: 256 tokens (40) 26.6 and 16.4
+  // and without launch: n 10,240, k 2,560: 16 tokens 8.4 and 12.8, 64 10.0 and 11.1, 128 11.6 and
+  // 11.4; n 40,960: 64 tokens 32.9 and 25.6
   const int dev = current_device(), sms = device_sms(dev);
   const int64_t big = ((m + 255) / 256) * ((n + 255) / 256);
-  const bool batch = big > sms / 4;
+  const bool batch = big > sms / 4 && !(m <= 64 && (n + 127) / 128 <= sms) && !float_rows;
   const int nt = batch ? 128 : m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
   p.split = 1;
   if (!batch) {
@@ -756,7 +852,8 @@ extern "C" int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t 
     for (int i = 0; i < 3 && tiles * p.split * 2 <= room[i] && p.split * 2 <= p.n_kb; ++i) p.split *= 2;
   }
   int rc;
-  if ((rc = encode(&p.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, k, m, ldx, kBK, nt, CU_TENSOR_MAP_SWIZZLE_128B, "x")))
+  if (!float_rows &&
+      (rc = encode(&p.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, k, m, ldx, kBK, nt, CU_TENSOR_MAP_SWIZZLE_128B, "x")))
     return rc;
   if ((rc = encode(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, k, n, ldw, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B, "w")))
     return rc;
@@ -776,4 +873,27 @@ extern "C" int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t 
   if (dtype == LF_DTYPE_BF16) return go(__nv_bfloat16{});
   if (dtype == LF_DTYPE_F16) return go(__half{});
   return go(float{});
+}
+
+}  // namespace
+
+namespace lf {
+
+// One launch or two, GPU time of calls in a row (us, bf16, n 1,024; a launch saves the host
+// 4.5 us besides): k 1,024: 1 row 4.4 and 5.0, 8 4.7 and 5.1, 16 5.6 and 5.1; k 4,096: 1 row 4.9
+// and 5.1, 4 5.4 and 5.4, 8 6.2 and 5.4, 16 8.2 and 5.5 (every CTA reads all rows).
+bool linear_int8_takes_rows(int64_t m, int k) { return m <= kRowsM && k <= kRowsK && m * k <= 16384; }
+
+int linear_int8_rows(void* stream, int dtype, const void* x, int64_t ldx, const int8_t* w, int64_t ldw,
+                     const float* w_scale, const void* bias, void* y, int64_t ldy, int64_t m, int n, int k, int act,
+                     int32_t* status) {
+  return run("lf_linear_rows_int8", stream, dtype, x, ldx, nullptr, true, w, ldw, w_scale, bias, y, ldy, m, n, k, act, status);
+}
+
+}  // namespace lf
+
+extern "C" int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t ldx, const float* x_scale,
+                              const int8_t* w, int64_t ldw, const float* w_scale, const void* bias, void* y,
+                              int64_t ldy, int64_t m, int n, int k, int act, int32_t* status) {
+  return run("lf_linear_int8", stream, dtype, x, ldx, x_scale, false, w, ldw, w_scale, bias, y, ldy, m, n, k, act, status);
 }

@@ -105,4 +105,84 @@ struct RowQuant {
   }
 };
 
+// A lane's 8 elements of a 256-element chunk: neighbours (VEC), kept as they lie in memory
+// until they are rounded, or 32 apart.  Elements past the row read as 0.
+template <typename T, bool VEC>
+struct QuantChunk {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* row, int32_t base, int lane, int32_t cols) {
+    if constexpr (VEC) {
+      const int32_t col = base + lane * 8;
+#pragma unroll
+      for (int i = 0; i < int(sizeof(T)) / 2; ++i)
+        w[i] = col < cols ? __ldg(reinterpret_cast<const uint4*>(row + col) + i) : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      T e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int32_t col = base + i * 32 + lane;
+        e[i] = col < cols ? row[col] : DT<T>::from_f(0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < int(sizeof(T)) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(e)[i];
+    }
+  }
+  // the largest magnitude as an integer that orders like it: two 16-bit halves, or 32 bits
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
+      const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 2) t = __vmaxu2(t, u[k] & 0x7fff7fffu);
+        else t = max(t, u[k] & 0x7fffffffu);
+      }
+    }
+    return t;
+  }
+  // the eight steps, the lane's first element in the low byte of x
+  __device__ __forceinline__ uint2 steps(const RowQuant& rq) const {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
+      const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 2) {
+          const float2 f = Pack2<T>::unpack(u[k]);
+          v[2 * k] = f.x;
+          v[2 * k + 1] = f.y;
+        } else {
+          v[4 * i + k] = __uint_as_float(u[k]);
+        }
+      }
+    }
+    return rq.template q8<T>(v);
+  }
+  __device__ __forceinline__ void store(int8_t* row, int32_t base, int lane, int32_t cols, const RowQuant& rq) const {
+    const uint2 q = steps(rq);
+    if constexpr (VEC) {
+      const int32_t col = base + lane * 8;
+      if (col < cols) *reinterpret_cast<uint2*>(row + col) = q;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int32_t col = base + i * 32 + lane;
+        if (col < cols) row[col] = int8_t((i < 4 ? q.x >> (8 * i) : q.y >> (8 * (i - 4))) & 0xffu);
+      }
+    }
+  }
+};
+
+// The f32 bits of a magnitude given by its type's bits.
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(uint32_t t) {
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t h = uint16_t(t);
+    return __float_as_uint(DT<T>::to_f(*reinterpret_cast<const T*>(&h)));
+  }
+  return t;
+}
+
 }  // namespace lf

@@ -132,7 +132,7 @@ def cross_attention_varlen(q: Tensor, k: Tensor, v: Tensor, batch: CrossBatch, n
     if batch.n_q > tq or batch.n_kv > tk:
         raise ValueError(f"the batch names {batch.n_q} query and {batch.n_kv} key rows, q has {tq} and k {tk}")
     if out is None:
-        out = torch.empty(tq, width, dtype=dtype, device=dev)
+        out = q.new_empty((tq, width))
     elif out.dtype != dtype or out.shape != q.shape:
         raise ValueError(f"out must be a ({tq}, {width}) {dtype} tensor with contiguous rows")
     nat.call(nat.lib().lf_cross_attention_varlen, "lf_cross_attention_varlen", dev, nat.dtype_code(dtype), q.data_ptr(),

@@ -29,6 +29,10 @@ def _padded(n: int) -> int:
     return (n + 15) // 16 * 16
 
 
+def _up256(n: int) -> int:
+    return (n + 255) // 256 * 256
+
+
 def _rows(t: Tensor) -> tuple[Tensor, int]:
     """``t`` as rows of its last dimension, each contiguous and at least a row apart, and
     their stride."""
@@ -131,7 +135,7 @@ def linear_int8(x: Tensor | Int8Rows, weight: Int8Weight, bias: Tensor | None = 
         x2, ldx = _rows(x)
         m = x2.shape[0]
     if out is None:
-        out = torch.empty(m, n, dtype=dtype, device=dev)
+        out = torch.empty(m, n, dtype=dtype, device=dev) if rows else x.new_empty((m, n))
         ldo, ret = n, out if len(shape) == 2 else out.view(*shape[:-1], n)
     else:
         o2 = out.reshape(-1, n)
@@ -146,14 +150,20 @@ def linear_int8(x: Tensor | Int8Rows, weight: Int8Weight, bias: Tensor | None = 
                  weight.q.data_ptr(), weight.ld, weight.scale.data_ptr(), b, out.data_ptr(), ldo, m, n, k, int(act), None)
     else:
         size = _rows_bytes(m, k)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         nat.call(nat.lib().lf_linear_rows_int8, "lf_linear_rows_int8", dev, code, x2.data_ptr(), ldx, weight.q.data_ptr(),
-                 weight.ld, weight.scale.data_ptr(), b, out.data_ptr(), ldo, m, n, k, int(act), ws.data_ptr(), size, None)
+                 weight.ld, weight.scale.data_ptr(), b, out.data_ptr(), ldo, m, n, k, int(act), nat.ptr(ws), size, None)
     return ret
 
 
 def _rows_bytes(m: int, k: int) -> int:
-    return nat.lib().lf_linear_rows_int8_workspace_bytes(m, k)
+    """``lf_linear_rows_int8_workspace_bytes``, without the call."""
+    return 0 if m <= 16 and k <= 4096 and m * k <= 16384 else _up256(m * _padded(k)) + _up256(4 * m)
+
+
+def _ffn_bytes(size: int, m: int, hidden: int, inner: int) -> int:
+    """``lf_ffn_int8_workspace_bytes``, without the call, for elements of ``size`` bytes."""
+    return _up256(m * _padded(hidden)) + _up256(m * _padded(inner)) + 2 * _up256(4 * m) + _up256(m * _padded(inner) * size)
 
 
 def add_layernorm_int8(a: Tensor, b: Tensor | None, weight: Tensor, bias: Tensor, eps: float) -> tuple[Tensor, Int8Rows]:
@@ -198,9 +208,9 @@ def ffn_int8(a: Tensor, residual: Tensor | None, ln_weight: Tensor, ln_bias: Ten
     m = a2.shape[0]
     w, bb = _bias(ln_weight, hidden, dtype), _bias(ln_bias, hidden, dtype)
     ub, db = _bias(up_bias, inner, dtype), _bias(down_bias, hidden, dtype)
-    h, o = (torch.empty(m, hidden, dtype=dtype, device=dev) for _ in range(2))
+    h, o = a2.new_empty((m, hidden)), a2.new_empty((m, hidden))
     lib, code = nat.lib(), nat.dtype_code(dtype)
-    size = lib.lf_ffn_int8_workspace_bytes(code, m, hidden, inner)
+    size = _ffn_bytes(dtype.itemsize, m, hidden, inner)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     nat.call(lib.lf_ffn_int8, "lf_ffn_int8", dev, code, a2.data_ptr(), lda, nat.ptr(r2), ldr, w.data_ptr(), bb.data_ptr(),
              float(eps), up.q.data_ptr(), up.ld, up.scale.data_ptr(), nat.ptr(ub), down.q.data_ptr(), down.ld,

@@ -155,6 +155,39 @@ def test_linear_int8_matches_the_formula(cuda, dtype, m, n, k):
             check_projection(y, q, xs, w, ws, bias, act)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 1024, 1024), (2, 130, 100), (3, 257, 4095), (4, 128, 129), (5, 3000, 2568),
+                                   (8, 96, 1040), (9, 12000, 264), (15, 64, 1023), (16, 512, 1024), (4, 40, 4096), (16, 1, 255)])
+def test_few_float_rows_are_their_quantised_rows(cuda, dtype, m, n, k):
+    """Up to 16 float rows of up to 16,384 elements in all, quantised inside the projection's launch, give
+    what quantize_rows and the projection of its rows give, bit for bit: the same integers,
+    scales and f32 operations.  Contiguous rows, and rows of a wider buffer from an odd column
+    on (an element a load)."""
+    g = torch.Generator(cuda).manual_seed(m * n + k)
+    wide = torch.randn(m, k + 7, device=cuda, generator=g).to(dtype)
+    w = Int8Weight.from_float(torch.randn(n, k, device=cuda, generator=g))
+    bias = torch.randn(n, device=cuda, generator=g).to(dtype)
+    for x in (wide[:, 3:3 + k].contiguous(), wide[:, 3:3 + k], wide[:, :k]):
+        for act in (0, 1):
+            before = nat.launch_count()
+            y = linear_int8(x, w, bias, act=act)
+            assert nat.launch_count() == before + 1
+            assert torch.equal(y, linear_int8(quantize_rows(x), w, bias, act=act))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_float_rows_that_are_not_finite(cuda, dtype):
+    x = torch.randn(6, 520, device=cuda).to(dtype)
+    x[1] = 0
+    x[2, 519] = float("inf")
+    x[4, 0] = float("nan")
+    w = Int8Weight.from_float(torch.randn(300, 520, device=cuda))
+    y = linear_int8(x, w)
+    assert y[[2, 4]].isnan().all() and (y[1] == 0).all() and y[[0, 3, 5]].isfinite().all()
+    keep = [0, 3, 5]
+    assert torch.equal(y[keep], linear_int8(x[keep], w))
+
+
 def test_rows_do_not_depend_on_their_batch(cuda):
     """The integer sum is exact, so a row's result is the same bits alone, in a small batch
     (the split kernel) and in a large one (the CTA-pair kernel)."""

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import latefuse_b200 as lf
-from latefuse_b200 import _native as nat
+from latefuse_b200 import _native as nat, int8_ops
 from latefuse_b200._build import build
 
 INVALID, UNSUPPORTED, WORKSPACE = 1, 2, 4
@@ -65,11 +65,26 @@ def test_linear_int8_refusals(lib, addr):
 
 
 def test_workspace_entries(lib, addr):
-    need = lib.lf_linear_rows_int8_workspace_bytes(4, 100)
-    assert need == 512 + 256  # four rows of 112 bytes, four scales, each to 256 bytes
+    need = lib.lf_linear_rows_int8_workspace_bytes(17, 100)
+    assert need == 2048 + 256  # 17 rows of 112 bytes, 17 scales, each to 256 bytes
     assert lib.lf_linear_rows_int8_workspace_bytes(4, 131073) == 0
-    g = lambda ws, size, dtype=1, k=100: lib.lf_linear_rows_int8(None, dtype, addr, 100, addr, 112, addr, None, addr, 32, 4, 32,
+    assert lib.lf_linear_rows_int8_workspace_bytes(4, 4096) == 0  # one launch, no workspace
+    for m in (0, 1, 4, 5, 16, 17, 100, 70001):
+        for k in (1, 16, 100, 1024, 1025, 4096, 4097, 131072):
+            assert int8_ops._rows_bytes(m, k) == lib.lf_linear_rows_int8_workspace_bytes(m, k)
+            for code, size in ((0, 4), (1, 2), (2, 2)):
+                assert int8_ops._ffn_bytes(size, m, 264, k) == lib.lf_ffn_int8_workspace_bytes(code, m, 264, k)
+    g = lambda ws, size, dtype=1, k=100: lib.lf_linear_rows_int8(None, dtype, addr, 100, addr, 112, addr, None, addr, 32, 17, 32,
                                                                  k, 0, ws, size, None)
+    one = lambda dtype=1, x=addr, ldx=100, w=addr, ldw=112, scale=addr, act=0, n=32: lib.lf_linear_rows_int8(
+        None, dtype, x, ldx, w, ldw, scale, None, addr, 32, 4, n, 100, act, None, 0, None)
+    refused(lib, one(dtype=7), INVALID, "dtype")
+    refused(lib, one(x=None), INVALID, "null")
+    refused(lib, one(scale=None), INVALID, "null")
+    refused(lib, one(ldx=99), INVALID, "stride")
+    refused(lib, one(w=addr + 8), INVALID, "16-byte")
+    refused(lib, one(act=9), INVALID, "act")
+    refused(lib, one(n=0), INVALID, "n 0")
     refused(lib, g(addr, need - 1), WORKSPACE, "workspace")
     refused(lib, g(None, need), WORKSPACE, "workspace")
     refused(lib, g(addr + 16, need), WORKSPACE, "aligned")
