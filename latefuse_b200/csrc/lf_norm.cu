@@ -102,11 +102,18 @@ __device__ __forceinline__ float warp_sum(float v) {
 
 constexpr int kNormWarps = 8;
 
+// CTAs an SM that the kernel's registers are kept to (0: the compiler's own choice).  With
+// QUANT at 16 bits the rounding's temporaries cost occupancy that the row's loads need, and
+// late gamma and beta cost less than their registers: 17,410 rows of 1,024 30.6 us against
+// 34.8 with neither, 16,384 of 2,048 47 against 78, of 2,560 61 against 70, of 4,096 137
+// against 148.
+constexpr int norm_ctas(int es, int nc, bool quant) { return !quant || es != 2 ? 0 : nc <= 4 ? 4 : nc <= 8 ? 3 : 2; }
+
 // MODE 0: a alone; 1: a + b (a second matrix); 2: a + v (one row vector); 3: the
 // embeddings, round(round(a[ia] + c[ic]) + b[ib]) of gathered table rows (the
 // encoder's word + token type, then + position, each sum rounded as torch rounds it).
 template <typename T, int NC, int MODE, bool QUANT = false>
-__global__ void __launch_bounds__(32 * kNormWarps)
+__global__ void __launch_bounds__(32 * kNormWarps, norm_ctas(sizeof(T), NC, QUANT))
 add_layernorm_kernel(const NormParams p, int full) {
   constexpr bool HAS_B = MODE != 0;
   pdl_wait();
@@ -149,9 +156,21 @@ add_layernorm_kernel(const NormParams p, int full) {
   }
   // gamma and beta too, so that their latency overlaps the reductions instead
   // of following them (rows up to 2048 wide; wider rows load them at the end,
-  // where the registers are free)
-  constexpr bool kEarly = NC <= 8;
+  // where the registers are free; with QUANT from 768 on, brought to L2 by the CTA's first warp)
+  constexpr bool kEarly = NC <= (QUANT ? 3 : 8);
   Raw8<T> g[kEarly ? NC : 1], bt[kEarly ? NC : 1];
+  if constexpr (QUANT && !kEarly) {
+    if (threadIdx.x < 32) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int col = c * 256 + lane * 8;
+        if (full || col < H) {
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(gamma + col));
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(beta + col));
+        }
+      }
+    }
+  }
   if constexpr (kEarly) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -198,6 +217,7 @@ add_layernorm_kernel(const NormParams p, int full) {
     }
   }
   const float rstd = rsqrtf(warp_sum(sq) / float(H) + p.eps);
+  QuantChunk<T, true> oc[QUANT ? NC : 1];  // the rounded row
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int col = c * 256 + lane * 8;
@@ -212,10 +232,12 @@ add_layernorm_kernel(const NormParams p, int full) {
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = (v[c][i] - mean) * rstd * gf[i] + bf[i];
-      Vec8<T>::store(out + col, o);
       if constexpr (QUANT) {
+        oc[c].set(o);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[c][i] = round_through<T>(o[i]);
+        for (int i = 0; i < int(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(out + col)[i] = oc[c].w[i];
+      } else {
+        Vec8<T>::store(out + col, o);
       }
     }
   }
@@ -223,17 +245,15 @@ add_layernorm_kernel(const NormParams p, int full) {
     uint32_t top = 0;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
-      if (full || c * 256 + lane * 8 < H) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, mag_bits(v[c][i]));
-      }
-    const RowQuant rq(__reduce_max_sync(0xffffffffu, top));
+      if (full || c * 256 + lane * 8 < H) top = sizeof(T) == 2 ? __vmaxu2(top, oc[c].top()) : max(top, oc[c].top());
+    if constexpr (sizeof(T) == 2) top = max(top >> 16, top & 0xffffu);
+    const RowQuant rq(top_bits<T>(__reduce_max_sync(0xffffffffu, top)));
     if (lane == 0) p.q_scale[row] = rq.scale;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = c * 256 + lane * 8;
       if (full || col < H) {
-        *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) = rq.q8<T>(v[c]);
+        *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) = oc[c].steps(rq);
       }
     }
   }

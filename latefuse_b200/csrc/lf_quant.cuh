@@ -127,6 +127,18 @@ struct QuantChunk {
       for (int i = 0; i < int(sizeof(T)) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(e)[i];
     }
   }
+  // eight values, rounded to T
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
+      if constexpr (sizeof(T) == 2)
+        w[i] = make_uint4(Pack2<T>::pack(v[0], v[1]), Pack2<T>::pack(v[2], v[3]), Pack2<T>::pack(v[4], v[5]),
+                          Pack2<T>::pack(v[6], v[7]));
+      else
+        w[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                          __float_as_uint(v[4 * i + 3]));
+    }
+  }
   // the largest magnitude as an integer that orders like it: two 16-bit halves, or 32 bits
   __device__ __forceinline__ uint32_t top() const {
     uint32_t t = 0;
