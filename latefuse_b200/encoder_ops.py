@@ -117,7 +117,8 @@ def cross_attention_varlen(q: Tensor, k: Tensor, v: Tensor, batch: CrossBatch, n
     fine); d a multiple of 8 up to 128; consecutive ``n_heads / n_kv_heads`` query heads
     share a key head (``n_kv_heads`` None: as many as ``n_heads``); ``scale`` positive, None:
     ``d ** -0.5``.  A sequence without keys gives zeros; rows of ``out`` in no sequence are
-    left as they were (undefined when ``out`` is None).  Returns ``out (Tq, n_heads * d)``."""
+    left as they were (undefined when ``out`` is None); ``out`` must not overlap q, k or v.
+    Returns ``out (Tq, n_heads * d)``."""
     items, dtype = batch.items, q.dtype
     dev = nat.require_cuda(q, k, v, items, out, status)
     n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
@@ -135,11 +136,33 @@ def cross_attention_varlen(q: Tensor, k: Tensor, v: Tensor, batch: CrossBatch, n
         out = q.new_empty((tq, width))
     elif out.dtype != dtype or out.shape != q.shape:
         raise ValueError(f"out must be a ({tq}, {width}) {dtype} tensor with contiguous rows")
+    elif _share_memory(out, q) or _share_memory(out, k) or _share_memory(out, v):
+        raise ValueError("out must not overlap q, k or v")
     nat.call(nat.lib().lf_cross_attention_varlen, "lf_cross_attention_varlen", dev, nat.dtype_code(dtype), q.data_ptr(),
              _ld(q, tq, width), tq, k.data_ptr(), _ld(k, tk, wk), v.data_ptr(), _ld(v, tk, wk), tk, n_heads, n_kv_heads, d,
              items.data_ptr(), items.shape[0], batch.max_q, batch.max_kv, d ** -0.5 if scale is None else float(scale),
              out.data_ptr(), _ld(out, tq, width), nat.ptr(status))
     return out
+
+
+def _share_memory(a: Tensor, b: Tensor) -> bool:
+    """Whether two matrices of contiguous rows have bytes in common.  Column ranges of rows
+    of one stride (slices of a fused buffer) have none where the columns differ; of other
+    strides, any that lie in each other's range count."""
+    (ra, ca), (rb, cb) = a.shape, b.shape
+    if not (ra and ca and rb and cb):
+        return False
+    wa, wb = ca * a.element_size(), cb * b.element_size()
+    la = a.stride(0) * a.element_size() if ra > 1 else wa
+    lb = b.stride(0) * b.element_size() if rb > 1 else wb
+    gap = b.data_ptr() - a.data_ptr()
+    if gap >= (ra - 1) * la + wa or -gap >= (rb - 1) * lb + wb:
+        return False
+    ld = max(la if ra > 1 else 0, lb if rb > 1 else 0)
+    if (ra > 1 and la != ld) or (rb > 1 and lb != ld) or ld == 0:
+        return True
+    off = gap % ld
+    return off < wa or off + wb > ld
 
 
 def _ld(t: Tensor, rows: int, width: int) -> int:

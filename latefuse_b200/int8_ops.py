@@ -16,11 +16,13 @@ the ``lf_*`` declarations in ``include/latefuse_b200.h``).
 
 from __future__ import annotations
 
+import math
+
 import torch
 from torch import Tensor
 
 from latefuse_b200 import _native as nat
-from latefuse_b200.encoder_ops import ACT_GELU, ACT_NONE
+from latefuse_b200.encoder_ops import ACT_GELU, ACT_NONE, _share_memory
 
 _MAX_K = 131072
 
@@ -54,7 +56,18 @@ class Int8Rows:
     __slots__ = ("q", "scale", "shape", "dtype", "ld")
 
     def __init__(self, q: Tensor, scale: Tensor, shape: tuple, dtype: torch.dtype):
-        self.q, self.scale, self.shape, self.dtype, self.ld = q, scale, tuple(shape), dtype, q.stride(0)
+        if q.dim() != 2 or q.dtype != torch.int8 or (q.shape[1] > 1 and q.stride(1) != 1):
+            raise ValueError(f"int8 rows (M, K) are needed, got {q.dtype} {tuple(q.shape)}, strides {q.stride()}")
+        m, k = q.shape
+        if scale.shape != (m,) or scale.dtype != torch.float32 or scale.device != q.device or not scale.is_contiguous():
+            raise ValueError(f"scale must be a contiguous ({m},) float32 tensor on {q.device}")
+        if not shape or shape[-1] != k or math.prod(shape[:-1]) != m:
+            raise ValueError(f"shape {tuple(shape)} is not {m} rows of {k}")
+        self._set(q, scale, tuple(shape), dtype, q.stride(0) if m > 1 else _padded(k))
+
+    def _set(self, q: Tensor, scale: Tensor, shape: tuple, dtype: torch.dtype, ld: int) -> Int8Rows:
+        self.q, self.scale, self.shape, self.dtype, self.ld = q, scale, shape, dtype, ld
+        return self
 
     def dequantize(self) -> Tensor:
         """The values the integers stand for, in ``shape`` and ``dtype``."""
@@ -103,7 +116,7 @@ def quantize_rows(x: Tensor) -> Int8Rows:
     scale = torch.empty(m, dtype=torch.float32, device=dev)
     nat.call(nat.lib().lf_quantize_rows, "lf_quantize_rows", dev, nat.dtype_code(x.dtype), x2.data_ptr(), ldx, m, k,
              q.data_ptr(), kp, scale.data_ptr())
-    return Int8Rows(q if kp == k else q[:, :k], scale, x.shape, x.dtype)
+    return Int8Rows.__new__(Int8Rows)._set(q if kp == k else q[:, :k], scale, x.shape, x.dtype, kp)
 
 
 def _bias(bias: Tensor | None, n: int, dtype: torch.dtype) -> Tensor | None:
@@ -143,6 +156,8 @@ def linear_int8(x: Tensor | Int8Rows, weight: Int8Weight, bias: Tensor | None = 
         if out.dtype != dtype or o2.shape[0] != m or o2.data_ptr() != out.data_ptr() or ldo < n or \
                 (n > 1 and o2.stride(1) != 1) or (out.dim() > 2 and not out.is_contiguous()):
             raise ValueError(f"out must be ({m}, {n}) {dtype} rows viewable without a copy")
+        if _share_memory(o2, x.q if rows else x2):
+            raise ValueError("out must not overlap x")
         ret = out
     code, b = nat.dtype_code(dtype), nat.ptr(bias)
     if rows:
@@ -181,7 +196,7 @@ def add_layernorm_int8(a: Tensor, b: Tensor | None, weight: Tensor, bias: Tensor
     nat.call(nat.lib().lf_add_layernorm_int8, "lf_add_layernorm_int8", dev, nat.dtype_code(dtype), a2.data_ptr(), lda,
              nat.ptr(b2), ldb, w.data_ptr(), bb.data_ptr(), float(eps), m, H, out.data_ptr(), H, q.data_ptr(), hp,
              scale.data_ptr())
-    return out, Int8Rows(q if hp == H else q[:, :H], scale, a.shape, dtype)
+    return out, Int8Rows.__new__(Int8Rows)._set(q if hp == H else q[:, :H], scale, a.shape, dtype, hp)
 
 
 def _same_rows(a: Tensor, b: Tensor | None) -> None:

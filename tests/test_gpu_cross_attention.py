@@ -269,3 +269,14 @@ def test_refusals(cuda):
         cross_attention_varlen(odd, q, q, batch, 2)
     with pytest.raises(nat.NativeLibraryError, match="CUDA tensors"):
         cross_attention_varlen(q.cpu(), q, q, batch, 2)
+
+
+def test_outputs_over_their_inputs_are_refused(cuda):
+    fused = torch.randn(6, 512, device=cuda, dtype=torch.bfloat16)
+    q, k, v, free = fused.split(128, dim=1)
+    batch = cross_batch([2, 4], [3, 3], cuda)
+    for taken in (q, k, v, fused[:, 64:192]):
+        with pytest.raises(ValueError, match="overlap"):
+            cross_attention_varlen(q, k, v, batch, 2, out=taken)
+    want = cross_attention_varlen(q, k, v, batch, 2)
+    assert torch.equal(cross_attention_varlen(q, k, v, batch, 2, out=free), want)

@@ -291,7 +291,7 @@ def test_ffn_int8_is_its_parts(cuda, dtype, m):
 def test_capture_replay_and_streams(cuda):
     """Captured calls replay on new inputs; two streams run their calls at once."""
     wt = Int8Weight(*weight(cuda, 520, 264, 1))
-    for m in (5, 3000):
+    for m in (5, 40, 3000):
         xs = [activations(cuda, m, 264, torch.bfloat16, s) for s in range(4)]
         want = [linear_int8(x, wt, act=ACT_GELU) for x in xs]
         static = xs[0].clone()
@@ -348,3 +348,17 @@ def test_refusals(cuda):
     assert isinstance(rows, Int8Rows)
     with pytest.raises(ValueError, match="columns"):
         linear_int8(rows, Int8Weight(*weight(cuda, 32, 48, 1)))
+
+
+@pytest.mark.parametrize("m", [4, 40])
+def test_outputs_over_their_inputs_are_refused(cuda, m):
+    fused = torch.randn(m, 96, device=cuda, dtype=torch.bfloat16)
+    wt = Int8Weight(*weight(cuda, 32, 64, 1))
+    x = fused[:, :64]
+    with pytest.raises(ValueError, match="overlap"):
+        linear_int8(x, wt, out=fused[:, 40:72])
+    want = linear_int8(x, wt)
+    assert torch.equal(linear_int8(x, wt, out=fused[:, 64:]), want)  # its own columns of the same rows
+    rows = quantize_rows(torch.randn(m, 64, device=cuda, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="overlap"):
+        linear_int8(rows, wt, out=rows.q.view(torch.bfloat16))

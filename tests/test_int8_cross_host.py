@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import latefuse_b200 as lf
-from latefuse_b200 import _native as nat, int8_ops
+from latefuse_b200 import _native as nat, encoder_ops, int8_ops
 from latefuse_b200._build import build
 
 INVALID, UNSUPPORTED, WORKSPACE = 1, 2, 4
@@ -181,3 +181,29 @@ def test_int8_weight_layout_and_refusals():
         lf.linear_int8(torch.ones(2, 37), w)
     with pytest.raises(nat.NativeLibraryError, match="CUDA tensors"):
         lf.cross_attention_varlen(torch.ones(2, 64), torch.ones(2, 64), torch.ones(2, 64), lf.cross_batch([2], [2], "cpu"), 1)
+
+
+def test_int8_rows_refusals():
+    q, s = torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6)
+    rows = lf.Int8Rows(q, s, (2, 3, 32), torch.bfloat16)
+    assert rows.ld == 32 and rows.dequantize().shape == (2, 3, 32)
+    assert lf.Int8Rows(q[:1, :20], s[:1], (20,), torch.float16).ld == 32  # a single row's stride is its own, padded
+    for bad in ((q.float(), s, (6, 32)), (q[0], s, (6, 32)), (q.t(), torch.zeros(32), (32, 6)), (q, s[:5], (6, 32)),
+                (q, torch.zeros(12)[::2], (6, 32)), (q, s.double(), (6, 32)), (q, s, (5, 32)), (q, s, (6, 31)), (q, s, ())):
+        with pytest.raises(ValueError):
+            lf.Int8Rows(*bad, torch.bfloat16)
+
+
+def test_shared_memory_is_found():
+    """Every pair of column and row ranges of one buffer, against the sets of their elements;
+    ranges of other row strides count as shared when they lie within each other."""
+    buf = torch.arange(7 * 12, dtype=torch.int16).reshape(7, 12)
+    views = [buf[a:b, c:d] for a, b in ((0, 7), (0, 3), (3, 7), (2, 3)) for c, d in ((0, 12), (0, 4), (4, 12), (3, 5), (2, 2))]
+    for x in views:
+        for y in views:
+            shared = bool(set(x.flatten().tolist()) & set(y.flatten().tolist()))
+            assert encoder_ops._share_memory(x, y) == shared, (x.shape, y.shape)
+    flat = buf.flatten()
+    assert encoder_ops._share_memory(flat[:20].view(2, 10), flat[10:34].view(3, 8))
+    assert not encoder_ops._share_memory(flat[:20].view(2, 10), flat[20:44].view(3, 8))
+    assert not encoder_ops._share_memory(buf, buf.clone())
