@@ -107,6 +107,16 @@ def test_long_keys_and_a_moving_max(cuda, heads, kv_heads, d, q):
     run(cuda, q, [2048, 2047, 130], heads, kv_heads, d, torch.float16, gap=1)
 
 
+@pytest.mark.parametrize("heads,d", [(16, 64), (8, 128)])
+@pytest.mark.parametrize("seqs", [1, 5, 8, 12, 20])
+def test_single_tokens_of_many_sequences(cuda, seqs, heads, d):
+    """As many sequences and heads as it takes for the keys to be split in eight, four, two or
+    not at all (few against many CTAs), of ragged lengths around 900."""
+    kv = [900 - 37 * (i % 7) for i in range(seqs)]
+    run(cuda, [1] * seqs, kv, heads, heads // 2, d, torch.bfloat16)
+    run(cuda, [2, 1] * (seqs // 2) + [1] * (seqs % 2), kv, heads, heads, d, torch.float16, growth=1.0)
+
+
 def test_many_units(cuda):
     """More units than SMs: every CTA walks several, with other group's tiles in between."""
     gen = torch.Generator().manual_seed(3)
