@@ -411,7 +411,8 @@ constexpr int kThreads = 128 * (1 + kGroups);
 // Registers: the producer / MMA warpgroup gives up what the softmax warpgroups take, so
 // that a row's 128 scores stay in registers (128 x 88 + 256 x 208 = 384 x 168, the launch's).
 constexpr int kRegsIssue = 88, kRegsSoftmax = 208;
-constexpr float kMaxSlack = 8.f;  // log2 units the running max may lag a tile's max
+constexpr float kMaxSlack = 8.f;    // log2 units the running max may lag a tile's max
+constexpr float kSumSlack = 256.f;  // 2^kMaxSlack
 
 template <int kD>
 struct Shape {
@@ -809,54 +810,66 @@ __global__ void __launch_bounds__(kThreads, 1) cross_prompt_kernel(const __grid_
           for (int q = 0; q < kKeys; ++q)
             if (q >= nvalid) s[q] = __float_as_uint(-INFINITY);
         }
-        float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int q = 0; q < 64; q += 2)
-          mxs[(q >> 1) & 3] = max3(mxs[(q >> 1) & 3], __uint_as_float(s[q]), __uint_as_float(s[q + 1]));
-        if (wide) {
-#pragma unroll
-          for (int q = 64; q < kKeys; q += 2)
-            mxs[(q >> 1) & 3] = max3(mxs[(q >> 1) & 3], __uint_as_float(s[q]), __uint_as_float(s[q + 1]));
-        }
-        // the scale is positive: max commutes with it
-        const float mx = max3(fmaxf(mxs[0], mxs[1]), mxs[2], mxs[3]) * sl2.x;
-        m_new = (j == 0 || mx > m + kMaxSlack) ? mx : m;
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;  // every score so far is -inf: p = 0
-        alpha = (j == 0) ? 1.f : sfu_ex2(m - m_use);
-        if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {  // O moves to the new maximum
-          go = wwait(bar(PV_DONE), (t & 1) ^ 1);
-          if (go) {
-            tc_fence_after();
+        // The running maximum only moves when a tile's exceeds it by kMaxSlack, so after the
+        // unit's first tile the exponentials start from it at once; no exponential is above
+        // 2^kMaxSlack unless their sum is, and a warp that finds a row's so takes the maximum and
+        // starts again (long prompts 158 -> 149 us).
+        bool exact = j == 0 || __any_sync(0xffffffffu, m == -INFINITY);
+        float2 sums[2];
 #pragma unroll 1
-            for (int b = 0; b < 2 * Sh::kBlocks; ++b) {
-              uint32_t ov[32];
-              tmem_ld32(o_addr + b * 32, ov);
+        while (true) {
+          if (exact) {
+            float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-              for (int q = 0; q < 32; ++q) ov[q] = __float_as_uint(__uint_as_float(ov[q]) * alpha);
-              tmem_st32(o_addr + b * 32, ov);
+            for (int q = 0; q < 64; q += 2)
+              mxs[(q >> 1) & 3] = max3(mxs[(q >> 1) & 3], __uint_as_float(s[q]), __uint_as_float(s[q + 1]));
+            if (wide) {
+#pragma unroll
+              for (int q = 64; q < kKeys; q += 2)
+                mxs[(q >> 1) & 3] = max3(mxs[(q >> 1) & 3], __uint_as_float(s[q]), __uint_as_float(s[q + 1]));
+            }
+            // the scale is positive: max commutes with it
+            const float mx = max3(fmaxf(mxs[0], mxs[1]), mxs[2], mxs[3]) * sl2.x;
+            m_new = (j == 0 || mx > m + kMaxSlack) ? mx : m;
+            alpha = (j == 0) ? 1.f : sfu_ex2(m - (m_new == -INFINITY ? 0.f : m_new));
+            if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {  // O moves to the new maximum
+              go = wwait(bar(PV_DONE), (t & 1) ^ 1);
+              if (go) {
+                tc_fence_after();
+#pragma unroll 1
+                for (int b = 0; b < 2 * Sh::kBlocks; ++b) {
+                  uint32_t ov[32];
+                  tmem_ld32(o_addr + b * 32, ov);
+#pragma unroll
+                  for (int q = 0; q < 32; ++q) ov[q] = __float_as_uint(__uint_as_float(ov[q]) * alpha);
+                  tmem_st32(o_addr + b * 32, ov);
+                }
+              }
             }
           }
-        }
-        // p = 2^(s - max), rounded to T, two keys a column
-        float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        const float2 neg_m = f2(-m_use);
+          // p = 2^(s - max), rounded to T, two keys a column; every score so far -inf: p = 0
+          const float2 neg_m = f2(m_new == -INFINITY ? 0.f : -m_new);
+          sums[0] = sums[1] = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int hh = 0; hh < kKeys / 64; ++hh) {
-          if (hh == 0 || wide) {
-            uint32_t w[32];
+          for (int hh = 0; hh < kKeys / 64; ++hh) {
+            if (hh == 0 || wide) {
+              uint32_t w[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int col = hh * 64 + 2 * i;
-              const float2 x = f2_fma(make_float2(__uint_as_float(s[col]), __uint_as_float(s[col + 1])), sl2, neg_m);
-              const float2 pr = make_float2(sfu_ex2(x.x), sfu_ex2(x.y));
-              sums[i & 1] = f2_add(sums[i & 1], pr);
-              w[i] = Pack2<T>::pack(pr.x, pr.y);
+              for (int i = 0; i < 32; ++i) {
+                const int col = hh * 64 + 2 * i;
+                const float2 x = f2_fma(make_float2(__uint_as_float(s[col]), __uint_as_float(s[col + 1])), sl2, neg_m);
+                const float2 pr = make_float2(sfu_ex2(x.x), sfu_ex2(x.y));
+                sums[i & 1] = f2_add(sums[i & 1], pr);
+                w[i] = Pack2<T>::pack(pr.x, pr.y);
+              }
+              if (hh == 0) go = wwait(bar(PV_DONE), (t & 1) ^ 1);
+              if (go) tmem_st32(p_addr + hh * 32, w);
             }
-            if (hh == 0) go = wwait(bar(PV_DONE), (t & 1) ^ 1);
-            if (go) tmem_st32(p_addr + hh * 32, w);
           }
+          sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+          if (exact || !__any_sync(0xffffffffu, sum > kSumSlack)) break;
+          exact = true;
         }
-        sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
       } else {
         go = work && wwait(bar(PV_DONE), (t & 1) ^ 1);
       }
