@@ -127,6 +127,34 @@ struct QuantChunk {
       for (int i = 0; i < int(sizeof(T)) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(e)[i];
     }
   }
+  // VEC's elements of a 16-bit row of any alignment: pairs where they are aligned, and the two
+  // single elements around them where the row starts between pairs.
+  __device__ __forceinline__ void load_near(const T* row, int32_t base, int lane, int32_t cols) {
+    static_assert(VEC && sizeof(T) == 2, "16-bit neighbours");
+    const int32_t col = base + lane * 8;
+    const uint16_t* at = reinterpret_cast<const uint16_t*>(row + col);
+    uint32_t u[4] = {0u, 0u, 0u, 0u};
+    if (col + 8 <= cols) {
+      if ((reinterpret_cast<uintptr_t>(row) & 2u) == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = __ldg(reinterpret_cast<const uint32_t*>(at) + i);
+      } else {
+        const uint32_t first = __ldg(at), last = __ldg(at + 7);
+        uint32_t m[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) m[i] = __ldg(reinterpret_cast<const uint32_t*>(at + 1) + i);
+        u[0] = first | (m[0] << 16);
+        u[1] = __funnelshift_r(m[0], m[1], 16);
+        u[2] = __funnelshift_r(m[1], m[2], 16);
+        u[3] = (m[2] >> 16) | (last << 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < cols) u[i >> 1] |= uint32_t(__ldg(at + i)) << (16 * (i & 1));
+    }
+    w[0] = make_uint4(u[0], u[1], u[2], u[3]);
+  }
   // eight values, rounded to T
   __device__ __forceinline__ void set(const float (&v)[8]) {
 #pragma unroll
@@ -176,7 +204,13 @@ struct QuantChunk {
     const uint2 q = steps(rq);
     if constexpr (VEC) {
       const int32_t col = base + lane * 8;
-      if (col < cols) *reinterpret_cast<uint2*>(row + col) = q;
+      if (col + 8 <= cols) {
+        *reinterpret_cast<uint2*>(row + col) = q;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (col + i < cols) row[col + i] = int8_t((i < 4 ? q.x >> (8 * i) : q.y >> (8 * (i - 4))) & 0xffu);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {

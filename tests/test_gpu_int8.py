@@ -83,6 +83,26 @@ def test_quantize_rows_is_the_definition(cuda, dtype, m, k):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [1, 9, 256, 1023, 9001])
+def test_quantize_rows_of_any_stride_and_alignment(cuda, dtype, k):
+    """x from even and odd columns of a wider buffer; q with rows of any stride and alignment,
+    whose bytes around them stay as they were."""
+    wide = activations(cuda, 21, k + 5, dtype, 3)
+    for first in (0, 1, 2, 3):
+        x = wide[:, first:first + k]
+        want = quantize_rows(x.contiguous())
+        rows = quantize_rows(x)
+        assert torch.equal(rows.q, want.q) and torch.equal(rows.scale, want.scale)
+        q = torch.full((21, k + 6), 99, dtype=torch.int8, device=cuda)
+        scale = torch.empty(21, device=cuda)
+        part = q[:, 3:3 + k]
+        nat.call(nat.lib().lf_quantize_rows, "lf_quantize_rows", x.device, nat.dtype_code(dtype), x.data_ptr(),
+                 x.stride(0), 21, k, part.data_ptr(), q.stride(0), scale.data_ptr())
+        assert torch.equal(part, want.q) and torch.equal(scale, want.scale)
+        assert (q[:, :3] == 99).all() and (q[:, 3 + k:] == 99).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_quantize_rows_ties_and_ends(cuda, dtype):
     """Rows whose largest value is 254 steps make every second integer a tie (to even);
     magnitudes at both ends of the type; strided and misaligned rows."""
