@@ -274,6 +274,23 @@ def packed_mean(h: Tensor, pb: PackedBatch) -> Tensor:
     return acc.to(h.dtype) / counts.unsqueeze(1)
 
 
+def _weight_state(*weights: Tensor) -> tuple:
+    """What changes when a weight is replaced, moved or edited in place (inference tensors
+    count no edits)."""
+    return tuple((id(w), w.data_ptr(), None if w.is_inference() else w._version) for w in weights)
+
+
+def _quantized(weight: Tensor, old: Int8Weight | None) -> Int8Weight:
+    """``weight`` in 8-bit integers, in ``old``'s memory where that fits: a captured forward
+    reads it by its address."""
+    new = Int8Weight.from_float(weight)
+    if old is None or old.shape != new.shape or old.q.device != new.q.device:
+        return new
+    old.q.copy_(new.q)
+    old.scale.copy_(new.scale)
+    return old
+
+
 class _Layer(nn.Module):
     def __init__(self, H: int, I: int, eps: float):
         super().__init__()
@@ -342,6 +359,8 @@ class EncoderWithLora(nn.Module):
         self.native_ffn_down = False
         #: the layers' FFN weights in 8-bit integers (:meth:`quantize_ffn`)
         self._ffn8: list[tuple[Int8Weight, Int8Weight]] | None = None
+        #: what each layer's pair was made from (:func:`_weight_state`)
+        self._ffn8_of: list[tuple] = []
         targets = serving_config.target_modules
         self._qkv_targets = [(m, _QKV.index(m)) for m in targets if m in _QKV]
         self._dense_target = "dense" in targets
@@ -433,10 +452,28 @@ class EncoderWithLora(nn.Module):
         LoRA delta) in 8-bit integers: weights with a scale per output channel, quantised
         here, activations with a scale per token (:mod:`latefuse_b200.int8_ops`).  The
         attention projections and their deltas stay in the model's dtype.  Call it once the
-        model is on its GPU, and again if FFN weights change; ``False`` goes back to the
-        model's own weights, which are kept."""
-        self._ffn8 = [(Int8Weight.from_float(layer.wi), Int8Weight.from_float(layer.wo2))
-                      for layer in self.layers] if enabled else None
+        model is on its GPU.  A layer whose FFN weights have changed or moved since is
+        quantised again by the next forward (call it again before a capture, and after edits
+        through ``.data`` or of inference tensors, which torch does not count); ``False``
+        goes back to the model's own weights, which are kept."""
+        if not enabled:
+            self._ffn8, self._ffn8_of = None, []
+            return
+        old = self._ffn8 or [(None, None)] * len(self.layers)
+        of = [_weight_state(layer.wi, layer.wo2) for layer in self.layers]
+        self._ffn8 = [(_quantized(layer.wi, up), _quantized(layer.wo2, down)) for layer, (up, down) in zip(self.layers, old)]
+        self._ffn8_of = of
+
+    def _ffn8_weights(self, idx: int) -> tuple[Int8Weight, Int8Weight]:
+        layer = self.layers[idx]
+        state = _weight_state(layer.wi, layer.wo2)
+        if self._ffn8_of[idx] != state:
+            if layer.wi.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"layer {idx}'s FFN weights have changed since quantize_ffn(): call it before the capture")
+            up, down = self._ffn8[idx]
+            self._ffn8[idx] = _quantized(layer.wi, up), _quantized(layer.wo2, down)
+            self._ffn8_of[idx] = state
+        return self._ffn8[idx]
 
     # -- forward -------------------------------------------------------------
     def position_ids(self, input_ids: Tensor) -> Tensor:
@@ -539,7 +576,7 @@ class EncoderWithLora(nn.Module):
         in 8-bit integers."""
         layer = self.layers[idx]
         if self._ffn8 is not None:
-            return self._ffn_int8(layer, self._ffn8[idx], ao, h)
+            return self._ffn_int8(layer, self._ffn8_weights(idx), ao, h)
         h1 = add_layernorm(ao, h, layer.ln1.weight, layer.ln1.bias, self.eps)
         if self._native_gelu and self._gemm_ok(h1.dtype, layer.wi.shape):
             mid = linear(h1, layer.wi, layer.bi, act=ACT_GELU)
