@@ -92,7 +92,16 @@ def cross_batch(q_lengths, kv_lengths, device, q_starts=None, kv_starts=None) ->
     ``kv_lengths[s]`` rows of encoder states (either may be 0).  Rows lie packed one
     sequence after the other unless ``q_starts`` / ``kv_starts`` name the first row of
     each: several sequences may share a range of states (beams of one text), query
-    ranges may not overlap."""
+    ranges may not overlap.  ``kv_lengths`` may be the :class:`PackedBatch` whose states are
+    read: sequence s then reads those of its input row s, which lie in packed order, not in
+    the rows' own."""
+    if isinstance(kv_lengths, PackedBatch):
+        if kv_starts is not None:
+            raise ValueError("a packed batch says where its rows lie: kv_starts cannot be given too")
+        lens = np.asarray(kv_lengths.lengths, dtype=np.int64)
+        kv_starts, olens = np.empty_like(lens), lens[kv_lengths.order]
+        kv_starts[kv_lengths.order] = np.cumsum(olens) - olens
+        kv_lengths = lens
     ql, kl = np.asarray(q_lengths, dtype=np.int64), np.asarray(kv_lengths, dtype=np.int64)
     if ql.ndim != 1 or ql.shape != kl.shape:
         raise ValueError(f"one query and one key length per sequence are needed, got {ql.shape} and {kl.shape}")
