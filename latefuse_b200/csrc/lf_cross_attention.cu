@@ -57,7 +57,7 @@ struct alignas(64) CrossParams {
   int32_t n_heads, n_kv_heads, group, d;
   const int4* items;   // two per record: {q_start, q_len, kv_start, kv_len}, {q_tile, 0, 0, 0}
   int32_t n_items;
-  int32_t max_q;       // decode: no record's q_len is above it
+  int32_t max_q;       // no record's q_len is above it
   int32_t row_blocks;  // decode: CTAs that share a key head's query rows
   int32_t split;       // decode: CTAs of the cluster that share a sequence's keys
   float scale_log2;    // scale * log2(e)
@@ -66,8 +66,8 @@ struct alignas(64) CrossParams {
   int32_t* status;
 };
 
-// A record, checked against the tensors: one that names rows outside them, or a tile past
-// its queries, is reported and stores nothing.
+// A record, checked against the tensors and the call: one that names rows outside them, more
+// queries than max_q, or a tile past its queries, is reported and stores nothing.
 struct Rec {
   int q0, nq, k0, nk, tile;
   bool ok;
@@ -75,7 +75,7 @@ struct Rec {
 __device__ __forceinline__ Rec read_rec(const CrossParams& p, int i) {
   const int4 a = __ldg(p.items + 2 * i), b = __ldg(p.items + 2 * i + 1);
   Rec r{a.x, a.y, a.z, a.w, b.x, true};
-  r.ok = r.q0 >= 0 && r.nq >= 0 && int64_t(r.q0) + r.nq <= p.n_q && r.k0 >= 0 && r.nk >= 0 &&
+  r.ok = r.q0 >= 0 && r.nq >= 0 && r.nq <= p.max_q && int64_t(r.q0) + r.nq <= p.n_q && r.k0 >= 0 && r.nk >= 0 &&
          int64_t(r.k0) + r.nk <= p.n_kv && r.tile >= 0 && (r.nq == 0 ? r.tile == 0 : int64_t(r.tile) * 128 < r.nq);
   return r;
 }
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) cross_decode_kernel(const _
 
   const Rec rec = read_rec(p, unit / p.n_kv_heads);
   // the cluster's CTAs share the record, so they leave together
-  if (!rec.ok || rec.tile != 0 || rec.nq > p.max_q) {
+  if (!rec.ok || rec.tile != 0) {
     if (tid == 0) set_status(p.status, LF_STATUS_BAD_SEGMENT);
     return;
   }
