@@ -564,8 +564,18 @@ int lf_attention_varlen(void* stream, int dtype, const void* qkv, int64_t ld_qkv
  * (they choose the kernel and how keys are split; max_q at most 128 promises that every
  * q_tile is 0).  A record outside [0, n_q) or [0, n_kv), or past max_q, sets
  * LF_STATUS_BAD_SEGMENT and stores nothing.  It allocates nothing and launches one
- * kernel; a row's bits depend on max_q, max_kv and the number of records (through the
- * choice of kernel and split), never on timing. */
+ * kernel.  total_kv, the sum of kv_len over the records, chooses the kernel and the split
+ * too; it changes no result beyond their rounding.  A row's bits depend on max_q, max_kv,
+ * total_kv, the number of records and of heads, and head_dim (through that choice), never
+ * on timing or on the rows that no record names.  lf_cross_attention_varlen is the same
+ * with total_kv = n_kv, which it is where the keys lie packed, each read by one record;
+ * where records share keys or k and v have rows that none reads, the other entry chooses
+ * better. */
+int lf_cross_attention_varlen_total(void* stream, int dtype, const void* q, int64_t ldq, int64_t n_q,
+                                    const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t n_kv,
+                                    int n_heads, int n_kv_heads, int head_dim, const int32_t* items, int n_items,
+                                    int max_q, int max_kv, int64_t total_kv, float scale, void* out, int64_t ld_out,
+                                    int32_t* status);
 int lf_cross_attention_varlen(void* stream, int dtype, const void* q, int64_t ldq, int64_t n_q,
                               const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t n_kv,
                               int n_heads, int n_kv_heads, int head_dim, const int32_t* items, int n_items,

@@ -131,6 +131,9 @@ SIGNATURES: dict[str, tuple] = {
     "lf_attention_varlen": (c_int, [
         c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int,
         c_void_p, c_int, ctypes.c_float, c_void_p, c_int64, c_void_p]),
+    "lf_cross_attention_varlen_total": (c_int, [
+        c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int,
+        c_int, c_void_p, c_int, c_int, c_int, c_int64, ctypes.c_float, c_void_p, c_int64, c_void_p]),
     "lf_cross_attention_varlen": (c_int, [
         c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int,
         c_int, c_void_p, c_int, c_int, c_int, ctypes.c_float, c_void_p, c_int64, c_void_p]),

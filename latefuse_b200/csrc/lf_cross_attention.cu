@@ -978,11 +978,11 @@ int launch_prompt(const CrossParams& p, int dev, cudaStream_t s) {
 
 using namespace lf;
 
-extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q, int64_t ldq, int64_t n_q,
-                                         const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t n_kv,
-                                         int n_heads, int n_kv_heads, int head_dim, const int32_t* items, int n_items,
-                                         int max_q, int max_kv, float scale, void* out, int64_t ld_out,
-                                         int32_t* status) {
+extern "C" int lf_cross_attention_varlen_total(void* stream, int dtype, const void* q, int64_t ldq, int64_t n_q,
+                                               const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t n_kv,
+                                               int n_heads, int n_kv_heads, int head_dim, const int32_t* items,
+                                               int n_items, int max_q, int max_kv, int64_t total_kv, float scale,
+                                               void* out, int64_t ld_out, int32_t* status) {
   const char* fn = "lf_cross_attention_varlen";
   if (dtype != LF_DTYPE_BF16 && dtype != LF_DTYPE_F16)
     return set_error(LF_ERR_UNSUPPORTED, "%s: dtype %d (bf16 or f16 only)", fn, dtype);
@@ -990,7 +990,8 @@ extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q,
     return set_error(LF_ERR_UNSUPPORTED, "%s: head_dim %d (a multiple of 8 up to 128)", fn, head_dim);
   if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0)
     return set_error(LF_ERR_INVALID, "%s: %d heads over %d key heads", fn, n_heads, n_kv_heads);
-  if (n_q < 0 || n_kv < 0 || n_q > INT32_MAX - 128 || n_kv > INT32_MAX - 128 || n_items < 0 || max_q < 0 || max_kv < 0)
+  if (n_q < 0 || n_kv < 0 || n_q > INT32_MAX - 128 || n_kv > INT32_MAX - 128 || n_items < 0 || max_q < 0 || max_kv < 0 ||
+      total_kv < 0)
     return set_error(LF_ERR_INVALID, "%s: bad sizes", fn);
   if (!(scale > 0.f) || !std::isfinite(scale)) return set_error(LF_ERR_INVALID, "%s: scale must be positive and finite", fn);
   if (n_items == 0 || n_q == 0 || max_q == 0) return LF_OK;
@@ -1027,8 +1028,8 @@ extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == LF_DTYPE_BF16;
   // Which kernel, and in how many parts the few-row kernel takes a sequence's keys: by their
-  // times in us as measured on this GPU (launch aside), keys a sequence by their mean, the
-  // longest sequence from the start on (the records' order).
+  // times in us as measured on this GPU (launch aside), keys a sequence by their mean over the
+  // records, the longest sequence from the start on (the records' order).
   // A few-row CTA takes 10.5 ns a key (64 columns; 13 at 128) alone and 20.5 with every place
   // taken (four or two an SM), between them by the square of the share taken, and 3 us beside
   // its keys, of which the first CTA's pass within the launch; clusters of four find nine
@@ -1044,7 +1045,7 @@ extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q,
   // and 43.
   const int64_t blocks = (int64_t(max_q) * p.group + kDecodeRows - 1) / kDecodeRows;
   const int64_t units = int64_t(n_items) * n_kv_heads;
-  const int64_t mean_kv = n_kv / n_items < max_kv ? n_kv / n_items : max_kv;
+  const int64_t mean_kv = total_kv / n_items < max_kv ? total_kv / n_items : max_kv;
   const bool narrow = head_dim <= 64;
   const double alone = narrow ? 0.0105 : 0.013, full = 0.0205, places = double(sms) * (narrow ? 4.0 : 2.0);
   int split = 1;
@@ -1083,4 +1084,13 @@ extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q,
   if ((rc = encode_rows(&p.v_map, dtype, vb, n_kv > 0 ? ldv : ldq, kv_rows, n_kv_heads, head_dim, key_tile, "v"))) return rc;
   if (narrow) return bf ? launch_prompt<__nv_bfloat16, 64>(p, dev, s) : launch_prompt<__half, 64>(p, dev, s);
   return bf ? launch_prompt<__nv_bfloat16, 128>(p, dev, s) : launch_prompt<__half, 128>(p, dev, s);
+}
+
+extern "C" int lf_cross_attention_varlen(void* stream, int dtype, const void* q, int64_t ldq, int64_t n_q,
+                                         const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t n_kv,
+                                         int n_heads, int n_kv_heads, int head_dim, const int32_t* items, int n_items,
+                                         int max_q, int max_kv, float scale, void* out, int64_t ld_out,
+                                         int32_t* status) {
+  return lf_cross_attention_varlen_total(stream, dtype, q, ldq, n_q, k, ldk, v, ldv, n_kv, n_heads, n_kv_heads, head_dim,
+                                         items, n_items, max_q, max_kv, n_kv < 0 ? 0 : n_kv, scale, out, ld_out, status);
 }

@@ -138,10 +138,11 @@ def cross_attention_varlen(q: Tensor, k: Tensor, v: Tensor, batch: CrossBatch, n
         raise ValueError(f"out must be a ({tq}, {width}) {dtype} tensor with contiguous rows")
     elif _share_memory(out, q) or _share_memory(out, k) or _share_memory(out, v):
         raise ValueError("out must not overlap q, k or v")
-    nat.call(nat.lib().lf_cross_attention_varlen, "lf_cross_attention_varlen", dev, nat.dtype_code(dtype), q.data_ptr(),
+    total_kv = batch.n_kv if batch.total_kv is None else batch.total_kv
+    nat.call(nat.lib().lf_cross_attention_varlen_total, "lf_cross_attention_varlen", dev, nat.dtype_code(dtype), q.data_ptr(),
              _ld(q, tq, width), tq, k.data_ptr(), _ld(k, tk, wk), v.data_ptr(), _ld(v, tk, wk), tk, n_heads, n_kv_heads, d,
-             items.data_ptr(), items.shape[0], batch.max_q, batch.max_kv, d ** -0.5 if scale is None else float(scale),
-             out.data_ptr(), _ld(out, tq, width), nat.ptr(status))
+             items.data_ptr(), items.shape[0], batch.max_q, batch.max_kv, total_kv,
+             d ** -0.5 if scale is None else float(scale), out.data_ptr(), _ld(out, tq, width), nat.ptr(status))
     return out
 
 

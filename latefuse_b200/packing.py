@@ -85,6 +85,7 @@ class CrossBatch:
     max_q: int
     max_kv: int
     items: Tensor     # (n, 8) int32 {q_start, q_len, kv_start, kv_len, q_tile, 0, 0, 0}, most work first
+    total_kv: int | None = None  # keys of all records, shared ones counted for each (None: as many as n_kv)
 
 
 def cross_batch(q_lengths, kv_lengths, device, q_starts=None, kv_starts=None) -> CrossBatch:
@@ -131,7 +132,8 @@ def cross_batch(q_lengths, kv_lengths, device, q_starts=None, kv_starts=None) ->
     if device.type == "cuda":
         host = host.pin_memory()
     return CrossBatch(n_seqs=int(ql.size), n_q=n_q, n_kv=n_kv, max_q=int(ql.max()) if ql.size else 0,
-                      max_kv=int(kl.max()) if kl.size else 0, items=host.to(device, non_blocking=True))
+                      max_kv=int(kl.max()) if kl.size else 0, items=host.to(device, non_blocking=True),
+                      total_kv=int((kl[order] * reps).sum()))
 
 
 def pack_rows(input_ids: Tensor, lengths: list[int], slots: list[int], position_pad: int | None,
