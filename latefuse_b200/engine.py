@@ -74,9 +74,14 @@ class _DeltaRunner:
         need = workspace_bytes(dtype, n_tokens, self.config.lora_rank, n_modules)
         if self._ws is None or self._ws.numel() < need or self._ws.device != device:
             self._ws = torch.empty(max(need, 256), dtype=torch.uint8, device=device)
+        self.status_word(device)
+        return self._ws
+
+    def status_word(self, device) -> Tensor:
+        """The word on ``device`` in which kernels report bad records and timeouts."""
         if self.status is None or self.status.device != device:
             self.status = torch.zeros(1, dtype=torch.int32, device=device)
-        return self._ws
+        return self.status
 
     @staticmethod
     def layerwise_cache(layer_w: LayerwiseBatchedWeights, module: str) -> FactorCache:
@@ -594,11 +599,14 @@ class EncoderWithLora(nn.Module):
 
     def _ffn_int8(self, layer: _Layer, weights: tuple[Int8Weight, Int8Weight], ao: Tensor, h: Tensor | None) -> Tensor:
         up, down = weights
+        status = self._runner.status_word(ao.device)
         if self._native_gelu:
-            h1, o = ffn_int8(ao, h, layer.ln1.weight, layer.ln1.bias, self.eps, up, layer.bi, down, layer.bo2)
+            h1, o = ffn_int8(ao, h, layer.ln1.weight, layer.ln1.bias, self.eps, up, layer.bi, down, layer.bo2,
+                             status=status)
         else:
             h1, rows = add_layernorm_int8(ao, h, layer.ln1.weight, layer.ln1.bias, self.eps)
-            o = linear_int8(self.act(linear_int8(rows, up, layer.bi)), down, layer.bo2)
+            mid = self.act(linear_int8(rows, up, layer.bi, status=status))
+            o = linear_int8(mid, down, layer.bo2, status=status)
         return add_layernorm(o, h1, layer.ln2.weight, layer.ln2.bias, self.eps, out=o)
 
     def _transposed(self, w: Tensor) -> Tensor | None:
@@ -661,8 +669,7 @@ class EncoderWithLora(nn.Module):
         """
         T = pb.n_tokens
         H, nh, hd = self.config.hidden_size, self.num_heads, self.head_dim
-        if self._runner.status is None or self._runner.status.device != pb.ids.device:
-            self._runner.status = torch.zeros(1, dtype=torch.int32, device=pb.ids.device)
+        self._runner.status_word(pb.ids.device)
         if H % 8 == 0 and H <= 4096:  # gathers, both adds and the LayerNorm in one launch
             h = embed_layernorm(pb.ids, pb.positions, pb.token_types, self.word_embeddings.weight,
                                 self.position_embeddings.weight, self.token_type_embeddings.weight,

@@ -130,13 +130,15 @@ def _bias(bias: Tensor | None, n: int, dtype: torch.dtype) -> Tensor | None:
 
 
 def linear_int8(x: Tensor | Int8Rows, weight: Int8Weight, bias: Tensor | None = None, act: int = ACT_NONE,
-                out: Tensor | None = None) -> Tensor:
+                out: Tensor | None = None, status: Tensor | None = None) -> Tensor:
     """``act(x @ weight.T + bias)`` in 8-bit integers: ``x (..., K)`` f32, bf16 or f16, quantised
     per row first, or :class:`Int8Rows`; ``act`` is ``ACT_NONE`` or ``ACT_GELU`` (the exact erf
     GELU).  The result has x's dtype and is rounded to it once.  Any M, N and K up to 131,072;
-    ``out`` must be viewable as rows without a copy and must not overlap ``x``."""
+    ``out`` must be viewable as rows without a copy and must not overlap ``x``.  A wait that
+    runs out sets ``LF_STATUS_TIMEOUT`` in ``status`` (an int32 on the GPU), where one is given,
+    and leaves the result unwritten."""
     rows = type(x) is Int8Rows
-    dev = nat.require_cuda(x.q if rows else x, weight.q, bias, out)
+    dev = nat.require_cuda(x.q if rows else x, weight.q, bias, out, status)
     n, k = weight.shape
     shape, dtype = x.shape, x.dtype
     if shape[-1] != k:
@@ -162,12 +164,14 @@ def linear_int8(x: Tensor | Int8Rows, weight: Int8Weight, bias: Tensor | None = 
     code, b = nat.dtype_code(dtype), nat.ptr(bias)
     if rows:
         nat.call(nat.lib().lf_linear_int8, "lf_linear_int8", dev, code, x.q.data_ptr(), x.ld, x.scale.data_ptr(),
-                 weight.q.data_ptr(), weight.ld, weight.scale.data_ptr(), b, out.data_ptr(), ldo, m, n, k, int(act), None)
+                 weight.q.data_ptr(), weight.ld, weight.scale.data_ptr(), b, out.data_ptr(), ldo, m, n, k, int(act),
+                 nat.ptr(status))
     else:
         size = _rows_bytes(m, k)
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         nat.call(nat.lib().lf_linear_rows_int8, "lf_linear_rows_int8", dev, code, x2.data_ptr(), ldx, weight.q.data_ptr(),
-                 weight.ld, weight.scale.data_ptr(), b, out.data_ptr(), ldo, m, n, k, int(act), nat.ptr(ws), size, None)
+                 weight.ld, weight.scale.data_ptr(), b, out.data_ptr(), ldo, m, n, k, int(act), nat.ptr(ws), size,
+                 nat.ptr(status))
     return ret
 
 
@@ -206,12 +210,12 @@ def _same_rows(a: Tensor, b: Tensor | None) -> None:
 
 def ffn_int8(a: Tensor, residual: Tensor | None, ln_weight: Tensor, ln_bias: Tensor, eps: float, up: Int8Weight,
              up_bias: Tensor | None, down: Int8Weight, down_bias: Tensor | None,
-             act: int = ACT_GELU) -> tuple[Tensor, Tensor]:
+             act: int = ACT_GELU, status: Tensor | None = None) -> tuple[Tensor, Tensor]:
     """The encoder layer's feed-forward half with both projections in 8-bit integers:
     ``h = layer_norm(a + residual)`` and ``o = down(act(up(h)))``, the middle activations
     rounded to a's dtype and then quantised per token.  Returns ``(h, o)``: the layer's
-    output is ``add_layernorm(o, h, ...)``."""
-    dev = nat.require_cuda(a, residual, ln_weight, ln_bias, up.q, up_bias, down.q, down_bias)
+    output is ``add_layernorm(o, h, ...)``.  ``status`` as for :func:`linear_int8`."""
+    dev = nat.require_cuda(a, residual, ln_weight, ln_bias, up.q, up_bias, down.q, down_bias, status)
     inner, hidden = up.shape
     dtype = a.dtype
     if a.shape[-1] != hidden or down.shape != (hidden, inner):
@@ -230,5 +234,5 @@ def ffn_int8(a: Tensor, residual: Tensor | None, ln_weight: Tensor, ln_bias: Ten
     nat.call(lib.lf_ffn_int8, "lf_ffn_int8", dev, code, a2.data_ptr(), lda, nat.ptr(r2), ldr, w.data_ptr(), bb.data_ptr(),
              float(eps), up.q.data_ptr(), up.ld, up.scale.data_ptr(), nat.ptr(ub), down.q.data_ptr(), down.ld,
              down.scale.data_ptr(), nat.ptr(db), m, hidden, inner, int(act), h.data_ptr(), hidden, o.data_ptr(), hidden,
-             ws.data_ptr(), size, None)
+             ws.data_ptr(), size, nat.ptr(status))
     return (h, o) if a.dim() == 2 else (h.view(a.shape), o.view(a.shape))
