@@ -444,7 +444,8 @@ int lf_linear_lora_shrink(void* stream, int dtype, const void* x, int64_t ldx, c
  * everything computed from it is NaN.  x is f32, bf16 or f16 with any row stride and
  * alignment; q has row stride ldq >= cols (bytes; a multiple of 16 with a 16-byte
  * aligned base for lf_linear_int8); bytes of q's rows past cols are not written.  Used
- * for activations (a row per token) and for weights (a row per output channel). */
+ * for activations (a row per token) and for weights (a row per output channel).  cols up
+ * to 2^31 - 4097 (LF_ERR_UNSUPPORTED above). */
 int lf_quantize_rows(void* stream, int dtype, const void* x, int64_t ldx, int64_t n_rows, int cols,
                      int8_t* q, int64_t ldq, float* scale);
 

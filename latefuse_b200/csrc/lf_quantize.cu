@@ -21,6 +21,9 @@ namespace lf {
 namespace {
 
 constexpr int kThreads = 256;
+// Column numbers are 32-bit, and a chunk past the row's end is formed before it is found empty:
+// 8 warps' chunks of 256, and a lane's eight columns.
+constexpr int kMaxCols = INT32_MAX - 4096;
 
 struct QuantParams {
   const void* x;
@@ -130,6 +133,8 @@ extern "C" int lf_quantize_rows(void* stream, int dtype, const void* x, int64_t 
   if (dtype != LF_DTYPE_BF16 && dtype != LF_DTYPE_F16 && dtype != LF_DTYPE_F32)
     return set_error(LF_ERR_INVALID, "lf_quantize_rows: unknown dtype %d", dtype);
   if (n_rows < 0 || cols <= 0) return set_error(LF_ERR_INVALID, "lf_quantize_rows: %lld rows of %d", (long long)n_rows, cols);
+  if (cols > kMaxCols)
+    return set_error(LF_ERR_UNSUPPORTED, "lf_quantize_rows: rows of %d above %d elements", cols, kMaxCols);
   if (n_rows == 0) return LF_OK;
   if (x == nullptr || q == nullptr || scale == nullptr)
     return set_error(LF_ERR_INVALID, "lf_quantize_rows: null x, q or scale");

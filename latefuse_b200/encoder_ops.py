@@ -120,11 +120,11 @@ def cross_attention_varlen(q: Tensor, k: Tensor, v: Tensor, batch: CrossBatch, n
     left as they were (undefined when ``out`` is None); ``out`` must not overlap q, k or v.
     Returns ``out (Tq, n_heads * d)``."""
     items, dtype = batch.items, q.dtype
-    dev = nat.require_cuda(q, k, v, items, out, status)
     n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
     tq, width = q.shape
-    if n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads or width % n_heads:
+    if n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads or width % n_heads or width >= 2**31:
         raise ValueError(f"{width} columns of {n_heads} heads over {n_kv_heads} key heads")
+    dev = nat.require_cuda(q, k, v, items, out, status)
     d = width // n_heads
     tk, wk = k.shape
     if v.shape != k.shape or wk != n_kv_heads * d or k.dtype != dtype or v.dtype != dtype:

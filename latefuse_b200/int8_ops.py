@@ -25,6 +25,8 @@ from latefuse_b200 import _native as nat
 from latefuse_b200.encoder_ops import ACT_GELU, ACT_NONE, _share_memory
 
 _MAX_K = 131072
+_MAX_N = 2**31 - 257
+_MAX_COLS = 2**31 - 1 - 4096  # lf_quantize_rows'
 
 
 def _padded(n: int) -> int:
@@ -89,8 +91,8 @@ class Int8Weight:
         if scale.shape != q.shape[:1] or scale.dtype != torch.float32 or scale.device != q.device:
             raise ValueError(f"scale must be a ({q.shape[0]},) float32 tensor on {q.device}")
         n, k = q.shape
-        if not 1 <= k <= _MAX_K or n < 1:
-            raise ValueError(f"weight of {n} x {k}: K must be in 1..{_MAX_K}")
+        if not 1 <= k <= _MAX_K or not 1 <= n <= _MAX_N:
+            raise ValueError(f"weight of {n} x {k}: K must be in 1..{_MAX_K}, N in 1..{_MAX_N}")
         if (k > 1 and q.stride(1) != 1) or q.data_ptr() % 16 or q.stride(0) % 16 or q.stride(0) < k:
             q = torch.empty(n, _padded(k), dtype=torch.int8, device=q.device)[:, :k].copy_(q)
         self.q, self.scale, self.shape, self.ld = q, scale.contiguous(), (n, k), q.stride(0)
@@ -106,9 +108,9 @@ class Int8Weight:
 def quantize_rows(x: Tensor) -> Int8Rows:
     """The rows (last dimension) of an f32, bf16 or f16 tensor in 8-bit integers with a scale
     each.  A row of zeros has scale 0; a row holding an infinity or NaN has scale NaN."""
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= _MAX_COLS:
+        raise ValueError(f"rows of 1 to {_MAX_COLS} elements are needed, got {tuple(x.shape)}")
     dev = nat.require_cuda(x)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"rows of at least one element are needed, got {tuple(x.shape)}")
     x2, ldx = _rows(x)
     m, k = x2.shape
     kp = _padded(k)
@@ -187,8 +189,10 @@ def _ffn_bytes(size: int, m: int, hidden: int, inner: int) -> int:
 
 def add_layernorm_int8(a: Tensor, b: Tensor | None, weight: Tensor, bias: Tensor, eps: float) -> tuple[Tensor, Int8Rows]:
     """``add_layernorm(a, b, weight, bias, eps)`` and its rows in 8-bit integers, in one pass."""
-    dev = nat.require_cuda(a, b, weight, bias)
     H, dtype = a.shape[-1], a.dtype
+    if H >= 2**31:
+        raise ValueError(f"rows of {H} elements")
+    dev = nat.require_cuda(a, b, weight, bias)
     _same_rows(a, b)
     a2, lda = _rows(a)
     b2, ldb = _rows(b) if b is not None else (None, 0)
