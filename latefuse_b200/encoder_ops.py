@@ -118,8 +118,12 @@ def cross_attention_varlen(q: Tensor, k: Tensor, v: Tensor, batch: CrossBatch, n
     share a key head (``n_kv_heads`` None: as many as ``n_heads``); ``scale`` positive, None:
     ``d ** -0.5``.  A sequence without keys gives zeros; rows of ``out`` in no sequence are
     left as they were (undefined when ``out`` is None); ``out`` must not overlap q, k or v.
+    A record that names rows outside the tensors, or a wait that runs out, is reported in
+    ``status`` (an int32 on the GPU) alone, and leaves its rows so too.
     Returns ``out (Tq, n_heads * d)``."""
     items, dtype = batch.items, q.dtype
+    if items.dtype != torch.int32 or items.dim() != 2 or items.shape[1] != 8 or not items.is_contiguous():
+        raise ValueError("items must be a contiguous (n, 8) int32 tensor (CrossBatch.items)")
     n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
     tq, width = q.shape
     if n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads or width % n_heads or width >= 2**31:
