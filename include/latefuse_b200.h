@@ -455,14 +455,15 @@ int lf_quantize_rows(void* stream, int dtype, const void* x, int64_t ldx, int64_
  * f16).  The integer sum is exact; scaling, bias and activation are f32, rounded to
  * dtype once (unlike lf_linear, which rounds before the GELU too).  Any m, n >= 1 and
  * 1 <= k <= 131072; x and w need 16-byte aligned rows, y and bias any alignment
- * (y rows that are 16-byte aligned are written faster).  x, w and y must not overlap. */
+ * (y rows that are 16-byte aligned are written faster).  y must overlap none of the
+ * inputs: x, w, their scales and the bias. */
 int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t ldx, const float* x_scale,
                    const int8_t* w, int64_t ldw, const float* w_scale, const void* bias,
                    void* y, int64_t ldy, int64_t m, int n, int k, int act, int32_t* status);
 
 /* lf_quantize_rows of x (m, k) into the workspace, then lf_linear_int8: the 8-bit projection
  * of float rows in one call of two launches; up to 16 rows of up to 4,096, 16,384 elements in all, take one launch
- * and no workspace (0 bytes).  x and y must not overlap.  The workspace (256-byte aligned, at least
+ * and no workspace (0 bytes).  y must overlap none of the inputs.  The workspace (256-byte aligned, at least
  * lf_linear_rows_int8_workspace_bytes) is free again when the launches have run, so calls
  * that may overlap on the GPU need one each. */
 size_t lf_linear_rows_int8_workspace_bytes(int64_t m, int k);

@@ -136,7 +136,7 @@ def linear_int8(x: Tensor | Int8Rows, weight: Int8Weight, bias: Tensor | None = 
     """``act(x @ weight.T + bias)`` in 8-bit integers: ``x (..., K)`` f32, bf16 or f16, quantised
     per row first, or :class:`Int8Rows`; ``act`` is ``ACT_NONE`` or ``ACT_GELU`` (the exact erf
     GELU).  The result has x's dtype and is rounded to it once.  Any M, N and K up to 131,072;
-    ``out`` must be viewable as rows without a copy and must not overlap ``x``.  A wait that
+    ``out`` must be viewable as rows without a copy and must overlap none of the inputs.  A wait that
     runs out sets ``LF_STATUS_TIMEOUT`` in ``status`` (an int32 on the GPU), where one is given,
     and leaves the result unwritten."""
     rows = type(x) is Int8Rows
@@ -160,8 +160,10 @@ def linear_int8(x: Tensor | Int8Rows, weight: Int8Weight, bias: Tensor | None = 
         if out.dtype != dtype or o2.shape[0] != m or o2.data_ptr() != out.data_ptr() or ldo < n or \
                 (n > 1 and o2.stride(1) != 1) or (out.dim() > 2 and not out.is_contiguous()):
             raise ValueError(f"out must be ({m}, {n}) {dtype} rows viewable without a copy")
-        if _share_memory(o2, x.q if rows else x2):
-            raise ValueError("out must not overlap x")
+        inputs = [x.q, x.scale] if rows else [x2]
+        for t in (*inputs, weight.q, weight.scale, *([] if bias is None else [bias])):
+            if _share_memory(o2, t if t.dim() == 2 else t.view(1, -1)):
+                raise ValueError("out must not overlap x, the weight, the scales or the bias")
         ret = out
     code, b = nat.dtype_code(dtype), nat.ptr(bias)
     if rows:
