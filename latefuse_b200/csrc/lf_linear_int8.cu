@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
     fence_mbar_init();
     prefetch_tmap(&p.x_map);
     prefetch_tmap(&p.w_map);
-    prefetch_tmap(&p.y_map);
+    if (p.tma_out) prefetch_tmap(&p.y_map);  // no map is made of other rows
   }
   if (warp == 1) {
     __syncwarp();
