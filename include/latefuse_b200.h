@@ -453,8 +453,9 @@ int lf_quantize_rows(void* stream, int dtype, const void* x, int64_t ldx, int64_
  * per row, int8 w (n, k) with a scale per output channel (both as lf_quantize_rows
  * writes them) and bias (n entries in dtype, or NULL); y (m, n) in dtype (f32, bf16 or
  * f16).  The integer sum is exact; scaling, bias and activation are f32, rounded to
- * dtype once (unlike lf_linear, which rounds before the GELU too).  Any m, n >= 1 and
- * 1 <= k <= 131072; x and w need 16-byte aligned rows, y and bias any alignment
+ * dtype once (unlike lf_linear, which rounds before the GELU too).  For bf16 and f16 the
+ * GELU is a fit within 2^-17 of |v| Phi(-|v|) up to |v| = 5 (past it within 4% of less than
+ * 1.5e-6).  Any m, n >= 1 and 1 <= k <= 131072; x and w need 16-byte aligned rows, y and bias any alignment
  * (y rows that are 16-byte aligned are written faster).  y must overlap none of the
  * inputs: x, w, their scales and the bias. */
 int lf_linear_int8(void* stream, int dtype, const int8_t* x, int64_t ldx, const float* x_scale,

@@ -90,40 +90,37 @@ __host__ __device__ constexpr uint32_t umma_idesc_i8(uint32_t m, uint32_t n) {
 
 __device__ __forceinline__ bool aborted(const int32_t* f) { return *reinterpret_cast<const volatile int32_t*>(f) != 0; }
 
-// The exact GELU of two values for a 16-bit result, v max(0, sign v) - |v| Phi(-|v|) with
+// The GELU of two values for a 16-bit result, v max(0, sign v) - |v| Phi(-|v|) with
 //     Phi(-z) = exp(-z^2 / 2) R(z),  R(z) = erfcx(z / sqrt 2) / 2,
-// R as a polynomial in min(z, 5) - 5/2 whose largest relative error is least: degree 8 for
-// bf16 (2^-13.0 of Phi(-z)), degree 10 for f16 (2^-16.8); beyond 5, where R is held, Phi
-// is below 3e-7 and still falls with the exponential.  One SFU operation a value where
-// gelu2_fast takes two: with K = 1024 the epilogue's GELU sets the projection's time
-// (17,410 x 4,096: 92 us with gelu2_fast, 62 to 68 with this, 57 without an activation).
+// R as a polynomial in min(z, 5) - 5/2 whose largest relative error is least: degree 11 for
+// bf16 (2^-18.8 of R), degree 12 for f16 (2^-20.7).  With the roundings of its evaluation
+// (2^-19.7 at most) and of the exponent (2^-19) |v| Phi(-|v|) is within 2^-17.4 (bf16) and
+// 2^-17.9 (f16) of its value, within 2^-18.4 and 2^-19.6 for |v| up to 2; beyond 5, where R is
+// held, it is below 1.5e-6, still falls with the exponential and is within 3.7%.  So
+// results are the formula's but where it lies next to a border between two 16-bit values:
+// 0.016% of normal inputs round the other way in bf16 and 0.033% in f16, where the formula
+// in f32 has 0.002% and 0.014% (degrees 8 and 10 had 0.9% and 0.5%).
+// One SFU operation a value where gelu2_fast takes two: with K = 1024 the epilogue's GELU
+// sets the projection's time (17,410 x 4,096, bf16 and f16: 76 and 77 us; 67 and 73 with
+// degrees 8 and 10, 54 without an activation).
 template <typename T>
 __device__ __forceinline__ float2 gelu2_narrow(float2 v) {
+  constexpr bool kBf16 = DT<T>::umma_fmt == 1;
+  constexpr int kDegree = kBf16 ? 11 : 12;
+  constexpr float kR[2][13] = {
+      {1.1876396754928464e-08f, -6.810693520264977e-08f, 1.1003712074852956e-07f, -3.798999443915818e-07f,
+       3.342534455441637e-06f, -1.5777091903146356e-05f, 6.238623609533533e-05f, -0.0002551310753915459f,
+       0.0010172546608373523f, -0.0038328650407493114f, 0.0136485006660223f, -0.04561358690261841f,
+       0.14133130013942719f},
+      {-5.840812988822108e-08f, 3.262648817781155e-07f, -5.428102554105863e-07f, 1.8756209101411514e-06f,
+       -1.4787478903599549e-05f, 6.693375325994566e-05f, -0.0002577411360107362f, 0.0010109581053256989f,
+       -0.003830085974186659f, 0.013651634566485882f, -0.04561440274119377f, 0.14133106172084808f}};
   const float2 z = make_float2(fminf(fabsf(v.x), 5.f), fminf(fabsf(v.y), 5.f));
   const float2 l = f2_mul(f2_mul(v, f2(-0.72134752044448170f)), v);  // -v^2 / 2 to base 2
   const float2 u = f2_add(z, f2(-2.5f));
-  float2 r;
-  if constexpr (DT<T>::umma_fmt == 1) {  // bf16
-    r = f2_fma(u, f2(5.790445356979035e-06f), f2(-2.9506778446375392e-05f));
-    r = f2_fma(r, u, f2(5.341164069250226e-05f));
-    r = f2_fma(r, u, f2(-0.00018099445151165128f));
-    r = f2_fma(r, u, f2(0.0010193546768277884f));
-    r = f2_fma(r, u, f2(-0.003963787574321032f));
-    r = f2_fma(r, u, f2(0.013666416518390179f));
-    r = f2_fma(r, u, f2(-0.04555509611964226f));
-    r = f2_fma(r, u, f2(0.14132584631443024f));
-  } else {
-    r = f2_fma(u, f2(2.788294750644127e-07f), f2(-1.515155076958763e-06f));
-    r = f2_fma(r, u, f2(2.5983151772379642e-06f));
-    r = f2_fma(r, u, f2(-8.94710683496669e-06f));
-    r = f2_fma(r, u, f2(6.310718163149431e-05f));
-    r = f2_fma(r, u, f2(-0.0002729224506765604f));
-    r = f2_fma(r, u, f2(0.0010191438486799598f));
-    r = f2_fma(r, u, f2(-0.003814229043200612f));
-    r = f2_fma(r, u, f2(0.013645598664879799f));
-    r = f2_fma(r, u, f2(-0.0456189326941967f));
-    r = f2_fma(r, u, f2(0.141331747174263f));
-  }
+  float2 r = f2(kR[kBf16][0]);
+#pragma unroll
+  for (int i = 1; i <= kDegree; ++i) r = f2_fma(r, u, f2(kR[kBf16][i]));
   const float2 h = f2_mul(r, make_float2(-sfu_ex2(l.x), -sfu_ex2(l.y)));
   return f2_fma(z, h, make_float2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f)));
 }
