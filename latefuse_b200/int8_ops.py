@@ -140,7 +140,7 @@ def linear_int8(x: Tensor | Int8Rows, weight: Int8Weight, bias: Tensor | None = 
     once.  Any M, N and K up to 131,072;
     ``out`` must be viewable as rows without a copy and must overlap none of the inputs.  A wait that
     runs out sets ``LF_STATUS_TIMEOUT`` in ``status`` (an int32 on the GPU), where one is given,
-    and leaves the result unwritten."""
+    and leaves the result undefined."""
     rows = type(x) is Int8Rows
     dev = nat.require_cuda(x.q if rows else x, weight.q, bias, out, status)
     n, k = weight.shape
