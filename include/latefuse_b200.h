@@ -555,7 +555,8 @@ int lf_attention_varlen(void* stream, int dtype, const void* qkv, int64_t ld_qkv
 /* Cross attention of packed sequences: for sequence s, query row i and head h
  *     out[i][h] = softmax_j(scale * q_i[h] . k_j[h / group]) @ v[h / group]
  * over the sequence's own keys j, group = n_heads / n_kv_heads (query heads that share a
- * key head).  A sequence without keys gives rows of zeros.  q and out rows hold n_heads
+ * key head).  A sequence without keys gives rows of zeros, and so do scores that are all
+ * -infinity (over finite values).  q and out rows hold n_heads
  * heads of head_dim elements side by side, k and v rows n_kv_heads; each of the four has
  * its own row stride (elements; columns of a fused projection are fine).  head_dim is a
  * multiple of 8 up to 128; dtype bf16 or f16; scale positive; statistics and sums in f32.

@@ -116,10 +116,10 @@ def cross_attention_varlen(q: Tensor, k: Tensor, v: Tensor, batch: CrossBatch, n
     rows of any stride that is a multiple of 8 (column slices of a fused projection are
     fine); d a multiple of 8 up to 128; consecutive ``n_heads / n_kv_heads`` query heads
     share a key head (``n_kv_heads`` None: as many as ``n_heads``); ``scale`` positive, None:
-    ``d ** -0.5``.  A sequence without keys gives zeros; rows of ``out`` in no sequence are
-    left as they were (undefined when ``out`` is None); ``out`` must not overlap q, k or v.
-    A record that names rows outside the tensors, or a wait that runs out, is reported in
-    ``status`` (an int32 on the GPU) alone, and leaves its rows so too.
+    ``d ** -0.5``.  A sequence without keys, or whose scores are all -infinity (over finite
+    values), gives zeros; rows of ``out`` in no sequence are left as they were (undefined when
+    ``out`` is None); ``out`` must not overlap q, k or v.  A record that names rows outside the
+    tensors, or a wait that runs out, is reported in ``status`` (an int32 on the GPU) alone.
     Returns ``out (Tq, n_heads * d)``."""
     items, dtype = batch.items, q.dtype
     if items.dtype != torch.int32 or items.dim() != 2 or items.shape[1] != 8 or not items.is_contiguous():

@@ -36,3 +36,17 @@ def test_a_record_past_max_q_stores_nothing(cuda, seqs, q_len, kv_len, heads):
         q0 = s * q_len + (s > 1)
         rows, keys = slice(q0, q0 + q_len), slice(s * kv_len, (s + 1) * kv_len)
         check_sequence(out[rows], q[rows], k[keys], v[keys], heads, heads, 0.125)
+
+
+@pytest.mark.parametrize("d", [64, 80])
+@pytest.mark.parametrize("seqs,q_len,kv_len,heads", [(3, 1, 200, 2), (3, 20, 2000, 2), (64, 128, 100, 16), (3, 140, 300, 2)])
+def test_scores_that_are_all_minus_infinity_give_zeros(cuda, seqs, q_len, kv_len, heads, d):
+    g = torch.Generator(device=cuda).manual_seed(seqs + d)
+    q = torch.randn(seqs * q_len, heads * d, device=cuda, generator=g).abs().add(0.5).bfloat16()
+    k, v = torch.randn(2, seqs * kv_len, heads * d, device=cuda, generator=g).bfloat16()
+    k[kv_len:2 * kv_len] = float("-inf")
+    out = cross_attention_varlen(q, k, v, cross_batch([q_len] * seqs, [kv_len] * seqs, cuda), heads)
+    assert (out[q_len:2 * q_len] == 0).all()
+    for s in (0, seqs - 1):
+        rows, keys = slice(s * q_len, (s + 1) * q_len), slice(s * kv_len, (s + 1) * kv_len)
+        check_sequence(out[rows], q[rows], k[keys], v[keys], heads, heads, d ** -0.5)

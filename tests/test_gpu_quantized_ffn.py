@@ -57,7 +57,7 @@ def test_a_capture_wants_them_quantised_before(cuda):
         scale(model)
         with pytest.raises(RuntimeError, match="before the capture"):
             with torch.cuda.graph(torch.cuda.CUDAGraph()):
-                model._ffn(1, ao, h)
+                model._ffn(1, ao + 1, h)
         got = model._ffn(1, ao, h)
         assert not torch.equal(got, want)
         graph.replay()  # the captured forward reads the same weights
