@@ -237,8 +237,8 @@ struct TileWalk {
 };
 
 // A staged 32 x 32 block into rows that are not 16-byte aligned, eight rows of 32 columns in
-// flight (17,410 x 1,024 -> 4,095: 117 us one row at a time, 72 so; with GELU 131 and 103).
-// Out of line: inlined it took registers from the aligned epilogue (GELU 71 -> 74 us).
+// flight (17,410 x 1,024 -> 4,095: 117 us one row at a time, 72 so; with GELU 131 and 103, now 111).
+// Out of line: inlined it took registers from the aligned epilogue (GELU 71 -> 74 us then).
 template <typename T>
 __device__ __noinline__ void store_rows(const uint8_t* block, T* dst, int64_t ld, int64_t rows, int32_t cols, int lane) {
   constexpr int kRowBytes = kOutCols * sizeof(T);
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
     }
     __syncwarp();
   } else {
-    // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
+    // ------------------------------------------------------------ epilogue (warps 2..17, both CTAs)
     const int quad = warp & 3;
     const int c0 = ((warp - 2) >> 2) * kWarpCols;  // this warp's columns of the tile
     const uint32_t taddr = tmem + (uint32_t(quad * 32) << 16) + c0;
